@@ -97,7 +97,7 @@ int ks_selftest_bounded_wait(uint64_t limit_ns, void *stream);
 int ks_set_wait_limit_ns(uint64_t limit_ns);
 
 /* ---- shared enums ------------------------------------------------------ */
-typedef enum ks_dtype { KS_BF16 = 0, KS_F32 = 1, KS_F64 = 2 } ks_dtype;
+typedef enum ks_dtype { KS_BF16 = 0, KS_F32 = 1, KS_F64 = 2, KS_F16 = 3 } ks_dtype;
 
 /* Row-op strategy (ElemMode, tools/tune/include/kernscope/tune/
  * elem_common.h:49-55).  ONEPASS: the row is read from HBM once and held in
@@ -248,6 +248,51 @@ int ks_flash_attention_validate(const ks_flash_attention_config *cfg,
                                 char *reason, size_t reason_len);
 int ks_flash_attention_launch(const ks_flash_attention_config *cfg,
                               const ks_flash_attention_args *args, void *stream);
+
+/* ---- linear cross entropy -------------------------------------------------
+ * Softmax cross entropy of a linear layer over a vocabulary, taken in tiles
+ * of the vocabulary; no counterpart in the reference.  With logits
+ * l[r,v] = sum_k h[r,k] w[v,k] (h [tokens, dim], w [vocab, dim], bf16 or
+ * fp16, row strides in elements, the last axis dense; fp32 accumulate):
+ *   lse[r]  = log sum_v exp l[r,v]
+ *   loss[r] = lse[r] - l[r, targets[r]]; 0 where targets[r] == ignore_index;
+ *             NaN where a target is neither that nor in [0, vocab)
+ *   d[r,v]  = g[r] (exp(l[r,v] - lse[r]) - [v == targets[r]])
+ *   dh = d w,  dw = d^T h, rounded once to the inputs' type.
+ * A token that counts is one whose target is not ignore_index.
+ * pass = KS_CE_FORWARD: loss and (if not NULL) lse.
+ *      = KS_CE_BACKWARD: dh and dw from lse; g[r] from dloss.
+ *      = KS_CE_GRAD: loss, lse (if not NULL), dh and dw in one call
+ *        (reduction mean or sum).
+ * reduction: KS_CE_NONE: loss has `tokens` values, dloss too.  KS_CE_MEAN
+ * (over the tokens that count; 0 with zero gradients when none does) and
+ * KS_CE_SUM: loss and dloss have one.  dloss == NULL stands for ones.
+ * g[r] = grad_scale * dloss / (mean: number of tokens that count), and 0 for
+ * the tokens that do not count or whose target is out of range.
+ * The logits are never kept.  The backward pass takes them again in pieces of
+ * the vocabulary, whose d (16 bits a value) live in the workspace.
+ * cfg.tile_m: 0 = chosen from the sizes, 128 = 128 x 128 tiles, 256 = 256 x
+ * 256 tiles.  cfg.piece: vocabulary columns per piece of the backward pass, a
+ * multiple of 256; 0 = as many as the workspace holds.
+ * ks_linear_ce_workspace_bytes() gives the least size that works and the
+ * size that the call makes use of (at most about limit bytes, or `least`
+ * where that is more); the workspace is 256-byte aligned.                    */
+typedef enum ks_ce_pass { KS_CE_FORWARD = 0, KS_CE_BACKWARD = 1, KS_CE_GRAD = 2 } ks_ce_pass;
+typedef enum ks_ce_reduction { KS_CE_NONE = 0, KS_CE_MEAN = 1, KS_CE_SUM = 2 } ks_ce_reduction;
+typedef struct ks_linear_ce_config { int tile_m; int64_t piece; } ks_linear_ce_config;
+typedef struct ks_linear_ce_args {
+  const void *h; const void *w; const int64_t *targets;
+  int64_t tokens; int64_t dim; int64_t vocab; int64_t h_stride; int64_t w_stride;
+  int dtype; int pass; int reduction; float grad_scale; int64_t ignore_index;
+  const float *dloss; float *loss; float *lse;
+  void *dh; void *dw; int64_t dh_stride; int64_t dw_stride;
+  void *workspace; size_t workspace_bytes;
+} ks_linear_ce_args;
+int ks_linear_ce_validate(const ks_linear_ce_config *cfg, const ks_linear_ce_args *args,
+                          char *reason, size_t reason_len);
+int ks_linear_ce_workspace_bytes(const ks_linear_ce_config *cfg, const ks_linear_ce_args *args,
+                                 size_t limit, size_t *least, size_t *bytes);
+int ks_linear_ce_launch(const ks_linear_ce_config *cfg, const ks_linear_ce_args *args, void *stream);
 
 /* ---- roofline peak probes (libs/bench/kernels/peaks.hip, driven by
  * tools/bench/main.cpp: kernscope-bench) ------------------------------------

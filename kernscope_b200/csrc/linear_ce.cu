@@ -1,0 +1,1021 @@
+// linear_ce.cu -- softmax cross entropy of a linear layer over a large
+// vocabulary, with its gradient, on the sm_100a tensor cores.
+//
+//   l = h w^T;  lse[r] = log sum_v exp l[r,v];  loss[r] = lse[r] - l[r,t[r]]
+//   d[r,v] = f[r] (exp(l[r,v] - lse[r]) - [v == t[r]])
+//   dh = d w;  dw = d^T h
+//
+// The logits [tokens, vocab] are never written.  Four GEMM-shaped passes share
+// one persistent kernel (TMA producer warp, one MMA-issuing thread, four
+// epilogue warps; tcgen05.mma kind::f16, fp32 accumulators in TMEM):
+//   STATS  l = h w^T; the epilogue reduces each tile's row to (max, sum of
+//          exponentials) and picks the target's logit out of the accumulator;
+//   PROB   l = h w^T again for one piece of the vocabulary; the epilogue
+//          writes d in 16 bits to the workspace;
+//   DH     dh (+)= d w over the piece's columns (split over K when there are
+//          few tiles; fp32 slabs, added up in a fixed order);
+//   DW     dw rows of the piece = d^T h, complete after one pass over the
+//          tokens, so each is rounded and written once.
+// Operand layouts: h and w K-major in STATS/PROB; d K-major and w MN-major in
+// DH; d MN-major (M = the vocabulary) and h MN-major in DW -- all straight
+// from the row-major tensors, no transpose pass.
+//
+// Rounding: products and sums are fp32; d is rounded to the inputs' type
+// because the tensor cores take 16-bit operands (relative 2^-8 per value in
+// bf16, 2^-11 in fp16, the size of the outputs' own rounding); the common factor
+// grad_scale / count is left out of d and applied to the fp32 accumulator, so
+// that a target's d, near -1, is near a power of two.  fp16 d is stored times
+// 1024, so that probabilities down to 6e-8 stay normal numbers.
+//
+// Every mbarrier wait is bounded (KsWait), as in matmul.cu.
+#include <algorithm>
+#include <cuda_fp16.h>
+
+#include "ks_common.cuh"
+
+namespace {
+
+constexpr int kBM = 128;
+constexpr int kBK = 64;                        // one 128-byte swizzle row of 16-bit values
+constexpr int kUmmaK = 16;
+constexpr int kThreads = 192;                  // producer, MMA, 4 x epilogue
+constexpr uint32_t kABox = kBM * kBK * 2;      // 128 rows x 64 K (or two boxes of 64 K x 64 columns): 16 KB
+constexpr uint32_t kBBox = kBK * 64 * 2;       // 64 K-rows x 64 columns: 8 KB
+constexpr uint32_t kCBuf = 32 * 128;           // one epilogue block: 32 rows x 32 columns, up to 4 bytes each
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kF16Range = 1024.f;            // factor on fp16 d
+
+enum Mode { STATS = 0, PROB = 1, DH = 2, DW = 3 };
+
+// Scalars between the kernels of one call, in the workspace.
+struct CeScalars {
+  float fscale;  // on every row's f: the range factor of d
+  float escale;  // on the accumulators of DH and DW
+  unsigned int counter;
+};
+
+struct CeGemm {
+  int M, N;               // output rows and columns
+  int kb_total;           // K-blocks of 64
+  int splits, kb_split;   // K-splits and K-blocks per split (DH)
+  int group;              // raster: > 0 groups of M-tiles, < 0 bands of N-tiles
+  int b3d;                // MN-major B map is (64 columns, K, blocks)
+  int f16;
+  // STATS / PROB
+  int64_t tokens, vocab;
+  int64_t v0;             // first vocabulary column of the piece (PROB)
+  const int64_t *targets;
+  int64_t ignore;
+  float2 *part;           // [N-tiles][rows_p] (max, sum)
+  float *tlogit;          // [rows_p]
+  int64_t rows_p;
+  const float *lse;
+  const float *dloss;     // per token, or nullptr
+  CeScalars *sc;
+  // DH
+  int out_f32, accumulate;
+};
+
+template <int BN, int STAGES, int ACC, int MH>
+struct Layout {
+  static constexpr uint32_t a_bytes = MH * kABox;
+  static constexpr uint32_t b_bytes = kBK * BN * 2;
+  static constexpr uint32_t a_off = 0;
+  static constexpr uint32_t b_off = a_off + STAGES * a_bytes;
+  static constexpr uint32_t c_off = b_off + STAGES * b_bytes;
+  static constexpr uint32_t bar_off = c_off + 8 * kCBuf;  // 4 warps x 2 buffers
+  static constexpr uint32_t n_bars = 2 * STAGES + ACC + ACC * MH + 1;
+  static constexpr uint32_t misc_off = bar_off + n_bars * 8;
+  static constexpr uint32_t bytes = misc_off + 16;
+  static constexpr uint32_t request = bytes + 1024;  // slack to align the base to 1024
+  static constexpr uint32_t tmem_cols = ACC * BN * MH;
+  static_assert(tmem_cols == 128 || tmem_cols == 256 || tmem_cols == 512, "a power of two of TMEM columns");
+  static_assert(request <= 227 * 1024, "shared memory");
+};
+
+KS_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+KS_DEV uint32_t pack2(float lo, float hi, bool f16) {
+  if (f16) {
+    __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t *>(&v);
+  }
+  return ks_pack_bf16x2(lo, hi);
+}
+
+KS_DEV void tma_reduce_add_2d(const CUtensorMap *m, const void *src, int c0, int c1) {
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(ks_smem_u32(src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// Work item t -> output tile and K-split; splits outermost, tiles rastered as
+// in matmul.cu (group > 0: groups of M-tiles, M fastest; group < 0: bands of
+// N-tiles, N fastest).
+KS_DEV void work_coords(int t, int num_m, int num_n, int group, int &tm, int &tn, int &split) {
+  const int tiles = num_m * num_n;
+  split = t / tiles;
+  t -= split * tiles;
+  if (group < 0) {
+    const int band = -group, size = band * num_m;
+    const int b = t / size, first = b * band, bn = min(num_n - first, band), r = t - b * size;
+    tn = first + r % bn;
+    tm = r / bn;
+  } else {
+    const int size = group * num_n;
+    const int g = t / size, first = g * group, gm = min(num_m - first, group), r = t - g * size;
+    tm = first + r % gm;
+    tn = r / gm;
+  }
+}
+
+template <int MODE, int BN, int STAGES, int ACC, int MH>
+__global__ void __launch_bounds__(kThreads, 1)
+    ce_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
+                   const __grid_constant__ CUtensorMap tma_c, const __grid_constant__ CeGemm p, KsWait wait) {
+  using L = Layout<BN, STAGES, ACC, MH>;
+  constexpr bool kAMn = MODE == DW;                // A is MN-major (d^T)
+  constexpr bool kBMn = MODE == DH || MODE == DW;  // B is MN-major
+  constexpr int kTM = kBM * MH;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = ks_smem_u32(smem_raw);
+  uint8_t *smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::bar_off);
+  uint64_t *full = bars, *empty = bars + STAGES, *tfull = bars + 2 * STAGES;
+  uint64_t *tempty = bars + 2 * STAGES + ACC;  // [acc * MH + half]
+  uint64_t *drain = bars + 2 * STAGES + ACC + ACC * MH;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::misc_off);
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::misc_off + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_m = (p.M + kTM - 1) / kTM, num_n = (p.N + BN - 1) / BN;
+  const int num_work = num_m * num_n * p.splits;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      ks_mbar_init(full + s, 1);
+      ks_mbar_init(empty + s, 1);
+    }
+    for (int a = 0; a < ACC; ++a) ks_mbar_init(tfull + a, 1);
+    for (int a = 0; a < ACC * MH; ++a) ks_mbar_init(tempty + a, 4);
+    ks_mbar_init(drain, 1);
+    *abort = 0;
+    ks_fence_mbar_init();
+    ks_prefetch_tmap(&tma_a);
+    ks_prefetch_tmap(&tma_b);
+    if (MODE != STATS) ks_prefetch_tmap(&tma_c);
+    if (MODE == STATS && blockIdx.x == 0) p.sc->counter = 0;  // for the combine kernel that follows
+  }
+  if (warp == 1) {
+    ks_tmem_alloc(tmem_slot, L::tmem_cols);
+    ks_tmem_relinquish();
+  }
+  ks_tc_fence_before();
+  __syncthreads();
+  ks_tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------ producer
+    int stage = 0;
+    uint32_t phase = 0, armed = 0, armed_parity = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < num_work && ok; t += gridDim.x) {
+      int tm, tn, split;
+      work_coords(t, num_m, num_n, p.group, tm, tn, split);
+      const int kb0 = split * p.kb_split, kb1 = min(kb0 + p.kb_split, p.kb_total);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!ks_mbar_wait(empty + stage, phase ^ 1u, abort, wait)) {
+          ok = false;
+          break;
+        }
+        uint8_t *a_dst = smem + L::a_off + stage * L::a_bytes;
+        uint8_t *b_dst = smem + L::b_off + stage * L::b_bytes;
+        ks_mbar_arrive_expect_tx(full + stage, L::a_bytes + L::b_bytes);
+        if (kAMn)  // boxes of 64 K-rows x 64 columns, one copy for all of them
+          ks_tma_load_3d(a_dst, &tma_a, full + stage, 0, kb * kBK, tm * (kTM / 64));
+        else
+          ks_tma_load_2d(a_dst, &tma_a, full + stage, kb * kBK, tm * kTM);
+        if (!kBMn) {
+          ks_tma_load_2d(b_dst, &tma_b, full + stage, kb * kBK, tn * BN);
+        } else if (p.b3d) {
+          ks_tma_load_3d(b_dst, &tma_b, full + stage, 0, kb * kBK, tn * (BN / 64));
+        } else {
+#pragma unroll
+          for (int j = 0; j < BN / 64; ++j)
+            ks_tma_load_2d(b_dst + j * kBBox, &tma_b, full + stage, tn * BN + j * 64, kb * kBK);
+        }
+        armed |= 1u << stage;
+        armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    // teardown: every load this thread issued must have landed before exit
+    for (int s = 0; s < STAGES; ++s)
+      if (armed & (1u << s)) ks_mbar_wait(full + s, (armed_parity >> s) & 1u, nullptr, wait);
+  } else if (warp == 1 && lane == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    const uint32_t idesc = p.f16 ? (ks_idesc_bf16_f32(kBM, BN, kAMn, kBMn) & ~((7u << 7) | (7u << 10)))  // f16 operands: format 0
+                                 : ks_idesc_bf16_f32(kBM, BN, kAMn, kBMn);
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    int i = 0;
+    auto issue = [&](int st, bool first_kb, uint32_t d_tmem, int h0, int h1) {
+      const uint32_t a_addr = ks_smem_u32(smem + L::a_off + st * L::a_bytes);
+      const uint32_t b_addr = ks_smem_u32(smem + L::b_off + st * L::b_bytes);
+#pragma unroll
+      for (int k = 0; k < kBK / kUmmaK; ++k) {
+        // K-major: 128-byte rows, 8-row groups 1024 bytes apart, 32 bytes per K=16.
+        // MN-major: 64-column boxes kBBox apart (LBO), 8 K-rows 1024 bytes apart (SBO), 2048 bytes per K=16.
+        const uint64_t bdesc = kBMn ? ks_umma_desc_sw128(b_addr + k * 2048, kBBox, 1024)
+                                    : ks_umma_desc_sw128(b_addr + k * 32, 16, 1024);
+#pragma unroll
+        for (int h = 0; h < MH; ++h) {
+          if (h < h0 || h >= h1) continue;
+          const uint64_t adesc = kAMn ? ks_umma_desc_sw128(a_addr + h * kABox + k * 2048, kBBox, 1024)
+                                      : ks_umma_desc_sw128(a_addr + h * kABox + k * 32, 16, 1024);
+          ks_umma_ss(d_tmem + h * BN, adesc, bdesc, idesc, !first_kb || k != 0);
+        }
+      }
+    };
+    for (int t = blockIdx.x; t < num_work && ok; t += gridDim.x, ++i) {
+      int tm, tn, split;
+      work_coords(t, num_m, num_n, p.group, tm, tn, split);
+      const int kb0 = split * p.kb_split, kb1 = min(kb0 + p.kb_split, p.kb_total);
+      const int acc = i % ACC;
+      const uint32_t acc_phase = (i / ACC) & 1;
+      // The epilogue frees the accumulator one 128-row half at a time: half
+      // 0's MMAs start at once, the other half's are deferred over at most
+      // STAGES - 1 K-blocks until it is drained too.
+      if (!ks_mbar_wait(tempty + acc * MH, acc_phase ^ 1u, abort, wait)) break;
+      ks_tc_fence_after();
+      const uint32_t d_tmem = tmem_base + acc * BN * MH;
+      bool rest_free = MH == 1;
+      int pend = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!ks_mbar_wait(full + stage, phase, abort, wait)) {
+          ok = false;
+          break;
+        }
+        ks_tc_fence_after();
+        issue(stage, kb == kb0, d_tmem, 0, 1);
+        if (!rest_free) {
+          if (pend + 1 < STAGES && kb + 1 < kb1 &&
+              !ks_mbar_test_wait(ks_smem_u32(tempty + acc * MH + 1), acc_phase ^ 1u)) {
+            ++pend;
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
+            continue;
+          }
+          for (int h = 1; h < MH && ok; ++h) ok = ks_mbar_wait(tempty + acc * MH + h, acc_phase ^ 1u, abort, wait);
+          if (!ok) break;
+          ks_tc_fence_after();
+          rest_free = true;
+          for (int q = pend; q > 0; --q) {
+            const int sp = (stage + STAGES - q) % STAGES;
+            issue(sp, kb - q == kb0, d_tmem, 1, MH);
+            ks_umma_commit(empty + sp);
+          }
+          pend = 0;
+        }
+        issue(stage, kb == kb0, d_tmem, 1, MH);
+        ks_umma_commit(empty + stage);
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (ok) ks_umma_commit(tfull + acc);
+    }
+    // teardown: all MMAs issued by this thread complete before TMEM is freed
+    ks_umma_commit(drain);
+    ks_mbar_wait(drain, 0, nullptr, wait);
+  } else if (warp >= 2) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;  // TMEM lane quadrant this warp may access
+    uint8_t *stg = smem + L::c_off + (warp - 2) * 2 * kCBuf;
+    const bool f16 = p.f16 != 0;
+    float escale = 1.f, fscale = 1.f;
+    if (MODE == DH || MODE == DW) escale = p.sc->escale;
+    if (MODE == PROB) fscale = p.sc->fscale;
+    int i = 0;
+    uint32_t nstore = 0;
+    for (int t = blockIdx.x; t < num_work; t += gridDim.x, ++i) {
+      const int acc = i % ACC;
+      const uint32_t acc_phase = (i / ACC) & 1;
+      int tm, tn, split;
+      work_coords(t, num_m, num_n, p.group, tm, tn, split);
+      // what this lane's rows need, loaded while the MMAs still run
+      int tcol[MH];       // target column relative to the tile, or one outside it
+      float lse2[MH], f[MH];
+      if (MODE == STATS || MODE == PROB) {
+#pragma unroll
+        for (int h = 0; h < MH; ++h) {
+          const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
+          tcol[h] = -1;
+          lse2[h] = 0.f;
+          f[h] = 0.f;
+          if (row < p.tokens) {
+            const int64_t target = p.targets[row];
+            const bool valid = target != p.ignore && target >= 0 && target < p.vocab;
+            if (valid) {
+              const int64_t c = target - p.v0 - int64_t(tn) * BN;
+              if (c >= 0 && c < BN) tcol[h] = int(c);
+              if (MODE == PROB) f[h] = p.dloss ? p.dloss[row] * fscale : fscale;
+            }
+            if (MODE == PROB) lse2[h] = p.lse[row] * kLog2e;
+          }
+        }
+      }
+      if (!ks_mbar_wait(tfull + acc, acc_phase, abort, wait)) break;
+      ks_tc_fence_after();
+      const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + acc * BN * MH;
+      const int64_t col0 = p.v0 + int64_t(tn) * BN;  // first vocabulary column of the tile (STATS, PROB)
+      float m = -INFINITY, s = 0.f;
+#pragma unroll 1
+      for (int cc = 0; cc < MH * (BN / 32); ++cc) {
+        const int h = cc / (BN / 32);
+        const int cb = (cc % (BN / 32)) * 32;  // first column of the block inside the tile
+        uint32_t r[32];
+        ks_tmem_ld32(t_addr + cc * 32, r);
+        ks_tmem_wait_ld();
+        if ((cc + 1) % (BN / 32) == 0) {  // this half is free for the next tile's MMAs
+          ks_tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ks_mbar_arrive(tempty + acc * MH + h);
+        }
+        if constexpr (MODE == STATS) {
+          const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cb;
+          if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
+            float v = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == tc) v = __uint_as_float(r[j]);
+            if (tc >= 0 && tc < 32) p.tlogit[int64_t(tm) * kTM + h * kBM + q * 32 + lane] = v;
+          }
+          const int64_t left = p.vocab - (col0 + cb);  // columns of the block inside the vocabulary
+          if (left < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j >= left) r[j] = __float_as_uint(-INFINITY);
+          }
+          float cm[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) cm[j] = __uint_as_float(r[j]);
+#pragma unroll
+          for (int j = 4; j < 32; ++j) cm[j & 3] = fmaxf(cm[j & 3], __uint_as_float(r[j]));
+          const float mn = fmaxf(m, fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])));
+          // an all -inf row so far: exponentials against 0 are 0, not NaN
+          const float base = mn == -INFINITY ? 0.f : mn * kLog2e;
+          float a4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) a4[j & 3] += ex2(fmaf(__uint_as_float(r[j]), kLog2e, -base));
+          s = s * ex2(fmaf(m, kLog2e, -base)) + ((a4[0] + a4[1]) + (a4[2] + a4[3]));
+          m = mn;
+          if (cb + 32 == BN) {
+            const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
+            if (row < p.tokens) p.part[int64_t(tn) * p.rows_p + row] = make_float2(m, s);
+            m = -INFINITY;
+            s = 0.f;
+          }
+        } else {
+          uint8_t *buf = stg + (nstore & 1) * kCBuf;
+          if (lane == 0) ks_bulk_wait_read<1>();  // the store two blocks back has read this buffer
+          __syncwarp();
+          if constexpr (MODE == PROB) {
+            const float fr = h == 0 ? f[0] : f[MH - 1];
+            const float l2 = h == 0 ? lse2[0] : lse2[MH - 1];
+            const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cb;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(fr * ex2(fmaf(__uint_as_float(r[j]), kLog2e, -l2)));
+            if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == tc) r[j] = __float_as_uint(__uint_as_float(r[j]) - fr);
+            }
+            const int64_t left = p.vocab - (col0 + cb);
+            if (left < 32 || fr == 0.f) {  // columns past the vocabulary, rows without gradient: zeros, whatever the logits
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j >= left || fr == 0.f) r[j] = 0u;
+            }
+          } else if (MODE == DW || !p.out_f32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
+          }
+          if (MODE == DH && p.out_f32) {
+            // row = lane: eight 16-byte chunks, chunk v at position v ^ (lane & 7) (128-byte swizzle)
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              *reinterpret_cast<uint4 *>(buf + lane * 128 + ((v ^ (lane & 7)) * 16)) =
+                  make_uint4(r[v * 4], r[v * 4 + 1], r[v * 4 + 2], r[v * 4 + 3]);
+          } else {
+            // row = lane: four 16-byte chunks, chunk v at position v ^ ((lane >> 1) & 3) (64-byte swizzle)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint4 w;
+              w.x = pack2(__uint_as_float(r[v * 8 + 0]), __uint_as_float(r[v * 8 + 1]), f16);
+              w.y = pack2(__uint_as_float(r[v * 8 + 2]), __uint_as_float(r[v * 8 + 3]), f16);
+              w.z = pack2(__uint_as_float(r[v * 8 + 4]), __uint_as_float(r[v * 8 + 5]), f16);
+              w.w = pack2(__uint_as_float(r[v * 8 + 6]), __uint_as_float(r[v * 8 + 7]), f16);
+              *reinterpret_cast<uint4 *>(buf + lane * 64 + ((v ^ ((lane >> 1) & 3)) * 16)) = w;
+            }
+          }
+          ks_fence_proxy_async();
+          __syncwarp();
+          const int c0 = tn * BN + cb;
+          const int64_t r0 = int64_t(tm) * kTM + h * kBM + q * 32;
+          if (c0 < p.N && r0 < p.M) {  // blocks past the edge hold nothing
+            if (lane == 0) {
+              if (MODE == DH && p.accumulate)
+                tma_reduce_add_2d(&tma_c, buf, c0, int(split * p.rows_p + r0));
+              else
+                ks_tma_store_2d(&tma_c, buf, c0, int((MODE == DH ? split * p.rows_p : 0) + r0));
+              ks_bulk_commit_group();
+            }
+            ++nstore;
+          }
+        }
+      }
+    }
+    if (MODE != STATS && lane == 0) ks_bulk_wait_all();
+  }
+
+  ks_tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ks_tc_fence_after();
+    ks_tmem_dealloc(tmem_base, L::tmem_cols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// lse and loss of every row from the tiles' (max, sum); the last block adds up
+// the loss over the rows, in a fixed order, and leaves the gradient's scalars.
+// 8 rows x 32 slices of the tiles per block: 64-byte segments of `part`.
+// ---------------------------------------------------------------------------
+constexpr int kCombRows = 8;
+
+__global__ void __launch_bounds__(256)
+    ce_combine_kernel(const float2 *__restrict__ part, int tiles, int64_t rows_p, const float *__restrict__ tlogit,
+                      const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab, int64_t ignore, int reduction,
+                      float grad_scale, const float *dloss, float range, float *__restrict__ loss,
+                      float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc) {
+  __shared__ float sm[8][kCombRows], ss[8][kCombRows];
+  __shared__ double shl[kCombRows], shn[kCombRows];
+  __shared__ bool is_last;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rr = tid & (kCombRows - 1), slice = tid / kCombRows;
+  const int64_t row = int64_t(blockIdx.x) * kCombRows + rr;
+  float m = -INFINITY, s = 0.f;
+  auto add = [&](float m2, float s2) {  // (m, s) (+) (m2, s2); a side with no finite maximum adds its sum as it is
+    const float mn = fmaxf(m, m2);
+    if (mn == -INFINITY) {
+      s += s2;  // zeros, or the NaN of a row that has one
+    } else {
+      s = s * ex2((m - mn) * kLog2e) + s2 * ex2((m2 - mn) * kLog2e);
+    }
+    m = mn;
+  };
+  if (row < tokens)
+    for (int t = slice; t < tiles; t += 256 / kCombRows) {
+      const float2 v = part[int64_t(t) * rows_p + row];
+      add(v.x, v.y);
+    }
+#pragma unroll
+  for (int o = kCombRows; o < 32; o <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    add(m2, s2);
+  }
+  if (lane < kCombRows) {
+    sm[warp][lane] = m;
+    ss[warp][lane] = s;
+  }
+  __syncthreads();
+  if (tid < kCombRows) {
+    m = sm[0][tid];
+    s = ss[0][tid];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) add(sm[w][tid], ss[w][tid]);
+    double l = 0.0, n = 0.0;
+    if (row < tokens) {
+      const float lse = m + logf(s);  // -inf + log 0: a row of -inf logits
+      lse_out[row] = lse;
+      const int64_t t = targets[row];
+      float v = 0.f;
+      if (t != ignore) {
+        v = t >= 0 && t < vocab ? lse - tlogit[row] : __int_as_float(0x7fc00000);
+        n = 1.0;
+      }
+      if (reduction == KS_CE_NONE && loss) loss[row] = v;
+      l = v;
+    }
+    shl[tid] = l;
+    shn[tid] = n;
+  }
+  if (reduction == KS_CE_NONE) return;
+  __syncthreads();
+  if (tid == 0) {
+    double l = 0.0, n = 0.0;
+    for (int j = 0; j < kCombRows; ++j) {
+      l += shl[j];
+      n += shn[j];
+    }
+    sums[blockIdx.x] = make_double2(l, n);
+    __threadfence();
+    is_last = atomicAdd(&sc->counter, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  __shared__ double wl[8], wn[8];
+  double l = 0.0, n = 0.0;
+  for (unsigned j = tid; j < gridDim.x; j += 256) {
+    const double2 v = __ldcg(sums + j);
+    l += v.x;
+    n += v.y;
+  }
+  l = ks_warp_sum_f64(l);
+  n = ks_warp_sum_f64(n);
+  if (lane == 0) {
+    wl[warp] = l;
+    wn[warp] = n;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    l = n = 0.0;
+    for (int j = 0; j < 8; ++j) {
+      l += wl[j];
+      n += wn[j];
+    }
+    const double c = reduction == KS_CE_MEAN ? (n > 0.0 ? n : 1.0) : 1.0;
+    if (loss) loss[0] = float(l / c);
+    sc->fscale = range;
+    sc->escale = float(double(grad_scale) * (dloss ? double(dloss[0]) : 1.0) / c / double(range));
+  }
+}
+
+// Gradient scalars of a backward call: mean and sum count the tokens; with a
+// dloss per token its largest magnitude is taken out of d by a power of two,
+// so that fp16 d keeps its range (one block: a few microseconds at 8192 tokens).
+__global__ void __launch_bounds__(1024)
+    ce_scalars_kernel(const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab, int64_t ignore, int reduction,
+                      float grad_scale, const float *__restrict__ dloss, float range, CeScalars *sc) {
+  __shared__ float shm[32];
+  __shared__ double shn[32];
+  float mx = 0.f;
+  double n = 0.0;
+  for (int64_t r = threadIdx.x; r < tokens; r += 1024) {
+    const int64_t t = targets[r];
+    if (t == ignore) continue;
+    n += 1.0;
+    if (reduction == KS_CE_NONE && dloss && t >= 0 && t < vocab) mx = fmaxf(mx, fabsf(dloss[r]));
+  }
+  mx = ks_warp_max(mx);
+  n = ks_warp_sum_f64(n);
+  if ((threadIdx.x & 31) == 0) {
+    shm[threadIdx.x >> 5] = mx;
+    shn[threadIdx.x >> 5] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  n = 0.0;
+  mx = 0.f;
+  for (int j = 0; j < 32; ++j) {
+    n += shn[j];
+    mx = fmaxf(mx, shm[j]);
+  }
+  double f = range, g = grad_scale;
+  if (reduction == KS_CE_NONE) {
+    if (dloss && mx > 0.f && mx < INFINITY) {
+      int e;
+      frexpf(mx, &e);
+      f = ldexp(double(range), max(-100, min(100, -e)));
+    }
+  } else {
+    if (dloss) g *= double(dloss[0]);
+    if (reduction == KS_CE_MEAN) g /= n > 0.0 ? n : 1.0;
+  }
+  sc->fscale = float(f);
+  sc->escale = float(g / f);
+}
+
+// dh = T(escale * sum of the fp32 slabs), slabs added in order.
+__global__ void __launch_bounds__(256)
+    ce_dh_finish_kernel(const float *__restrict__ slabs, int count, int64_t slab_elems, int64_t ld, int64_t rows,
+                        int64_t cols, const CeScalars *sc, uint16_t *__restrict__ out, int64_t out_stride, int f16,
+                        int vec) {
+  const float e = sc->escale;
+  const int64_t cv = (cols + 3) / 4, total = rows * cv;
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
+    const int64_t r = i / cv, c = (i - r * cv) * 4;
+    float4 a = *reinterpret_cast<const float4 *>(slabs + r * ld + c);
+    for (int k = 1; k < count; ++k) {
+      const float4 b = *reinterpret_cast<const float4 *>(slabs + k * slab_elems + r * ld + c);
+      a.x += b.x;
+      a.y += b.y;
+      a.z += b.z;
+      a.w += b.w;
+    }
+    const uint32_t lo = pack2(a.x * e, a.y * e, f16 != 0), hi = pack2(a.z * e, a.w * e, f16 != 0);
+    uint16_t *o = out + r * out_stride + c;
+    if (vec && c + 4 <= cols) {
+      *reinterpret_cast<uint2 *>(o) = make_uint2(lo, hi);
+    } else {
+      const uint16_t v[4] = {uint16_t(lo), uint16_t(lo >> 16), uint16_t(hi), uint16_t(hi >> 16)};
+      for (int j = 0; j < 4 && c + j < cols; ++j) o[j] = v[j];
+    }
+  }
+}
+
+// 2-D copy of 16-bit values between row strides, one side of which TMA cannot
+// address (odd strides or unaligned bases).  A warp takes 256 consecutive
+// columns of a row at a time, 32 loads of 2 bytes per lane-strided step, so
+// that both sides move in full 64-byte pieces whatever their alignment.
+__global__ void __launch_bounds__(256)
+    ce_copy2d_kernel(const uint16_t *__restrict__ src, int64_t src_stride, uint16_t *__restrict__ dst,
+                     int64_t dst_stride, int64_t rows, int64_t cols) {
+  const int64_t chunks = (cols + 255) / 256, total = rows * chunks;
+  const int lane = threadIdx.x & 31;
+  for (int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += int64_t(gridDim.x) * 8) {
+    const int64_t r = i / chunks, c = (i - r * chunks) * 256;
+    const uint16_t *s = src + r * src_stride + c;
+    uint16_t *d = dst + r * dst_stride + c;
+    const int n = int(min(int64_t(256), cols - c));
+    uint16_t v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j * 32 + lane < n) v[j] = s[j * 32 + lane];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j * 32 + lane < n) d[j * 32 + lane] = v[j];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+bool tma_ok(const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0; }
+
+// One GEMM's tile: 256 x 256 (one CTA, two M=128 MMAs per B tile) or 128 x 128.
+struct Tile {
+  bool large;
+  int tm() const { return large ? 256 : 128; }
+  int64_t tiles(int64_t m, int64_t n) const { return ((m + tm() - 1) / tm()) * ((n + tm() - 1) / tm()); }
+};
+
+// The large tile reads half as many operand bytes per product; the small one
+// fills the SMs where the large leaves them idle.
+Tile pick(int64_t m, int64_t n, int forced, int sms) {
+  if (forced) return Tile{forced == 256};
+  const int64_t tl = Tile{true}.tiles(m, n);
+  return Tile{tl >= sms};
+}
+
+struct Plan {
+  Tile g1, gh, gw;
+  bool pack_h, pack_w, pad_dh, pad_dw;
+  int64_t ld;            // row stride of packed h / w / padded outputs
+  int64_t rows_p;        // tokens rounded up to 256
+  int64_t n_tiles;       // vocabulary tiles of STATS
+  int64_t piece, pieces; // vocabulary columns per piece, pieces
+  int splits, kb_split;  // K-splits of DH, K-blocks in each
+  bool slabs;            // DH goes through fp32 slabs
+  int64_t slab_ld, slab_elems;
+  size_t o_sc, o_sums, o_part, o_tlogit, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
+  size_t fixed, bytes;   // bytes: fixed + the piece's d (and padded dw)
+};
+
+int check(const ks_linear_ce_config &c, const ks_linear_ce_args &a, char *reason, size_t len) {
+  if (c.tile_m != 0 && c.tile_m != 128 && c.tile_m != 256) {
+    ks::set_reason(reason, len, "linear_ce: tile_m must be 0 (chosen), 128 or 256");
+    return KS_ERR_INVALID_CONFIG;
+  }
+  if (c.piece < 0 || c.piece % 256 != 0) {
+    ks::set_reason(reason, len, "linear_ce: piece must be 0 (chosen) or a multiple of 256");
+    return KS_ERR_INVALID_CONFIG;
+  }
+  if (a.dtype != KS_BF16 && a.dtype != KS_F16) {
+    ks::set_reason(reason, len, "linear_ce: dtype must be bf16 or fp16");
+    return KS_ERR_INVALID_CONFIG;
+  }
+  if (a.pass < KS_CE_FORWARD || a.pass > KS_CE_GRAD || a.reduction < KS_CE_NONE || a.reduction > KS_CE_SUM) {
+    ks::set_reason(reason, len, "linear_ce: pass or reduction out of range");
+    return KS_ERR_INVALID_CONFIG;
+  }
+  if (a.pass == KS_CE_GRAD && a.reduction == KS_CE_NONE) {
+    ks::set_reason(reason, len, "linear_ce: loss and gradient in one call need reduction mean or sum");
+    return KS_ERR_INVALID_CONFIG;
+  }
+  const int64_t lim = (int64_t(1) << 31) - 512;
+  if (a.tokens <= 0 || a.dim <= 0 || a.vocab <= 0 || a.tokens > lim || a.dim > lim || a.vocab > lim) {
+    ks::set_reason(reason, len, "linear_ce: tokens, dim and vocab must be positive and below 2^31 - 512 (got %lld, %lld, %lld)",
+                   (long long)a.tokens, (long long)a.dim, (long long)a.vocab);
+    return KS_ERR_INVALID_ARGS;
+  }
+  if (a.h_stride < a.dim || a.w_stride < a.dim ||
+      (a.pass != KS_CE_FORWARD && (a.dh_stride < a.dim || a.dw_stride < a.dim))) {
+    ks::set_reason(reason, len, "linear_ce: a row stride is smaller than dim");
+    return KS_ERR_INVALID_ARGS;
+  }
+  ks::set_reason(reason, len, "");
+  return KS_OK;
+}
+
+// `avail`: workspace bytes; 0 asks for the least plan.
+void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t avail, Plan &p) {
+  const int sms = ks::sm_count();
+  const bool fwd = a.pass != KS_CE_BACKWARD, bwd = a.pass != KS_CE_FORWARD;
+  p.g1 = pick(a.tokens, a.vocab, c.tile_m, sms);
+  p.gh = pick(a.tokens, a.dim, c.tile_m, sms);
+  p.gw = pick(a.vocab, a.dim, c.tile_m, sms);
+  p.pack_h = !tma_ok(a.h, a.h_stride);
+  p.pack_w = !tma_ok(a.w, a.w_stride);
+  p.pad_dh = bwd && !tma_ok(a.dh, a.dh_stride);
+  p.pad_dw = bwd && !tma_ok(a.dw, a.dw_stride);
+  p.ld = up(a.dim, 8);
+  p.rows_p = up(a.tokens, 256);
+  p.n_tiles = (a.vocab + p.g1.tm() - 1) / p.g1.tm();
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = o;
+    o += (bytes + 1023) / 1024 * 1024;
+    return at;
+  };
+  p.o_sc = take(sizeof(CeScalars));
+  p.o_sums = take(fwd ? size_t((a.tokens + kCombRows - 1) / kCombRows) * 16 : 0);
+  p.o_part = take(fwd ? size_t(p.n_tiles) * p.rows_p * 8 : 0);
+  p.o_tlogit = take(fwd ? size_t(p.rows_p) * 4 : 0);
+  p.o_lse = take(fwd ? size_t(p.rows_p) * 4 : 0);
+  p.o_h = take(p.pack_h ? size_t(a.tokens) * p.ld * 2 : 0);
+  p.o_w = take(p.pack_w ? size_t(a.vocab) * p.ld * 2 : 0);
+  p.splits = p.kb_split = 1;
+  p.slabs = false;
+  p.piece = p.pieces = 0;
+  p.o_dh = p.o_slab = p.o_dw = p.o_d = o;
+  if (bwd) {
+    const int64_t whole = up(a.vocab, 256);
+    const size_t per_col = size_t(a.tokens) * 2 + (p.pad_dw ? size_t(p.ld) * 2 : 0);
+    auto lay = [&](int64_t piece, size_t from) {
+      o = from;
+      p.piece = piece;
+      p.pieces = (a.vocab + piece - 1) / piece;
+      // few output tiles: split the piece's columns until the SMs are filled, at least 8 K-blocks each
+      const int64_t tiles = p.gh.tiles(a.tokens, a.dim), kbs = (std::min(piece, a.vocab) + kBK - 1) / kBK;
+      const int64_t s = std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kbs / 8));
+      p.kb_split = int((kbs + s - 1) / s);
+      p.splits = int((kbs + p.kb_split - 1) / p.kb_split);
+      p.slabs = p.splits > 1 || p.pieces > 1;
+      p.slab_ld = up(a.dim, 32);
+      p.slab_elems = p.rows_p * p.slab_ld;
+      p.o_dh = take(p.pad_dh && !p.slabs ? size_t(a.tokens) * p.ld * 2 : 0);
+      p.o_slab = take(p.slabs ? size_t(p.splits) * p.slab_elems * 4 : 0);
+      p.fixed = o;
+      p.o_dw = take(p.pad_dw ? size_t(std::min(piece, a.vocab)) * p.ld * 2 : 0);
+      p.o_d = take(size_t(a.tokens) * piece * 2);
+      p.bytes = o;
+    };
+    const size_t from = o;
+    int64_t piece = c.piece ? std::min(c.piece, whole) : whole;
+    lay(piece, from);
+    while (!c.piece && p.bytes > avail && piece > 256) {
+      // bytes fall with the piece; the slabs come in once it is not whole
+      const int64_t n = avail > p.fixed ? int64_t((avail - p.fixed) / per_col) / 256 * 256 : 256;
+      piece = std::max<int64_t>(256, std::min<int64_t>(piece - 256, n));
+      lay(piece, from);
+    }
+  } else {
+    p.fixed = p.bytes = o;
+  }
+}
+
+template <int MODE, int BN, int STAGES, int ACC, int MH>
+int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g, cudaStream_t st) {
+  using L = Layout<BN, STAGES, ACC, MH>;
+  auto kern = ce_gemm_kernel<MODE, BN, STAGES, ACC, MH>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(L::request));
+  if (e != cudaSuccess) return ks::map_cuda(e);
+  const int64_t work = int64_t((g.M + kBM * MH - 1) / (kBM * MH)) * ((g.N + BN - 1) / BN) * g.splits;
+  if (work > (int64_t(1) << 30)) return KS_ERR_INVALID_ARGS;
+  const int sms = ks::sm_count();
+  kern<<<int(std::min<int64_t>(work, sms)), kThreads, L::request, st>>>(ta, tb, tc, g, ks::wait_ctx());
+  return ks::map_cuda(cudaGetLastError());
+}
+
+template <int MODE>
+int launch_tile(Tile t, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g,
+                cudaStream_t st) {
+  return t.large ? launch<MODE, 256, 3, 1, 2>(ta, tb, tc, g, st) : launch<MODE, 128, 5, 2, 1>(ta, tb, tc, g, st);
+}
+
+CUtensorMapDataType tm_type(int dtype) {
+  return dtype == KS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// K-major operand [rows, cols]: boxes of 64 columns (K) x `box` rows.
+int map_k(CUtensorMap *m, int dtype, const void *p, int64_t rows, int64_t cols, int64_t stride, int box) {
+  return ks::encode_tmap_2d(m, tm_type(dtype), p, uint64_t(cols), uint64_t(rows), uint64_t(stride) * 2, kBK, box,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// MN-major operand [K rows, cols]: boxes of 64 columns x 64 K-rows; all of a
+// tile's boxes in one copy when the columns are whole blocks of 64.
+int map_mn(CUtensorMap *m, int dtype, const void *p, int64_t rows, int64_t cols, int64_t stride, int tile, int *b3d) {
+  if (cols % 64 == 0 && ks::encode_tmap_3d(m, tm_type(dtype), p, 64, uint64_t(rows), uint64_t(cols / 64),
+                                           uint64_t(stride) * 2, 128, 64, kBK, tile / 64,
+                                           CU_TENSOR_MAP_SWIZZLE_128B) == KS_OK) {
+    *b3d = 1;
+    return KS_OK;
+  }
+  *b3d = 0;
+  return ks::encode_tmap_2d(m, tm_type(dtype), p, uint64_t(cols), uint64_t(rows), uint64_t(stride) * 2, 64, kBK,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Output [rows, cols] of 16-bit values: 32 x 32 blocks, 64-byte swizzle.
+int map_out(CUtensorMap *m, int dtype, void *p, int64_t rows, int64_t cols, int64_t stride) {
+  return ks::encode_tmap_2d(m, tm_type(dtype), p, uint64_t(cols), uint64_t(rows), uint64_t(stride) * 2, 32, 32,
+                            CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+int copy2d(const void *src, int64_t ss, void *dst, int64_t ds, int64_t rows, int64_t cols, cudaStream_t st) {
+  const int64_t items = rows * ((cols + 255) / 256);
+  const int grid = int(std::min<int64_t>((items + 7) / 8, int64_t(ks::sm_count()) * 8));
+  ce_copy2d_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t *>(src), ss, static_cast<uint16_t *>(dst), ds, rows,
+                                         cols);
+  return ks::map_cuda(cudaGetLastError());
+}
+
+int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
+  char *ws = static_cast<char *>(a.workspace);
+  const bool fwd = a.pass != KS_CE_BACKWARD, bwd = a.pass != KS_CE_FORWARD;
+  auto sc = reinterpret_cast<CeScalars *>(ws + p.o_sc);
+  const float range = a.dtype == KS_F16 ? kF16Range : 1.f;
+  int s;
+  const void *h = a.h, *w = a.w;
+  int64_t hs = a.h_stride, wst = a.w_stride;
+  if (p.pack_h) {
+    if ((s = copy2d(a.h, a.h_stride, ws + p.o_h, p.ld, a.tokens, a.dim, st)) != KS_OK) return s;
+    h = ws + p.o_h;
+    hs = p.ld;
+  }
+  if (p.pack_w) {
+    if ((s = copy2d(a.w, a.w_stride, ws + p.o_w, p.ld, a.vocab, a.dim, st)) != KS_OK) return s;
+    w = ws + p.o_w;
+    wst = p.ld;
+  }
+  CeGemm g = {};
+  g.f16 = a.dtype == KS_F16;
+  g.tokens = a.tokens;
+  g.vocab = a.vocab;
+  g.targets = a.targets;
+  g.ignore = a.ignore_index;
+  g.rows_p = p.rows_p;
+  g.sc = sc;
+  g.splits = 1;
+  const int64_t kd = (a.dim + kBK - 1) / kBK;
+  CUtensorMap th, tw;
+  const int t1 = p.g1.tm();
+  if ((s = map_k(&th, a.dtype, h, a.tokens, a.dim, hs, t1)) != KS_OK) return s;
+  float *lse = a.lse;
+  if (fwd) {
+    if (!lse) lse = reinterpret_cast<float *>(ws + p.o_lse);
+    if ((s = map_k(&tw, a.dtype, w, a.vocab, a.dim, wst, t1)) != KS_OK) return s;
+    g.M = int(a.tokens);
+    g.N = int(a.vocab);
+    g.kb_total = g.kb_split = int(kd);
+    g.group = -8;
+    g.part = reinterpret_cast<float2 *>(ws + p.o_part);
+    g.tlogit = reinterpret_cast<float *>(ws + p.o_tlogit);
+    if ((s = launch_tile<STATS>(p.g1, th, tw, th, g, st)) != KS_OK) return s;
+    const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
+    ce_combine_kernel<<<blocks, 256, 0, st>>>(g.part, int(p.n_tiles), p.rows_p, g.tlogit, a.targets, a.tokens, a.vocab,
+                                              a.ignore_index, a.reduction, a.grad_scale, a.dloss, range, a.loss, lse,
+                                              reinterpret_cast<double2 *>(ws + p.o_sums), sc);
+    if ((s = ks::map_cuda(cudaGetLastError())) != KS_OK) return s;
+  }
+  if (!bwd) return KS_OK;
+  if (!fwd) {
+    ce_scalars_kernel<<<1, 1024, 0, st>>>(a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale,
+                                          a.dloss, range, sc);
+    if ((s = ks::map_cuda(cudaGetLastError())) != KS_OK) return s;
+  }
+  char *d = ws + p.o_d;
+  float *slabs = reinterpret_cast<float *>(ws + p.o_slab);
+  for (int64_t i = 0; i < p.pieces; ++i) {
+    const int64_t v0 = i * p.piece, vp = std::min(p.piece, a.vocab - v0), vpad = up(vp, 256);
+    const char *wp = static_cast<const char *>(w) + v0 * wst * 2;
+    CUtensorMap ta, tb, tc;
+    // d of the piece: [tokens, vpad], columns past the vocabulary zero
+    if ((s = map_k(&tw, a.dtype, wp, vp, a.dim, wst, t1)) != KS_OK) return s;
+    if ((s = map_out(&tc, a.dtype, d, a.tokens, vpad, vpad)) != KS_OK) return s;
+    g.M = int(a.tokens);
+    g.N = int(vpad);
+    g.kb_total = g.kb_split = int(kd);
+    g.splits = 1;
+    g.group = -8;
+    g.v0 = v0;
+    g.lse = lse;
+    g.dloss = a.reduction == KS_CE_NONE ? a.dloss : nullptr;
+    if ((s = launch_tile<PROB>(p.g1, th, tw, tc, g, st)) != KS_OK) return s;
+    // dh (+)= d w
+    const int th_ = p.gh.tm();
+    if ((s = map_k(&ta, a.dtype, d, a.tokens, vp, vpad, th_)) != KS_OK) return s;
+    if ((s = map_mn(&tb, a.dtype, wp, vp, a.dim, wst, th_, &g.b3d)) != KS_OK) return s;
+    const bool slabbed = p.slabs;
+    if (slabbed)
+      s = ks::encode_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, slabs, uint64_t(p.slab_ld),
+                             uint64_t(p.splits) * p.rows_p, uint64_t(p.slab_ld) * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    else
+      s = map_out(&tc, a.dtype, p.pad_dh ? ws + p.o_dh : a.dh, a.tokens, a.dim, p.pad_dh ? p.ld : a.dh_stride);
+    if (s != KS_OK) return s;
+    g.N = int(a.dim);
+    g.kb_total = int((vp + kBK - 1) / kBK);
+    g.kb_split = p.kb_split;
+    g.splits = int((g.kb_total + g.kb_split - 1) / g.kb_split);
+    g.group = 8;
+    g.out_f32 = slabbed;
+    g.accumulate = slabbed && i > 0;
+    if ((s = launch_tile<DH>(p.gh, ta, tb, tc, g, st)) != KS_OK) return s;
+    // rows v0.. of dw = d^T h
+    const int tw_ = p.gw.tm();
+    int a3d = 0;
+    if ((s = map_mn(&ta, a.dtype, d, a.tokens, vpad, vpad, tw_, &a3d)) != KS_OK) return s;
+    if (!a3d) return KS_ERR_OTHER;
+    if ((s = map_mn(&tb, a.dtype, h, a.tokens, a.dim, hs, tw_, &g.b3d)) != KS_OK) return s;
+    char *dwp = static_cast<char *>(a.dw) + v0 * a.dw_stride * 2;
+    if ((s = map_out(&tc, a.dtype, p.pad_dw ? ws + p.o_dw : dwp, vp, a.dim, p.pad_dw ? p.ld : a.dw_stride)) != KS_OK)
+      return s;
+    g.M = int(vp);
+    g.kb_total = g.kb_split = int((a.tokens + kBK - 1) / kBK);
+    g.splits = 1;
+    g.out_f32 = g.accumulate = 0;
+    if ((s = launch_tile<DW>(p.gw, ta, tb, tc, g, st)) != KS_OK) return s;
+    if (p.pad_dw && (s = copy2d(ws + p.o_dw, p.ld, dwp, a.dw_stride, vp, a.dim, st)) != KS_OK) return s;
+  }
+  if (p.slabs) {
+    const int64_t items = a.tokens * ((a.dim + 3) / 4);
+    const int grid = int(std::min<int64_t>((items + 255) / 256, int64_t(ks::sm_count()) * 8));
+    const int vec = reinterpret_cast<uintptr_t>(a.dh) % 8 == 0 && a.dh_stride % 4 == 0;
+    ce_dh_finish_kernel<<<grid, 256, 0, st>>>(slabs, p.splits, p.slab_elems, p.slab_ld, a.tokens, a.dim, sc,
+                                              static_cast<uint16_t *>(a.dh), a.dh_stride, a.dtype == KS_F16, vec);
+    return ks::map_cuda(cudaGetLastError());
+  }
+  if (p.pad_dh) return copy2d(ws + p.o_dh, p.ld, a.dh, a.dh_stride, a.tokens, a.dim, st);
+  return KS_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ks_linear_ce_validate(const ks_linear_ce_config *cfg, const ks_linear_ce_args *a, char *reason, size_t len) {
+  if (!cfg || !a) return KS_ERR_INVALID_ARGS;
+  return check(*cfg, *a, reason, len);
+}
+
+int ks_linear_ce_workspace_bytes(const ks_linear_ce_config *cfg, const ks_linear_ce_args *a, size_t limit,
+                                 size_t *least, size_t *bytes) {
+  if (!cfg || !a || !least || !bytes) return KS_ERR_INVALID_ARGS;
+  const int s = check(*cfg, *a, nullptr, 0);
+  if (s != KS_OK) return s;
+  Plan p;
+  make_plan(*cfg, *a, 0, p);
+  *least = p.bytes;
+  make_plan(*cfg, *a, std::max(limit, *least), p);
+  *bytes = p.bytes;
+  return KS_OK;
+}
+
+int ks_linear_ce_launch(const ks_linear_ce_config *cfg, const ks_linear_ce_args *a, void *stream) {
+  if (!cfg || !a || !a->h || !a->w || !a->targets) return KS_ERR_INVALID_ARGS;
+  int s = check(*cfg, *a, nullptr, 0);
+  if (s != KS_OK) return s;
+  if (a->pass != KS_CE_BACKWARD && !a->loss) return KS_ERR_INVALID_ARGS;
+  if (a->pass == KS_CE_BACKWARD && !a->lse) return KS_ERR_INVALID_ARGS;
+  if (a->pass != KS_CE_FORWARD && (!a->dh || !a->dw)) return KS_ERR_INVALID_ARGS;
+  auto odd = [](const void *p, uintptr_t m) { return (reinterpret_cast<uintptr_t>(p) & (m - 1)) != 0; };
+  if (odd(a->h, 2) || odd(a->w, 2) || odd(a->targets, 8) || odd(a->dloss, 4) || odd(a->loss, 4) || odd(a->lse, 4) ||
+      odd(a->dh, 2) || odd(a->dw, 2))
+    return KS_ERR_INVALID_ARGS;
+  Plan p;
+  make_plan(*cfg, *a, a->workspace_bytes, p);
+  if (!a->workspace || p.bytes > a->workspace_bytes || odd(a->workspace, 256)) return KS_ERR_WORKSPACE;
+  if ((s = ks::check_arch_sm100()) != KS_OK) return s;
+  return run(*a, p, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -22,9 +22,11 @@ KS_ERR_WORKSPACE = -22
 KS_ERR_DEVICE_TIMEOUT = -23
 KS_ERR_ARCH = -24
 
-KS_BF16, KS_F32, KS_F64 = 0, 1, 2
+KS_BF16, KS_F32, KS_F64, KS_F16 = 0, 1, 2, 3
 KS_MODE_ONEPASS, KS_MODE_TWOPASS, KS_MODE_STRIDED, KS_MODE_TREE, KS_MODE_STAGED, KS_MODE_CLUSTER = 0, 1, 2, 3, 4, 5
 KS_GELU_ERF, KS_GELU_TANH = 0, 1
+KS_CE_FORWARD, KS_CE_BACKWARD, KS_CE_GRAD = 0, 1, 2
+KS_CE_NONE, KS_CE_MEAN, KS_CE_SUM = 0, 1, 2
 
 MODE_NAMES = {"onepass": 0, "twopass": 1, "strided": 2, "tree": 3, "staged": 4}
 
@@ -94,6 +96,21 @@ class FlashAttentionArgs(C.Structure):
                 ("d", C.c_int64), ("scale", C.c_float)]
 
 
+class LinearCeConfig(C.Structure):
+    _fields_ = [("tile_m", C.c_int), ("piece", C.c_int64)]
+
+
+class LinearCeArgs(C.Structure):
+    _fields_ = [("h", C.c_void_p), ("w", C.c_void_p), ("targets", C.c_void_p),
+                ("tokens", C.c_int64), ("dim", C.c_int64), ("vocab", C.c_int64),
+                ("h_stride", C.c_int64), ("w_stride", C.c_int64),
+                ("dtype", C.c_int), ("ce_pass", C.c_int), ("reduction", C.c_int), ("grad_scale", C.c_float),
+                ("ignore_index", C.c_int64),
+                ("dloss", C.c_void_p), ("loss", C.c_void_p), ("lse", C.c_void_p),
+                ("dh", C.c_void_p), ("dw", C.c_void_p), ("dh_stride", C.c_int64), ("dw_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 CONFIG_TYPES = {
     "softmax": SoftmaxConfig, "layernorm": LayerNormConfig, "bias_gelu": BiasGeluConfig,
     "reduction": ReductionConfig, "matmul": MatmulConfig, "flash_attention": FlashAttentionConfig,
@@ -145,6 +162,10 @@ PROTOTYPES = {
     "ks_flash_attention_validate": (C.c_int, [_P(FlashAttentionConfig), _P(FlashAttentionArgs), C.c_char_p,
                                               C.c_size_t]),
     "ks_flash_attention_launch": (C.c_int, [_P(FlashAttentionConfig), _P(FlashAttentionArgs), C.c_void_p]),
+    "ks_linear_ce_validate": (C.c_int, [_P(LinearCeConfig), _P(LinearCeArgs), C.c_char_p, C.c_size_t]),
+    "ks_linear_ce_workspace_bytes": (C.c_int, [_P(LinearCeConfig), _P(LinearCeArgs), C.c_size_t, _P(C.c_size_t),
+                                               _P(C.c_size_t)]),
+    "ks_linear_ce_launch": (C.c_int, [_P(LinearCeConfig), _P(LinearCeArgs), C.c_void_p]),
     "ks_peak_sink_words": (C.c_int, [_P(C.c_size_t)]),
     "ks_peak_copy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "ks_peak_read": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
@@ -194,7 +215,7 @@ def validate(family: str, cfg, *shape_or_args) -> tuple[int, str]:
     """Run ks_<family>_validate; returns (status, reason)."""
     buf = C.create_string_buffer(512)
     fn = getattr(lib, f"ks_{family}_validate")
-    if family in ("reduction", "flash_attention"):
+    if family in ("reduction", "flash_attention", "linear_ce"):
         st = fn(C.byref(cfg), C.byref(shape_or_args[0]), buf, 512)
     else:
         st = fn(C.byref(cfg), *[C.c_int64(v) for v in shape_or_args], buf, 512)

@@ -213,6 +213,150 @@ def flash_attention(q, k, v, causal: bool = True, scale: float = 0.0, out=None, 
     return out
 
 
+# ---------------------------------------------------------------------------
+# Training operators at the vocabulary end of a language model
+# ---------------------------------------------------------------------------
+_DT_TRAIN = {torch.bfloat16: N.KS_BF16, torch.float16: N.KS_F16, torch.float32: N.KS_F32}
+_REDUCTIONS = {"none": N.KS_CE_NONE, "mean": N.KS_CE_MEAN, "sum": N.KS_CE_SUM}
+
+
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    """torch.empty from the pool of the stream that the launch goes to: scratch
+    freed after the call is then reused only behind the launch."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _check_rows(name, t, dtypes, device=None):
+    """A [rows, cols] CUDA tensor on the current device with dense rows (any row
+    stride of at least cols)."""
+    if not (t.is_cuda and t.dim() == 2 and t.dtype in dtypes):
+        raise ValueError(f"{name} must be a 2-D CUDA tensor of {' or '.join(str(d) for d in dtypes)}")
+    if t.device.index != torch.cuda.current_device() or (device is not None and t.device != device):
+        raise ValueError(f"{name} is on {t.device}, not on the current device")
+    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
+        raise ValueError(f"{name} must have dense rows (stride 1 along the last axis) that do not overlap")
+
+
+def _row_stride(t) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def _check_ids(name, t, n, device):
+    if not (t.is_cuda and t.device == device and t.dtype == torch.int64 and t.is_contiguous() and t.numel() == n):
+        raise ValueError(f"{name} must be a contiguous int64 tensor of {n} values on {device}")
+
+
+def _check_f32(name, t, n, device):
+    if not (t.is_cuda and t.device == device and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n):
+        raise ValueError(f"{name} must be a contiguous float32 tensor of {n} values on {device}")
+
+
+def _linear_ce_args(h, w, targets, ce_pass, reduction, ignore_index, grad_scale=1.0) -> N.LinearCeArgs:
+    _check_rows("h", h, (torch.bfloat16, torch.float16))
+    _check_rows("w", w, (h.dtype,), h.device)
+    if h.shape[1] != w.shape[1]:
+        raise ValueError("h and w differ in their last dimension")
+    _check_ids("targets", targets, h.shape[0], h.device)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
+    a = N.LinearCeArgs()
+    a.h, a.w, a.targets = h.data_ptr(), w.data_ptr(), targets.data_ptr()
+    a.tokens, a.dim, a.vocab = h.shape[0], h.shape[1], w.shape[0]
+    a.h_stride, a.w_stride = _row_stride(h), _row_stride(w)
+    a.dh_stride = a.dw_stride = a.dim
+    a.dtype, a.ce_pass, a.reduction = _DT_TRAIN[h.dtype], ce_pass, _REDUCTIONS[reduction]
+    a.grad_scale, a.ignore_index = grad_scale, ignore_index
+    return a
+
+
+# Default bound on the scratch of one call: a piece of the vocabulary large
+# enough that its three GEMMs run at full rate.
+LINEAR_CE_WORKSPACE_LIMIT = 1 << 30
+
+
+def linear_cross_entropy_workspace_bytes(args: N.LinearCeArgs, cfg=None, limit=None) -> tuple[int, int]:
+    """(least, preferred) workspace bytes of one ks_linear_ce_launch."""
+    cfg = cfg or N.LinearCeConfig()
+    least, want = C.c_size_t(0), C.c_size_t(0)
+    N.check("ks_linear_ce_workspace_bytes",
+            N.lib.ks_linear_ce_workspace_bytes(C.byref(cfg), C.byref(args),
+                                               LINEAR_CE_WORKSPACE_LIMIT if limit is None else limit,
+                                               C.byref(least), C.byref(want)))
+    return least.value, want.value
+
+
+def _linear_ce_run(a, cfg, workspace, device, stream):
+    cfg = cfg or N.LinearCeConfig()
+    if workspace is None:
+        workspace = _empty(linear_cross_entropy_workspace_bytes(a, cfg)[1], torch.uint8, device, stream)
+    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    N.check("ks_linear_ce_launch", N.lib.ks_linear_ce_launch(C.byref(cfg), C.byref(a), _stream_ptr(stream)))
+
+
+def linear_cross_entropy(h, w, targets, ignore_index: int = -100, reduction: str = "none", cfg=None, workspace=None,
+                         stream=None):
+    """Loss of each token (or their mean or sum) and log-sum-exp of each token's
+    logits h @ w.T, without the logits in memory: h [tokens, dim], w [vocab,
+    dim] (bf16 or fp16), targets int64.  Returns (loss, lse) in fp32."""
+    a = _linear_ce_args(h, w, targets, N.KS_CE_FORWARD, reduction, ignore_index)
+    n = a.tokens
+    loss = _empty(n if reduction == "none" else 1, torch.float32, h.device, stream)
+    lse = _empty(n, torch.float32, h.device, stream)
+    if n == 0:
+        return loss.zero_(), lse
+    a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
+    _linear_ce_run(a, cfg, workspace, h.device, stream)
+    return loss, lse
+
+
+def _linear_ce_grads(a, h, w, dh, dw, stream):
+    dh = _empty(h.shape, h.dtype, h.device, stream) if dh is None else dh
+    dw = _empty(w.shape, w.dtype, w.device, stream) if dw is None else dw
+    for name, t, like in (("dh", dh, h), ("dw", dw, w)):
+        _check_rows(name, t, (like.dtype,), like.device)
+        if t.shape != like.shape:
+            raise ValueError(f"{name} must have the shape {tuple(like.shape)}")
+    a.dh, a.dw, a.dh_stride, a.dw_stride = dh.data_ptr(), dw.data_ptr(), _row_stride(dh), _row_stride(dw)
+    return dh, dw
+
+
+def linear_cross_entropy_backward(h, w, targets, lse, dloss=None, ignore_index: int = -100, reduction: str = "none",
+                                  grad_scale: float = 1.0, dh=None, dw=None, cfg=None, workspace=None, stream=None):
+    """Gradients (dh, dw) of linear_cross_entropy from its lse.  dloss: the
+    incoming fp32 gradient, one value per token for reduction "none", one value
+    otherwise; None stands for ones.  Tokens with targets == ignore_index take no
+    part, and the mean divides by the number of the others."""
+    a = _linear_ce_args(h, w, targets, N.KS_CE_BACKWARD, reduction, ignore_index, grad_scale)
+    _check_f32("lse", lse, a.tokens, h.device)
+    if dloss is not None:
+        _check_f32("dloss", dloss, a.tokens if reduction == "none" else 1, h.device)
+    dh, dw = _linear_ce_grads(a, h, w, dh, dw, stream)
+    if a.tokens == 0:
+        return dh, dw.zero_()
+    a.lse, a.dloss = lse.data_ptr(), dloss.data_ptr() if dloss is not None else None
+    _linear_ce_run(a, cfg, workspace, h.device, stream)
+    return dh, dw
+
+
+def linear_cross_entropy_grad(h, w, targets, ignore_index: int = -100, reduction: str = "mean", grad_scale: float = 1.0,
+                              dh=None, dw=None, cfg=None, workspace=None, stream=None):
+    """Loss (fp32, one value) and the gradients of grad_scale * loss with respect
+    to h and w in one call: what a training step needs of its last layer."""
+    a = _linear_ce_args(h, w, targets, N.KS_CE_GRAD, reduction, ignore_index, grad_scale)
+    if reduction == "none":
+        raise ValueError("loss and gradient in one call need reduction 'mean' or 'sum'")
+    loss = _empty(1, torch.float32, h.device, stream)
+    dh, dw = _linear_ce_grads(a, h, w, dh, dw, stream)
+    if a.tokens == 0:
+        return loss.zero_(), dh, dw.zero_()
+    a.loss = loss.data_ptr()
+    _linear_ce_run(a, cfg, workspace, h.device, stream)
+    return loss, dh, dw
+
+
 def device_error_take() -> int:
     w = C.c_int(0)
     N.check("ks_device_error_take", N.lib.ks_device_error_take(C.byref(w)))
