@@ -269,8 +269,10 @@ int ks_flash_attention_launch(const ks_flash_attention_config *cfg,
  * KS_CE_SUM: loss and dloss have one.  dloss == NULL stands for ones.
  * g[r] = grad_scale * dloss / (mean: number of tokens that count), and 0 for
  * the tokens that do not count or whose target is out of range.
- * The logits are never kept.  The backward pass takes them again in pieces of
- * the vocabulary, whose d (16 bits a value) live in the workspace.
+ * The logits are never kept.  A gradient call forms d (16 bits a value) in the
+ * workspace, in pieces of the vocabulary, from logits taken a second time;
+ * KS_CE_GRAD with a workspace that holds d whole keeps 16-bit exponentials
+ * there in the first pass and saves the second.
  * cfg.tile_m: 0 = chosen from the sizes, 128 = 128 x 128 tiles, 256 = 256 x
  * 256 tiles.  cfg.piece: vocabulary columns per piece of the backward pass, a
  * multiple of 256; 0 = as many as the workspace holds.

@@ -5,13 +5,18 @@
 //   d[r,v] = f[r] (exp(l[r,v] - lse[r]) - [v == t[r]])
 //   dh = d w;  dw = d^T h
 //
-// The logits [tokens, vocab] are never written.  Four GEMM-shaped passes share
+// The logits [tokens, vocab] are never written.  Five GEMM-shaped passes share
 // one persistent kernel (TMA producer warp, one MMA-issuing thread, four
 // epilogue warps; tcgen05.mma kind::f16, fp32 accumulators in TMEM):
 //   STATS  l = h w^T; the epilogue reduces each tile's row to (max, sum of
 //          exponentials) and picks the target's logit out of the accumulator;
+//   STORE  STATS that also writes exp(l - tile maximum) in 16 bits, for a call
+//          that takes loss and gradient together and whose workspace holds 16
+//          bits for every (token, column); a memory-bound pass then turns it
+//          into d in place, and the logits are taken once: 6 instead of 8
+//          tokens x vocab x dim operations;
 //   PROB   l = h w^T again for one piece of the vocabulary; the epilogue
-//          writes d in 16 bits to the workspace;
+//          writes d in 16 bits to the workspace (every other gradient call);
 //   DH     dh (+)= d w over the piece's columns (split over K when there are
 //          few tiles; fp32 slabs, added up in a fixed order);
 //   DW     dw rows of the piece = d^T h, complete after one pass over the
@@ -25,7 +30,12 @@
 // bf16, 2^-11 in fp16, the size of the outputs' own rounding); the common factor
 // grad_scale / count is left out of d and applied to the fp32 accumulator, so
 // that a target's d, near -1, is near a power of two.  fp16 d is stored times
-// 1024, so that probabilities down to 6e-8 stay normal numbers.
+// 1024, so that probabilities down to 6e-8 stay normal numbers.  STORE rounds
+// the exponential too, a second rounding of p (not of the target's d, which is
+// formed from its logit).  The target's logit is taken a second time, as a
+// plain fp32 dot product: the tensor cores' accumulators truncate (a bias of
+// about 4e-6 of a logit at dim 2048), which the sum over the vocabulary
+// averages out but a loss of one large logit would show.
 //
 // Every mbarrier wait is bounded (KsWait), as in matmul.cu.
 #include <algorithm>
@@ -44,8 +54,9 @@ constexpr uint32_t kBBox = kBK * 64 * 2;       // 64 K-rows x 64 columns: 8 KB
 constexpr uint32_t kCBuf = 32 * 128;           // one epilogue block: 32 rows x 32 columns, up to 4 bytes each
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kF16Range = 1024.f;            // factor on fp16 d
+constexpr float kF16Exp = 32768.f;             // factor on STORE's fp16 exponentials, which are at most 1
 
-enum Mode { STATS = 0, PROB = 1, DH = 2, DW = 3 };
+enum Mode { STATS = 0, PROB = 1, DH = 2, DW = 3, STORE = 4 };
 
 // Scalars between the kernels of one call, in the workspace.
 struct CeScalars {
@@ -134,6 +145,35 @@ KS_DEV void work_coords(int t, int num_m, int num_n, int group, int &tm, int &tn
   }
 }
 
+KS_DEV float max32(const uint32_t (&r)[32]) {
+  float m[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m[j] = __uint_as_float(r[j]);
+#pragma unroll
+  for (int j = 4; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], __uint_as_float(r[j]));
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+// Maximum over this lane's row of one accumulator half, `left` columns of it
+// inside the vocabulary.
+template <int BN>
+KS_DEV float half_max(uint32_t t_addr, int64_t left) {
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < BN; c += 32) {
+    uint32_t r[32];
+    ks_tmem_ld32(t_addr + c, r);
+    ks_tmem_wait_ld();
+    if (left - c < 32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j >= left - c) r[j] = __float_as_uint(-INFINITY);
+    }
+    m = fmaxf(m, max32(r));
+  }
+  return m;
+}
+
 template <int MODE, int BN, int STAGES, int ACC, int MH>
 __global__ void __launch_bounds__(kThreads, 1)
     ce_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -169,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ks_prefetch_tmap(&tma_a);
     ks_prefetch_tmap(&tma_b);
     if (MODE != STATS) ks_prefetch_tmap(&tma_c);
-    if (MODE == STATS && blockIdx.x == 0) p.sc->counter = 0;  // for the combine kernel that follows
+    if ((MODE == STATS || MODE == STORE) && blockIdx.x == 0) p.sc->counter = 0;  // for the combine kernel that follows
   }
   if (warp == 1) {
     ks_tmem_alloc(tmem_slot, L::tmem_cols);
@@ -319,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // what this lane's rows need, loaded while the MMAs still run
       int tcol[MH];       // target column relative to the tile, or one outside it
       float lse2[MH], f[MH];
-      if (MODE == STATS || MODE == PROB) {
+      if (MODE == STATS || MODE == STORE || MODE == PROB) {
 #pragma unroll
         for (int h = 0; h < MH; ++h) {
           const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
@@ -347,6 +387,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int cc = 0; cc < MH * (BN / 32); ++cc) {
         const int h = cc / (BN / 32);
         const int cb = (cc % (BN / 32)) * 32;  // first column of the block inside the tile
+        if (MODE == STORE && cb == 0) m = half_max<BN>(t_addr + cc * 32, p.vocab - col0);
         uint32_t r[32];
         ks_tmem_ld32(t_addr + cc * 32, r);
         ks_tmem_wait_ld();
@@ -355,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane == 0) ks_mbar_arrive(tempty + acc * MH + h);
         }
-        if constexpr (MODE == STATS) {
+        if constexpr (MODE == STATS || MODE == STORE) {
           const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cb;
           if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
             float v = 0.f;
@@ -370,18 +411,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 32; ++j)
               if (j >= left) r[j] = __float_as_uint(-INFINITY);
           }
-          float cm[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) cm[j] = __uint_as_float(r[j]);
-#pragma unroll
-          for (int j = 4; j < 32; ++j) cm[j & 3] = fmaxf(cm[j & 3], __uint_as_float(r[j]));
-          const float mn = fmaxf(m, fmaxf(fmaxf(cm[0], cm[1]), fmaxf(cm[2], cm[3])));
+          const float mn = MODE == STORE ? m : fmaxf(m, max32(r));
           // an all -inf row so far: exponentials against 0 are 0, not NaN
           const float base = mn == -INFINITY ? 0.f : mn * kLog2e;
           float a4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) a4[j & 3] += ex2(fmaf(__uint_as_float(r[j]), kLog2e, -base));
-          s = s * ex2(fmaf(m, kLog2e, -base)) + ((a4[0] + a4[1]) + (a4[2] + a4[3]));
+          for (int j = 0; j < 32; ++j) {
+            const float x = ex2(fmaf(__uint_as_float(r[j]), kLog2e, -base));
+            a4[j & 3] += x;
+            if (MODE == STORE) r[j] = __float_as_uint(f16 ? x * kF16Exp : x);
+          }
+          if (MODE == STATS) s *= ex2(fmaf(m, kLog2e, -base));
+          s += (a4[0] + a4[1]) + (a4[2] + a4[3]);
           m = mn;
           if (cb + 32 == BN) {
             const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
@@ -389,7 +430,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             m = -INFINITY;
             s = 0.f;
           }
-        } else {
+        }
+        if constexpr (MODE != STATS) {
           uint8_t *buf = stg + (nstore & 1) * kCBuf;
           if (lane == 0) ks_bulk_wait_read<1>();  // the store two blocks back has read this buffer
           __syncwarp();
@@ -467,12 +509,45 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kCombRows = 8;
 
+// <h[row], w[t]> in fp32 by one warp.
+KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool f16, int lane) {
+  auto val = [&](uint32_t v, int hi) {
+    if (f16) {
+      const __half2 x = *reinterpret_cast<const __half2 *>(&v);
+      return hi ? __high2float(x) : __low2float(x);
+    }
+    return hi ? ks_bf16_hi(v) : ks_bf16_lo(v);
+  };
+  float a0 = 0.f, a1 = 0.f;
+  int64_t k = 0;
+  if (((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15) == 0) {
+    for (; k + 8 <= dim; k += 256) {
+      const int64_t at = k + lane * 8;
+      if (at + 8 > dim) continue;
+      const uint4 x = *reinterpret_cast<const uint4 *>(h + at), y = *reinterpret_cast<const uint4 *>(w + at);
+      a0 = fmaf(val(x.x, 0), val(y.x, 0), a0);
+      a1 = fmaf(val(x.x, 1), val(y.x, 1), a1);
+      a0 = fmaf(val(x.y, 0), val(y.y, 0), a0);
+      a1 = fmaf(val(x.y, 1), val(y.y, 1), a1);
+      a0 = fmaf(val(x.z, 0), val(y.z, 0), a0);
+      a1 = fmaf(val(x.z, 1), val(y.z, 1), a1);
+      a0 = fmaf(val(x.w, 0), val(y.w, 0), a0);
+      a1 = fmaf(val(x.w, 1), val(y.w, 1), a1);
+    }
+    k = dim / 8 * 8;
+  }
+  for (k += lane; k < dim; k += 32) a0 = fmaf(val(h[k], 0), val(w[k], 0), a0);
+  return ks_warp_sum(a0 + a1);
+}
+
 __global__ void __launch_bounds__(256)
-    ce_combine_kernel(const float2 *__restrict__ part, int tiles, int64_t rows_p, const float *__restrict__ tlogit,
+    ce_combine_kernel(const float2 *__restrict__ part, int tiles, int64_t rows_p, const uint16_t *__restrict__ h,
+                      int64_t h_stride, const uint16_t *__restrict__ w, int64_t w_stride, int64_t dim, int f16,
+                      float *__restrict__ tlogit,
                       const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab, int64_t ignore, int reduction,
                       float grad_scale, const float *dloss, float range, float *__restrict__ loss,
                       float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc) {
-  __shared__ float sm[8][kCombRows], ss[8][kCombRows];
+  __shared__ float sm[8][kCombRows], ss[8][kCombRows], dot[kCombRows];
   __shared__ double shl[kCombRows], shn[kCombRows];
   __shared__ bool is_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -493,6 +568,15 @@ __global__ void __launch_bounds__(256)
       const float2 v = part[int64_t(t) * rows_p + row];
       add(v.x, v.y);
     }
+  {
+    static_assert(kCombRows == 8, "one warp per row");
+    const int64_t r = int64_t(blockIdx.x) * kCombRows + warp;
+    const int64_t t = r < tokens ? targets[r] : -1;
+    if (t != ignore && t >= 0 && t < vocab) {
+      const float v = target_dot(h + r * h_stride, w + t * w_stride, dim, f16 != 0, lane);
+      if (lane == 0) dot[warp] = v;
+    }
+  }
 #pragma unroll
   for (int o = kCombRows; o < 32; o <<= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
@@ -510,12 +594,20 @@ __global__ void __launch_bounds__(256)
     for (int w = 1; w < 8; ++w) add(sm[w][tid], ss[w][tid]);
     double l = 0.0, n = 0.0;
     if (row < tokens) {
+      const int64_t t = targets[row];
+      const bool valid = t != ignore && t >= 0 && t < vocab;
+      float lt = 0.f;
+      if (valid) {  // the target's logit as the dot product, in the sum too
+        lt = dot[tid];
+        const float old = tlogit[row];
+        if (isfinite(lt) && isfinite(old)) s += ex2((lt - m) * kLog2e) - ex2((old - m) * kLog2e);
+        tlogit[row] = lt;
+      }
       const float lse = m + logf(s);  // -inf + log 0: a row of -inf logits
       lse_out[row] = lse;
-      const int64_t t = targets[row];
       float v = 0.f;
       if (t != ignore) {
-        v = t >= 0 && t < vocab ? lse - tlogit[row] : __int_as_float(0x7fc00000);
+        v = valid ? lse - lt : __int_as_float(0x7fc00000);
         n = 1.0;
       }
       if (reduction == KS_CE_NONE && loss) loss[row] = v;
@@ -563,6 +655,78 @@ __global__ void __launch_bounds__(256)
     if (loss) loss[0] = float(l / c);
     sc->fscale = range;
     sc->escale = float(double(grad_scale) * (dloss ? double(dloss[0]) : 1.0) / c / double(range));
+  }
+}
+
+// STORE's exponentials e -> d in place: d = f (e exp(tile maximum - lse) -
+// [target]).  A warp takes 256 columns (16 bytes a lane) of one row at a time,
+// four of them in flight; a block's eight warps take eight rows, whose tile
+// maxima share 32-byte sectors.  Reads and writes 2 bytes a value.
+__global__ void __launch_bounds__(256)
+    ce_scale_kernel(uint16_t *__restrict__ d, int64_t ld, const float2 *__restrict__ part, int64_t rows_p, int tile_log2,
+                    const float *__restrict__ lse, const float *__restrict__ tlogit, const int64_t *__restrict__ targets,
+                    int64_t tokens, int64_t vocab, int64_t ignore, const CeScalars *__restrict__ sc, int f16) {
+  const int lane = threadIdx.x & 31;
+  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (row >= tokens) return;
+  const int64_t t = targets[row];
+  const bool valid = t != ignore && t >= 0 && t < vocab;
+  const float f = valid ? sc->fscale : 0.f, fe = f16 ? f / kF16Exp : f;
+  const float l2 = lse[row] * kLog2e;
+  uint16_t *dr = d + row * ld;
+  const float dt = valid ? f * ex2(fmaf(tlogit[row], kLog2e, -l2)) - f : 0.f;
+  const int64_t step = int64_t(gridDim.y) * 256;
+  for (int64_t c0 = int64_t(blockIdx.y) * 256 + lane * 8; c0 < ld; c0 += 4 * step) {
+    uint4 v[4];
+    float k[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = c0 + j * step;
+      k[j] = 0.f;
+      if (c < ld && valid) {
+        v[j] = *reinterpret_cast<const uint4 *>(dr + c);
+        if (c < vocab) k[j] = part[(c >> tile_log2) * rows_p + row].x;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = c0 + j * step;
+      if (c >= ld) continue;
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (valid) {
+        const float g = k[j] == -INFINITY ? 0.f : fe * ex2(fmaf(k[j], kLog2e, -l2));  // a tile of -inf logits holds zeros
+        uint32_t x[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float lo, hi;
+          if (f16) {
+            const __half2 y = *reinterpret_cast<const __half2 *>(&x[i]);
+            lo = __low2float(y);
+            hi = __high2float(y);
+          } else {
+            lo = ks_bf16_lo(x[i]);
+            hi = ks_bf16_hi(x[i]);
+          }
+          x[i] = pack2(lo * g, hi * g, f16 != 0);
+        }
+        const int64_t at = t - c;
+        if (at >= 0 && at < 8) {
+          const uint32_t y = pack2(dt, dt, f16 != 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (i == at >> 1) x[i] = at & 1 ? (x[i] & 0xffffu) | (y & 0xffff0000u) : (x[i] & 0xffff0000u) | (y & 0xffffu);
+        }
+        if (c + 8 > vocab) {  // columns past the vocabulary
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (c + 2 * i >= vocab) x[i] = 0;
+            else if (c + 2 * i + 1 >= vocab) x[i] &= 0xffffu;
+          }
+        }
+        o = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+      *reinterpret_cast<uint4 *>(dr + c) = o;
+    }
   }
 }
 
@@ -694,6 +858,7 @@ struct Plan {
   int64_t piece, pieces; // vocabulary columns per piece, pieces
   int splits, kb_split;  // K-splits of DH, K-blocks in each
   bool slabs;            // DH goes through fp32 slabs
+  bool store;            // one piece, from STORE's exponentials
   int64_t slab_ld, slab_elems;
   size_t o_sc, o_sums, o_part, o_tlogit, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
   size_t fixed, bytes;   // bytes: fixed + the piece's d (and padded dw)
@@ -748,7 +913,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   p.pad_dw = bwd && !tma_ok(a.dw, a.dw_stride);
   p.ld = up(a.dim, 8);
   p.rows_p = up(a.tokens, 256);
-  p.n_tiles = (a.vocab + p.g1.tm() - 1) / p.g1.tm();
+  p.n_tiles = up(a.vocab, 256) / p.g1.tm();  // of STORE, which runs over whole 256-column blocks
   size_t o = 0;
   auto take = [&](size_t bytes) {
     const size_t at = o;
@@ -763,7 +928,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   p.o_h = take(p.pack_h ? size_t(a.tokens) * p.ld * 2 : 0);
   p.o_w = take(p.pack_w ? size_t(a.vocab) * p.ld * 2 : 0);
   p.splits = p.kb_split = 1;
-  p.slabs = false;
+  p.slabs = p.store = false;
   p.piece = p.pieces = 0;
   p.o_dh = p.o_slab = p.o_dw = p.o_d = o;
   if (bwd) {
@@ -797,9 +962,11 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
       piece = std::max<int64_t>(256, std::min<int64_t>(piece - 256, n));
       lay(piece, from);
     }
+    p.store = a.pass == KS_CE_GRAD && p.pieces == 1;
   } else {
     p.fixed = p.bytes = o;
   }
+  if (!p.store) p.n_tiles = (a.vocab + p.g1.tm() - 1) / p.g1.tm();
 }
 
 template <int MODE, int BN, int STAGES, int ACC, int MH>
@@ -900,11 +1067,20 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.group = -8;
     g.part = reinterpret_cast<float2 *>(ws + p.o_part);
     g.tlogit = reinterpret_cast<float *>(ws + p.o_tlogit);
-    if ((s = launch_tile<STATS>(p.g1, th, tw, th, g, st)) != KS_OK) return s;
+    if (p.store) {
+      CUtensorMap te;  // [tokens, whole tiles]: the columns past the vocabulary are -inf logits, zeros
+      if ((s = map_out(&te, a.dtype, ws + p.o_d, a.tokens, up(a.vocab, 256), up(a.vocab, 256))) != KS_OK) return s;
+      g.N = int(up(a.vocab, 256));
+      s = launch_tile<STORE>(p.g1, th, tw, te, g, st);
+    } else {
+      s = launch_tile<STATS>(p.g1, th, tw, th, g, st);
+    }
+    if (s != KS_OK) return s;
     const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
-    ce_combine_kernel<<<blocks, 256, 0, st>>>(g.part, int(p.n_tiles), p.rows_p, g.tlogit, a.targets, a.tokens, a.vocab,
-                                              a.ignore_index, a.reduction, a.grad_scale, a.dloss, range, a.loss, lse,
-                                              reinterpret_cast<double2 *>(ws + p.o_sums), sc);
+    ce_combine_kernel<<<blocks, 256, 0, st>>>(
+        g.part, int(p.n_tiles), p.rows_p, static_cast<const uint16_t *>(h), hs, static_cast<const uint16_t *>(w), wst,
+        a.dim, g.f16, g.tlogit, a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale, a.dloss, range,
+        a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc);
     if ((s = ks::map_cuda(cudaGetLastError())) != KS_OK) return s;
   }
   if (!bwd) return KS_OK;
@@ -930,7 +1106,17 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.v0 = v0;
     g.lse = lse;
     g.dloss = a.reduction == KS_CE_NONE ? a.dloss : nullptr;
-    if ((s = launch_tile<PROB>(p.g1, th, tw, tc, g, st)) != KS_OK) return s;
+    if (p.store) {
+      const unsigned rows8 = unsigned((a.tokens + 7) / 8);
+      const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, std::max<int64_t>(1, 8192 / rows8)));
+      ce_scale_kernel<<<dim3(rows8, cols), 256, 0, st>>>(reinterpret_cast<uint16_t *>(d), vpad, g.part, p.rows_p,
+                                                         t1 == 256 ? 8 : 7, lse, g.tlogit, a.targets, a.tokens, a.vocab,
+                                                         a.ignore_index, sc, g.f16);
+      s = ks::map_cuda(cudaGetLastError());
+    } else {
+      s = launch_tile<PROB>(p.g1, th, tw, tc, g, st);
+    }
+    if (s != KS_OK) return s;
     // dh (+)= d w
     const int th_ = p.gh.tm();
     if ((s = map_k(&ta, a.dtype, d, a.tokens, vp, vpad, th_)) != KS_OK) return s;

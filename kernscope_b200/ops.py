@@ -272,9 +272,9 @@ def _linear_ce_args(h, w, targets, ce_pass, reduction, ignore_index, grad_scale=
     return a
 
 
-# Default bound on the scratch of one call: a piece of the vocabulary large
-# enough that its three GEMMs run at full rate.
-LINEAR_CE_WORKSPACE_LIMIT = 1 << 30
+# Default bound on the scratch of one call.  Where 2 bytes for every (token,
+# vocabulary entry) fit, loss and gradient take the logits once; with less, twice.
+LINEAR_CE_WORKSPACE_LIMIT = 4 << 30
 
 
 def linear_cross_entropy_workspace_bytes(args: N.LinearCeArgs, cfg=None, limit=None) -> tuple[int, int]:

@@ -8,8 +8,9 @@ the last place of the inputs' type, 2^-8 bf16 / 2^-11 fp16; e = 2^-24 fp32):
   (the factor 2 for accumulators that truncate);
 * lse adds the exponentials' and the logarithm's own error, a few e of the
   magnitudes involved: 32 e (1 + |lse| + max |l|);
-* d = f (exp(l - lse) - 1) is rounded once to 16 bits and multiplied in fp32:
-  |error of dh| <= (u + 2 x error of a logit + 2 n e) |d|.|w| + u |dh|, n the
+* d = f (exp(l - lse) - 1) is rounded to 16 bits, p once before that where the
+  call keeps exponentials (2 u in all), and multiplied in fp32:
+  |error of dh| <= (2 u + 2 x error of a logit + 2 n e) |d|.|w| + u |dh|, n the
   length of the sum; dw the same with |d|^T.|h|.  |d| is taken as
   f (p + [v == t]): the subtraction's operands.  fp16 adds its smallest
   steps: 2^-25 / 1024 per d, 2^-25 per output (with the scale of the loss).
@@ -75,7 +76,7 @@ def _exact(torch, h, w, t, f=None):
         fp16 = h.dtype == torch.float16
         u = 2.0 ** -11 if fp16 else 2.0 ** -8
         step = (2.0 ** -25 / 1024 if fp16 else 0.0) * f.abs().max()
-        rel = u + 2 * lse_tol[:, None]
+        rel = 2 * u + 2 * lse_tol[:, None]
         out["dh"], out["dw"] = d @ wd, d.t() @ hd
         tiny = 2.0 ** -25 if fp16 else 0.0
         out["dh_tol"] = (rel + 2 * w.shape[0] * E) * (mag @ wd.abs()) + step * wd.abs().sum(0) + u * out["dh"].abs() + tiny
@@ -228,6 +229,24 @@ def test_workspace_least_and_dirty(ks, tile):
     with pytest.raises(N.KsError) as e:
         ops.linear_cross_entropy_grad(h, w, t, reduction="sum", cfg=cfg, workspace=_dirty(torch, least - 1))
     assert e.value.status == N.KS_ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_loss_of_one_large_logit(ks, dtype, tile):
+    """Logits of a few hundred, targets with probability near one: the loss is a
+    difference of nearly equal numbers and stays within the bound of an fp32 dot
+    product, the target's logit being the same number in both."""
+    N, ops, torch = ks
+    n, dim, vocab = 64, 2048, 1000
+    h, w, t = _make(torch, n, dim, vocab, _dt(torch, dtype), seed=31, lean=300.0)
+    loss, lse = ops.linear_cross_entropy(h, w, t, cfg=N.LinearCeConfig(tile, 0))
+    ref = _exact(torch, h, w, t)
+    _near(torch, lse, ref["lse"], ref["lse_tol"], "lse")
+    valid = ref["valid"]
+    # dot product: at most dim / 256 + 13 additions deep
+    tol = 32 * E * (1 + ref["lse"].abs()) + 24 * E * (h.double().abs() * w.double().abs()[t.clamp(min=0)]).sum(1)
+    _near(torch, loss[valid], ref["loss"][valid], 2 * tol[valid], "loss")
 
 
 def test_no_token_counts(ks):
