@@ -296,6 +296,40 @@ int ks_linear_ce_workspace_bytes(const ks_linear_ce_config *cfg, const ks_linear
                                  size_t limit, size_t *least, size_t *bytes);
 int ks_linear_ce_launch(const ks_linear_ce_config *cfg, const ks_linear_ce_args *args, void *stream);
 
+/* ---- embedding ------------------------------------------------------------
+ * out[i,:] = scale * table[tokens[i],:] in fp32, rounded once; a token outside
+ * [0, vocab) gives zeros (the rows of another shard of the table).  bf16,
+ * fp16 or fp32; row strides in elements, dense rows; tokens int64.  No
+ * counterpart in the reference.                                             */
+typedef struct ks_embedding_args {
+  const int64_t *tokens; int64_t tokens_count; const void *table; void *out;
+  int64_t vocab; int64_t dim; int64_t table_stride; int64_t out_stride;
+  int dtype; float scale;
+} ks_embedding_args;
+int ks_embedding_validate(const ks_embedding_args *args, char *reason, size_t reason_len);
+int ks_embedding_launch(const ks_embedding_args *args, void *stream);
+
+/* Gradient of the table: dtable[v,:] = scale * sum over tokens[i] == v of
+ * dout[i,:] (added to dtable's values if accumulate != 0; else every row is
+ * written, zeros where no token is).  fp32 sums in the order of the positions,
+ * one rounding; the same bits every time.  Tokens outside [0, vocab) and
+ * those equal to padding_idx have no part.  out_dtype: dout's type or fp32.
+ * cfg.chunk: sorted positions per warp, 1..32, 0 = chosen from the sizes.
+ * The workspace (256-byte aligned) holds the sorted tokens and the partial
+ * sums of tokens that lie in several chunks.                                 */
+typedef struct ks_embedding_grad_config { int chunk; } ks_embedding_grad_config;
+typedef struct ks_embedding_grad_args {
+  const int64_t *tokens; int64_t tokens_count; const void *dout; void *dtable;
+  int64_t vocab; int64_t dim; int64_t dout_stride; int64_t dtable_stride;
+  int dtype; int out_dtype; int accumulate; float scale; int64_t padding_idx;
+  void *workspace; size_t workspace_bytes;
+} ks_embedding_grad_args;
+int ks_embedding_grad_validate(const ks_embedding_grad_config *cfg, const ks_embedding_grad_args *args,
+                               char *reason, size_t reason_len);
+int ks_embedding_grad_workspace_bytes(const ks_embedding_grad_config *cfg, const ks_embedding_grad_args *args,
+                                      size_t *bytes);
+int ks_embedding_grad_launch(const ks_embedding_grad_config *cfg, const ks_embedding_grad_args *args, void *stream);
+
 /* ---- roofline peak probes (libs/bench/kernels/peaks.hip, driven by
  * tools/bench/main.cpp: kernscope-bench) ------------------------------------
  * Each enqueues one kernel on `stream` and returns at once; time them with

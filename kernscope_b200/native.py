@@ -111,6 +111,23 @@ class LinearCeArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class EmbeddingArgs(C.Structure):
+    _fields_ = [("tokens", C.c_void_p), ("tokens_count", C.c_int64), ("table", C.c_void_p), ("out", C.c_void_p),
+                ("vocab", C.c_int64), ("dim", C.c_int64), ("table_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("dtype", C.c_int), ("scale", C.c_float)]
+
+
+class EmbeddingGradConfig(C.Structure):
+    _fields_ = [("chunk", C.c_int)]
+
+
+class EmbeddingGradArgs(C.Structure):
+    _fields_ = [("tokens", C.c_void_p), ("tokens_count", C.c_int64), ("dout", C.c_void_p), ("dtable", C.c_void_p),
+                ("vocab", C.c_int64), ("dim", C.c_int64), ("dout_stride", C.c_int64), ("dtable_stride", C.c_int64),
+                ("dtype", C.c_int), ("out_dtype", C.c_int), ("accumulate", C.c_int), ("scale", C.c_float),
+                ("padding_idx", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 CONFIG_TYPES = {
     "softmax": SoftmaxConfig, "layernorm": LayerNormConfig, "bias_gelu": BiasGeluConfig,
     "reduction": ReductionConfig, "matmul": MatmulConfig, "flash_attention": FlashAttentionConfig,
@@ -166,6 +183,12 @@ PROTOTYPES = {
     "ks_linear_ce_workspace_bytes": (C.c_int, [_P(LinearCeConfig), _P(LinearCeArgs), C.c_size_t, _P(C.c_size_t),
                                                _P(C.c_size_t)]),
     "ks_linear_ce_launch": (C.c_int, [_P(LinearCeConfig), _P(LinearCeArgs), C.c_void_p]),
+    "ks_embedding_validate": (C.c_int, [_P(EmbeddingArgs), C.c_char_p, C.c_size_t]),
+    "ks_embedding_launch": (C.c_int, [_P(EmbeddingArgs), C.c_void_p]),
+    "ks_embedding_grad_validate": (C.c_int, [_P(EmbeddingGradConfig), _P(EmbeddingGradArgs), C.c_char_p, C.c_size_t]),
+    "ks_embedding_grad_workspace_bytes": (C.c_int, [_P(EmbeddingGradConfig), _P(EmbeddingGradArgs),
+                                                    _P(C.c_size_t)]),
+    "ks_embedding_grad_launch": (C.c_int, [_P(EmbeddingGradConfig), _P(EmbeddingGradArgs), C.c_void_p]),
     "ks_peak_sink_words": (C.c_int, [_P(C.c_size_t)]),
     "ks_peak_copy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "ks_peak_read": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
@@ -215,7 +238,7 @@ def validate(family: str, cfg, *shape_or_args) -> tuple[int, str]:
     """Run ks_<family>_validate; returns (status, reason)."""
     buf = C.create_string_buffer(512)
     fn = getattr(lib, f"ks_{family}_validate")
-    if family in ("reduction", "flash_attention", "linear_ce"):
+    if family in ("reduction", "flash_attention", "linear_ce", "embedding_grad"):
         st = fn(C.byref(cfg), C.byref(shape_or_args[0]), buf, 512)
     else:
         st = fn(C.byref(cfg), *[C.c_int64(v) for v in shape_or_args], buf, 512)

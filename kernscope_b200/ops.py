@@ -357,6 +357,63 @@ def linear_cross_entropy_grad(h, w, targets, ignore_index: int = -100, reduction
     return loss, dh, dw
 
 
+_TRAIN_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def embedding(tokens, table, scale: float = 1.0, out=None, stream=None) -> torch.Tensor:
+    """scale * table[tokens] (tokens int64 of any shape, table [vocab, dim] in
+    bf16, fp16 or fp32); tokens outside [0, vocab) give rows of zeros."""
+    _check_rows("table", table, _TRAIN_DTYPES)
+    _check_ids("tokens", tokens, tokens.numel(), table.device)
+    n, (vocab, dim) = tokens.numel(), table.shape
+    out = _empty((*tokens.shape, dim), table.dtype, table.device, stream) if out is None else out
+    if out.numel() != n * dim:
+        raise ValueError(f"out must hold {n} rows of {dim}")
+    rows = out if out.dim() == 2 else out.view(n, dim)
+    _check_rows("out", rows, (table.dtype,), table.device)
+    if n == 0:
+        return out
+    args = N.EmbeddingArgs(tokens.data_ptr(), n, table.data_ptr(), out.data_ptr(), vocab, dim, _row_stride(table),
+                           _row_stride(rows), _DT_TRAIN[table.dtype], scale)
+    N.check("ks_embedding_launch", N.lib.ks_embedding_launch(C.byref(args), _stream_ptr(stream)))
+    return out
+
+
+def embedding_backward(tokens, dout, vocab: int, scale: float = 1.0, padding_idx: int = -1, dtable=None, dtype=None,
+                       accumulate: bool = False, cfg=None, workspace=None, stream=None) -> torch.Tensor:
+    """Gradient of `embedding` with respect to its table: [vocab, dim] in dout's
+    type or fp32 (`dtype`, or that of `dtable`).  accumulate adds to `dtable`'s
+    values and touches the rows of `tokens` alone; otherwise every row is
+    written.  Tokens equal to padding_idx or outside [0, vocab) have no part."""
+    n = tokens.numel()
+    rows = dout if dout.dim() == 2 else dout.view(n, dout.shape[-1])
+    _check_rows("dout", rows, _TRAIN_DTYPES)
+    _check_ids("tokens", tokens, rows.shape[0], rows.device)
+    dim = rows.shape[1]
+    if dtable is None:
+        if accumulate:
+            raise ValueError("accumulate needs the dtable to add to")
+        dtable = _empty((vocab, dim), dtype or dout.dtype, rows.device, stream)
+    _check_rows("dtable", dtable, (dout.dtype, torch.float32), rows.device)
+    if tuple(dtable.shape) != (vocab, dim) or (dtype is not None and dtable.dtype != dtype):
+        raise ValueError(f"dtable must be [{vocab}, {dim}]" + (f" of {dtype}" if dtype is not None else ""))
+    if n == 0:
+        return dtable if accumulate else dtable.zero_()
+    args = N.EmbeddingGradArgs(tokens.data_ptr(), n, rows.data_ptr(), dtable.data_ptr(), vocab, dim, _row_stride(rows),
+                               _row_stride(dtable), _DT_TRAIN[dout.dtype], _DT_TRAIN[dtable.dtype], int(accumulate),
+                               scale, padding_idx)
+    cfg = cfg or N.EmbeddingGradConfig()
+    if workspace is None:
+        need = C.c_size_t(0)
+        N.check("ks_embedding_grad_workspace_bytes",
+                N.lib.ks_embedding_grad_workspace_bytes(C.byref(cfg), C.byref(args), C.byref(need)))
+        workspace = _empty(need.value, torch.uint8, rows.device, stream)
+    args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    N.check("ks_embedding_grad_launch",
+            N.lib.ks_embedding_grad_launch(C.byref(cfg), C.byref(args), _stream_ptr(stream)))
+    return dtable
+
+
 def device_error_take() -> int:
     w = C.c_int(0)
     N.check("ks_device_error_take", N.lib.ks_device_error_take(C.byref(w)))
