@@ -330,6 +330,27 @@ int ks_embedding_grad_workspace_bytes(const ks_embedding_grad_config *cfg, const
                                       size_t *bytes);
 int ks_embedding_grad_launch(const ks_embedding_grad_config *cfg, const ks_embedding_grad_args *args, void *stream);
 
+/* ---- gradient clipping ------------------------------------------------------
+ * norm = sqrt(sum of g^2 over all tensors) and out = g * min(1, max_norm /
+ * (norm + eps)), rounded once, for any number of dense tensors in bf16, fp16
+ * and fp32.  out may be the gradient itself (NULL stands for it) but may not
+ * overlap another tensor.  Squares are summed in fp32 over at most 32 values,
+ * then in fp64; the same bits every time.  A norm that is not finite gives
+ * what the formula gives.  No counterpart in the reference.
+ * ks_grad_clip_plan() (host only) writes the table of work for a set of
+ * tensors into host memory; `table` NULL asks for its size.  The caller
+ * copies it to the device once (32-byte aligned) and uses it as long as the
+ * tensors stay where they are.  ks_grad_clip_launch() reads the device copy.  */
+typedef struct ks_grad_tensor { const void *grad; void *out; int64_t numel; int dtype; } ks_grad_tensor;
+int ks_grad_clip_plan(const ks_grad_tensor *tensors, int64_t count, void *table, size_t table_bytes,
+                      size_t *bytes, int64_t *chunks);
+typedef struct ks_grad_clip_args {
+  const void *table; int64_t chunks; float max_norm; float eps; float *norm;
+  void *workspace; size_t workspace_bytes;
+} ks_grad_clip_args;
+int ks_grad_clip_workspace_bytes(int64_t chunks, size_t *bytes);
+int ks_grad_clip_launch(const ks_grad_clip_args *args, void *stream);
+
 /* ---- roofline peak probes (libs/bench/kernels/peaks.hip, driven by
  * tools/bench/main.cpp: kernscope-bench) ------------------------------------
  * Each enqueues one kernel on `stream` and returns at once; time them with

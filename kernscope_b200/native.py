@@ -128,6 +128,15 @@ class EmbeddingGradArgs(C.Structure):
                 ("padding_idx", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class GradTensor(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("numel", C.c_int64), ("dtype", C.c_int)]
+
+
+class GradClipArgs(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("chunks", C.c_int64), ("max_norm", C.c_float), ("eps", C.c_float),
+                ("norm", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 CONFIG_TYPES = {
     "softmax": SoftmaxConfig, "layernorm": LayerNormConfig, "bias_gelu": BiasGeluConfig,
     "reduction": ReductionConfig, "matmul": MatmulConfig, "flash_attention": FlashAttentionConfig,
@@ -189,6 +198,10 @@ PROTOTYPES = {
     "ks_embedding_grad_workspace_bytes": (C.c_int, [_P(EmbeddingGradConfig), _P(EmbeddingGradArgs),
                                                     _P(C.c_size_t)]),
     "ks_embedding_grad_launch": (C.c_int, [_P(EmbeddingGradConfig), _P(EmbeddingGradArgs), C.c_void_p]),
+    "ks_grad_clip_plan": (C.c_int, [_P(GradTensor), C.c_int64, C.c_void_p, C.c_size_t, _P(C.c_size_t),
+                                    _P(C.c_int64)]),
+    "ks_grad_clip_workspace_bytes": (C.c_int, [C.c_int64, _P(C.c_size_t)]),
+    "ks_grad_clip_launch": (C.c_int, [_P(GradClipArgs), C.c_void_p]),
     "ks_peak_sink_words": (C.c_int, [_P(C.c_size_t)]),
     "ks_peak_copy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "ks_peak_read": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),

@@ -414,6 +414,58 @@ def embedding_backward(tokens, dout, vocab: int, scale: float = 1.0, padding_idx
     return dtable
 
 
+class GradClipper:
+    """Global norm and clipping of a fixed set of gradients.
+
+    `grads`: dense CUDA tensors in bf16, fp16 or fp32; `out`: where the scaled
+    gradients go, one tensor of the same type and size each (default: in place).
+    The table of work is made once, here, and holds the tensors' addresses: make
+    a new clipper when gradients move.  ``clip(max_norm)`` enqueues both passes
+    and returns the norm before clipping (fp32, one value, on the device).
+    """
+
+    def __init__(self, grads, out=None):
+        self.grads = list(grads)
+        self.out = self.grads if out is None else list(out)
+        if len(self.out) != len(self.grads):
+            raise ValueError("grads and out differ in length")
+        if not self.grads:
+            raise ValueError("no gradients")
+        self.device = self.grads[0].device
+        for g, o in zip(self.grads, self.out):
+            for t in (g, o):
+                if not (t.is_cuda and t.device == self.device and t.dtype in _DT_TRAIN and t.is_contiguous()):
+                    raise ValueError("gradients must be contiguous bf16, fp16 or fp32 tensors on one CUDA device")
+            if o.dtype != g.dtype or o.numel() != g.numel():
+                raise ValueError("an output differs in type or size from its gradient")
+        spans = sorted({(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i)
+                        for i, pair in enumerate(zip(self.grads, self.out)) for t in pair if t.numel()})
+        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+            raise ValueError("gradients (or outputs) overlap")
+        n = len(self.grads)
+        tensors = (N.GradTensor * n)(*[N.GradTensor(g.data_ptr(), o.data_ptr(), g.numel(), _DT_TRAIN[g.dtype])
+                                       for g, o in zip(self.grads, self.out)])
+        size, chunks = C.c_size_t(0), C.c_int64(0)
+        N.check("ks_grad_clip_plan", N.lib.ks_grad_clip_plan(tensors, n, None, 0, C.byref(size), C.byref(chunks)))
+        host = torch.empty(max(32, size.value), dtype=torch.uint8)
+        N.check("ks_grad_clip_plan", N.lib.ks_grad_clip_plan(tensors, n, host.data_ptr(), host.numel(), C.byref(size),
+                                                             C.byref(chunks)))
+        need = C.c_size_t(0)
+        N.check("ks_grad_clip_workspace_bytes", N.lib.ks_grad_clip_workspace_bytes(chunks.value, C.byref(need)))
+        self._table = host.to(self.device)
+        self._need, self._chunks = need.value, chunks.value
+
+    def clip(self, max_norm: float, eps: float = 1e-6, stream=None) -> torch.Tensor:
+        if self.device.index != torch.cuda.current_device():
+            raise ValueError(f"the gradients are on {self.device}, not on the current device")
+        norm = _empty(1, torch.float32, self.device, stream)
+        ws = _empty(self._need, torch.uint8, self.device, stream)
+        args = N.GradClipArgs(self._table.data_ptr(), self._chunks, max_norm, eps, norm.data_ptr(), ws.data_ptr(),
+                              self._need)
+        N.check("ks_grad_clip_launch", N.lib.ks_grad_clip_launch(C.byref(args), _stream_ptr(stream)))
+        return norm
+
+
 def device_error_take() -> int:
     w = C.c_int(0)
     N.check("ks_device_error_take", N.lib.ks_device_error_take(C.byref(w)))
