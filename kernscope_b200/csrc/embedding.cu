@@ -9,8 +9,8 @@
 // of the tokens brings equal ones together, then each warp walks `chunk`
 // consecutive sorted positions over one segment of columns, adding in fp32
 // and writing a row when its token ends.  A token whose positions lie in
-// several chunks leaves an fp32 partial sum per chunk, and a second kernel
-// adds those in order.  No floating-point atomics.
+// several chunks leaves an fp32 partial sum per chunk, and the warp that
+// finishes last adds those in order.  No floating-point atomics.
 #include <algorithm>
 #include <cuda_fp16.h>
 
@@ -129,28 +129,50 @@ constexpr int kCluster = 8;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 
-KS_DEV void zero_span(char *p, int64_t bytes, int64_t first, int64_t step) {  // bytes even, p 2-byte aligned
+constexpr int kZeroBytes = 32 * 1024;  // one bulk store of zeros
+
+KS_DEV void bulk_store(void *dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
+               "r"(ks_smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+// Zeros over [p, p + bytes) (p and bytes even), the pieces of kZeroBytes dealt
+// out over `ctas` CTAs; the even bytes before and after whole 16-byte words by
+// the first of them.
+KS_DEV void zero_span(char *p, int64_t bytes, const void *zeros, int64_t cta, int64_t ctas) {
   const int64_t head = min(bytes, int64_t((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15));
-  const int64_t vecs = (bytes - head) / 16, tail = bytes - head - vecs * 16;
-  uint4 *v = reinterpret_cast<uint4 *>(p + head);
-  for (int64_t i = first; i < vecs; i += step) v[i] = make_uint4(0, 0, 0, 0);
-  if (first < head / 2) reinterpret_cast<uint16_t *>(p)[first] = 0;
-  if (first < tail / 2) reinterpret_cast<uint16_t *>(p + bytes - tail)[first] = 0;
+  const int64_t body = (bytes - head) / 16 * 16, tail = bytes - head - body;
+  if (threadIdx.x == 0)
+    for (int64_t at = cta * kZeroBytes; at < body; at += ctas * kZeroBytes)
+      bulk_store(p + head + at, zeros, uint32_t(min(body - at, int64_t(kZeroBytes))));
+  if (cta == 0 && threadIdx.x < head / 2) reinterpret_cast<uint16_t *>(p)[threadIdx.x] = 0;
+  if (cta == 0 && threadIdx.x < tail / 2) reinterpret_cast<uint16_t *>(p + bytes - tail)[threadIdx.x] = 0;
 }
 
 __global__ void __launch_bounds__(kSortThreads, 1)
     emb_sort_kernel(const int64_t *__restrict__ tokens, int64_t n, int64_t vocab, int64_t padding, int passes, int bits,
-                    uint2 *buf0, uint2 *buf1, char *zero, int64_t zero_rows, int64_t zero_bytes, int64_t zero_stride) {
+                    uint2 *buf0, uint2 *buf1, uint32_t *counters, int64_t counters_n, char *zero, int64_t zero_rows,
+                    int64_t zero_bytes, int64_t zero_stride) {
+  extern __shared__ __align__(16) uint32_t sh[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) ks_pdl_release();
   if (blockIdx.x >= kCluster) {
     const int64_t ctas = gridDim.x - kCluster, cta = blockIdx.x - kCluster;
+    for (int i = tid; i < kZeroBytes / 16; i += kSortThreads) reinterpret_cast<uint4 *>(sh)[i] = make_uint4(0, 0, 0, 0);
+    ks_fence_proxy_async();
+    __syncthreads();
     if (zero_rows == 1)
-      zero_span(zero, zero_bytes, cta * kSortThreads + tid, ctas * kSortThreads);
+      zero_span(zero, zero_bytes, sh, cta, ctas);
     else
-      for (int64_t r = cta; r < zero_rows; r += ctas) zero_span(zero + r * zero_stride, zero_bytes, tid, kSortThreads);
+      for (int64_t r = cta; r < zero_rows; r += ctas) zero_span(zero + r * zero_stride, zero_bytes, sh, 0, 1);
+    if (tid == 0) {
+      ks_bulk_commit_group();
+      ks_bulk_wait_all();
+    }
     return;
   }
-  extern __shared__ uint32_t sh[];
+  for (int64_t i = int64_t(blockIdx.x) * kSortThreads + tid; i < counters_n; i += kCluster * kSortThreads) counters[i] = 0;
   const int bins = 1 << bits;
   uint32_t *count = sh;                     // [warp][bin]: counts, then this warp's first rank in the CTA
   uint32_t *cta_count = sh + kSortWarps * bins;  // [bin], read by the whole cluster
@@ -252,14 +274,35 @@ struct Sum {
   }
   KS_DEV static int64_t col(int j, int lane) { return VEC ? lane * W + j : lane + j * 32; }
   KS_DEV void put_part(float *p, int64_t c, int64_t dim, int lane) const {
+    if constexpr (VEC) {
+      if (c + lane * W < dim) {
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (c + col(j, lane) < dim) p[c + col(j, lane)] = a[j];
+        for (int j = 0; j < W; j += 4)
+          *reinterpret_cast<float4 *>(p + c + lane * W + j) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if (c + col(j, lane) < dim) p[c + col(j, lane)] = a[j];
+    }
   }
   KS_DEV void add_part(const float *p, int64_t c, int64_t dim, int lane) {
+    if constexpr (VEC) {
+      if (c + lane * W < dim) {
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (c + col(j, lane) < dim) a[j] += __ldcg(p + c + col(j, lane));
+        for (int j = 0; j < W; j += 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + c + lane * W + j));
+          a[j] += v.x;
+          a[j + 1] += v.y;
+          a[j + 2] += v.z;
+          a[j + 3] += v.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        if (c + col(j, lane) < dim) a[j] += __ldcg(p + c + col(j, lane));
+    }
   }
   KS_DEV void finish(typename O::T *row, int64_t c, int64_t dim, int lane, float scale, bool accumulate) {
     Raw<ODT, W, VEC> o;
@@ -270,27 +313,106 @@ struct Sum {
   }
 };
 
+// What every warp of a launch shares.
+template <int DT, int ODT>
+struct GradArgs {
+  const uint2 *sorted;
+  int64_t n;
+  int chunk;
+  const typename Elem<DT>::T *dout;
+  int64_t dout_stride;
+  typename Elem<ODT>::T *dtable;
+  int64_t dtable_stride, vocab, dim;
+  float scale;
+  int accumulate;
+  float *part;
+  int64_t ld;
+  uint32_t *arrived;  // [chunk][2][segment] warps of a group that left their partials, [chunk][segment] groups
+  int64_t chunks;
+};
+
+constexpr int64_t kGroup = 64;  // chunks whose partials one warp adds up
+
+// A token of which this warp (chunk ch, segment seg) has just left a partial
+// sum, in slot 1 if it begins here, goes on elsewhere.  The last of the warps
+// that hold a part of it, within each group of 64 chunks, adds the group's
+// partials in order; the last group adds the groups'.  So the order of the sum
+// is that of the chunks, whoever comes last, and a token that fills the whole
+// batch (131072 positions: 4096 partials) is joined in two short chains.
 template <int DT, int ODT, bool VEC>
-__global__ void __launch_bounds__(256)
-    emb_grad_kernel(const uint2 *__restrict__ sorted, int64_t n, int chunk, const typename Elem<DT>::T *__restrict__ dout,
-                    int64_t dout_stride, typename Elem<ODT>::T *dtable, int64_t dtable_stride, int64_t vocab,
-                    int64_t dim, float scale, int accumulate, float *__restrict__ part, int64_t ld) {
+KS_DEV void join(const GradArgs<DT, ODT> &g, uint32_t key, int64_t ch, int64_t seg, int64_t segs, bool begins, bool goes_on,
+                 int lane) {
+  using S = Sum<DT, ODT, VEC>;
+  const int64_t c = seg * S::kSeg;
+  int64_t a = ch, b = ch;  // the token's first and last chunk
+  if (!begins) {
+    for (int64_t j = ch - 1;; j -= 32) {  // lane l: does it begin before chunk j - l?
+      const int64_t at = (j - lane) * g.chunk;
+      const bool on = at > 0 && __ldcg(&g.sorted[at - 1].x) == key;
+      const uint32_t stop = __ballot_sync(0xffffffffu, !on);
+      if (stop) {
+        a = j - (__ffs(stop) - 1);
+        break;
+      }
+    }
+  }
+  if (goes_on) {
+    for (int64_t j = ch + 1;; j += 32) {  // lane l: does it go on past chunk j + l?
+      const int64_t end = (j + lane + 1) * g.chunk;
+      const bool on = end < g.n && __ldcg(&g.sorted[end].x) == key;
+      const uint32_t stop = __ballot_sync(0xffffffffu, !on);
+      if (stop) {
+        b = j + (__ffs(stop) - 1);
+        break;
+      }
+    }
+  }
+  auto slot = [&](int64_t chunk) { return g.part + (chunk * 2 + (chunk == a ? 1 : 0)) * g.ld; };
+  auto last_of = [&](uint32_t *counter, int64_t expected) {
+    __threadfence();
+    __syncwarp();
+    uint32_t before = 0;
+    if (lane == 0) before = atomicAdd(counter, 1u);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    __threadfence();
+    return int64_t(before) == expected - 1;
+  };
+  const int64_t first = max(a, ch / kGroup * kGroup), last = min(b, ch / kGroup * kGroup + kGroup - 1);
+  if (!last_of(g.arrived + (first * 2 + (first == a ? 1 : 0)) * segs + seg, last - first + 1)) return;
+  S sum;
+  sum.clear();
+#pragma unroll 4
+  for (int64_t j = first; j <= last; ++j) sum.add_part(slot(j), c, g.dim, lane);
+  const int64_t ga = a / kGroup, gb = b / kGroup;
+  if (ga != gb) {
+    sum.put_part(slot(first), c, g.dim, lane);
+    if (!last_of(g.arrived + g.chunks * 2 * segs + a * segs + seg, gb - ga + 1)) return;
+    sum.clear();
+#pragma unroll 4
+    for (int64_t j = ga; j <= gb; ++j) sum.add_part(slot(max(a, j * kGroup)), c, g.dim, lane);
+  }
+  sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, lane, g.scale, g.accumulate != 0);
+}
+
+template <int DT, int ODT, bool VEC>
+__global__ void __launch_bounds__(256) emb_grad_kernel(const __grid_constant__ GradArgs<DT, ODT> g) {
   using S = Sum<DT, ODT, VEC>;
   constexpr int U = 8;
+  ks_pdl_wait();
   const int lane = threadIdx.x & 31;
-  const int64_t segs = (dim + S::kSeg - 1) / S::kSeg;
+  const int64_t segs = (g.dim + S::kSeg - 1) / S::kSeg;
   const int64_t id = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t ch = id / segs, c = (id - ch * segs) * S::kSeg;
-  const int64_t lo = ch * chunk;
-  if (lo >= n) return;
-  const int cnt = int(min(int64_t(chunk), n - lo));
+  const int64_t ch = id / segs, seg = id - ch * segs, c = seg * S::kSeg;
+  const int64_t lo = ch * g.chunk;
+  if (lo >= g.n) return;
+  const int cnt = int(min(int64_t(g.chunk), g.n - lo));
   uint2 kv = make_uint2(0, 0);
-  if (lane < cnt) kv = __ldg(sorted + lo + lane);
+  if (lane < cnt) kv = __ldcg(g.sorted + lo + lane);
   const uint32_t none = 0xffffffffu;  // no token: vocab < 2^31
-  const uint32_t prev = lo > 0 ? __ldg(&sorted[lo - 1].x) : none;
-  const uint32_t next = lo + cnt < n ? __ldg(&sorted[lo + cnt].x) : none;
+  const uint32_t prev = lo > 0 ? __ldcg(&g.sorted[lo - 1].x) : none;
+  const uint32_t next = lo + cnt < g.n ? __ldcg(&g.sorted[lo + cnt].x) : none;
   bool from_before = prev == __shfl_sync(0xffffffffu, kv.x, 0);
-  float *slots = part + ch * 2 * ld;
+  float *slots = g.part + ch * 2 * g.ld;
   S sum;
   sum.clear();
   for (int i0 = 0; i0 < cnt; i0 += U) {
@@ -299,63 +421,30 @@ __global__ void __launch_bounds__(256)
     for (int u = 0; u < U; ++u) {
       const uint32_t key = __shfl_sync(0xffffffffu, kv.x, (i0 + u) & 31);
       const int64_t pos = __shfl_sync(0xffffffffu, kv.y, (i0 + u) & 31);
-      const bool take = i0 + u < cnt && key < vocab;
-      x[u].load(dout + (take ? pos * dout_stride : 0) + c, c, take ? dim : 0, lane);
+      const bool take = i0 + u < cnt && key < g.vocab;
+      x[u].load(g.dout + (take ? pos * g.dout_stride : 0) + c, c, take ? g.dim : 0, lane);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u;
       if (i >= cnt) break;
       const uint32_t key = __shfl_sync(0xffffffffu, kv.x, i);
-      if (key >= vocab) return;  // the excluded tokens come last
+      if (key >= g.vocab) return;  // the excluded tokens come last
       const uint32_t after = i + 1 < cnt ? __shfl_sync(0xffffffffu, kv.x, (i + 1) & 31) : next;
 #pragma unroll
       for (int j = 0; j < S::W; ++j) sum.a[j] += S::E::get(x[u].v[j]);
       if (after != key || i + 1 == cnt) {
-        if (from_before)
-          sum.put_part(slots, c, dim, lane);
-        else if (after == key)
-          sum.put_part(slots + ld, c, dim, lane);
-        else
-          sum.finish(dtable + int64_t(key) * dtable_stride, c, dim, lane, scale, accumulate != 0);
+        if (from_before || after == key) {
+          sum.put_part(from_before ? slots : slots + g.ld, c, g.dim, lane);
+          join<DT, ODT, VEC>(g, key, ch, seg, segs, !from_before, after == key, lane);
+        } else {
+          sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, lane, g.scale, g.accumulate != 0);
+        }
         sum.clear();
         from_before = false;
       }
     }
   }
-}
-
-// Tokens that lie in several chunks: the warp of the chunk that a token begins
-// in adds its tail and the later chunks' heads, in order.
-template <int DT, int ODT, bool VEC>
-__global__ void __launch_bounds__(256)
-    emb_join_kernel(const uint2 *__restrict__ sorted, int64_t n, int chunk, typename Elem<ODT>::T *dtable,
-                    int64_t dtable_stride, int64_t vocab, int64_t dim, float scale, int accumulate,
-                    const float *__restrict__ part, int64_t ld) {
-  using S = Sum<DT, ODT, VEC>;
-  const int lane = threadIdx.x & 31;
-  const int64_t segs = (dim + S::kSeg - 1) / S::kSeg;
-  const int64_t id = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t ch = id / segs, c = (id - ch * segs) * S::kSeg;
-  const int64_t lo = ch * chunk, hi = lo + chunk;
-  if (hi >= n) return;
-  const uint32_t key = __ldg(&sorted[hi - 1].x);
-  if (__ldg(&sorted[hi].x) != key || key >= vocab) return;
-  if (lo > 0 && __ldg(&sorted[lo - 1].x) == key) return;  // begins earlier
-  S sum;
-  sum.clear();
-  sum.add_part(part + (ch * 2 + 1) * ld, c, dim, lane);
-  for (int64_t first = ch + 1;; first += 32) {
-    // lane l looks at chunk first + l: does the token go on past it?
-    const int64_t end = (first + lane + 1) * chunk;
-    const bool on = end < n && __ldg(&sorted[end].x) == key;
-    const uint32_t stops = __ballot_sync(0xffffffffu, !on);
-    const int many = stops ? __ffs(stops) : 32;
-#pragma unroll 4
-    for (int j = 0; j < many; ++j) sum.add_part(part + (first + j) * 2 * ld, c, dim, lane);
-    if (stops) break;
-  }
-  sum.finish(dtable + int64_t(key) * dtable_stride, c, dim, lane, scale, accumulate != 0);
 }
 
 // ---------------------------------------------------------------------------
@@ -386,7 +475,8 @@ struct GradPlan {
   int chunk;
   int64_t chunks, ld;
   int bits, passes;
-  size_t o_buf0, o_buf1, o_part, bytes;
+  int64_t counters;
+  size_t o_buf0, o_buf1, o_count, o_part, bytes;
 };
 
 int grad_check(const ks_embedding_grad_config &c, const ks_embedding_grad_args &a, char *reason, size_t len) {
@@ -412,11 +502,11 @@ GradPlan grad_plan(const ks_embedding_grad_config &c, const ks_embedding_grad_ar
   GradPlan p;
   const int64_t n = a.tokens_count;
   const int64_t segs = (a.dim * elem_size(a.dtype) + 511) / 512;
-  // 32 positions a warp where that leaves 8 warps for every SM, fewer positions otherwise
+  // 32 positions a warp where that leaves 16 warps for every SM, fewer positions otherwise
   p.chunk = c.chunk;
   if (p.chunk == 0) {
     p.chunk = 32;
-    while (p.chunk > 4 && (n + p.chunk - 1) / p.chunk * segs < 8LL * ks::sm_count()) p.chunk /= 2;
+    while (p.chunk > 4 && (n + p.chunk - 1) / p.chunk * segs < 16LL * ks::sm_count()) p.chunk /= 2;
   }
   p.chunks = (n + p.chunk - 1) / p.chunk;
   p.ld = (a.dim + 63) / 64 * 64;
@@ -432,6 +522,9 @@ GradPlan grad_plan(const ks_embedding_grad_config &c, const ks_embedding_grad_ar
   };
   p.o_buf0 = take(size_t(n) * 8);
   p.o_buf1 = take(p.passes > 1 ? size_t(n) * 8 : 0);
+  // (segments of the narrower lane-strided path are as many: 512 bytes or 32 x per elements alike)
+  p.counters = p.chunks * 3 * segs;
+  p.o_count = take(size_t(p.counters) * 4);
   p.o_part = take(size_t(p.chunks) * 2 * p.ld * 4);
   p.bytes = o;
   return p;
@@ -443,17 +536,24 @@ int grad_launch(const ks_embedding_grad_args &a, const GradPlan &p, cudaStream_t
   using T = typename Elem<DT>::T;
   using O = typename Elem<ODT>::T;
   char *ws = static_cast<char *>(a.workspace);
-  auto sorted = reinterpret_cast<const uint2 *>(ws + (p.passes & 1 ? p.o_buf0 : p.o_buf1));
-  auto part = reinterpret_cast<float *>(ws + p.o_part);
+  const GradArgs<DT, ODT> g = {reinterpret_cast<const uint2 *>(ws + (p.passes & 1 ? p.o_buf0 : p.o_buf1)),
+                               a.tokens_count,
+                               p.chunk,
+                               static_cast<const T *>(a.dout),
+                               a.dout_stride,
+                               static_cast<O *>(a.dtable),
+                               a.dtable_stride,
+                               a.vocab,
+                               a.dim,
+                               a.scale,
+                               a.accumulate,
+                               reinterpret_cast<float *>(ws + p.o_part),
+                               p.ld,
+                               reinterpret_cast<uint32_t *>(ws + p.o_count),
+                               p.chunks};
   const int64_t segs = (a.dim + S::kSeg - 1) / S::kSeg, blocks = (p.chunks * segs + 7) / 8;
   if (blocks > 0x7fffffff) return KS_ERR_INVALID_ARGS;
-  emb_grad_kernel<DT, ODT, VEC><<<unsigned(blocks), 256, 0, st>>>(
-      sorted, a.tokens_count, p.chunk, static_cast<const T *>(a.dout), a.dout_stride, static_cast<O *>(a.dtable),
-      a.dtable_stride, a.vocab, a.dim, a.scale, a.accumulate, part, p.ld);
-  emb_join_kernel<DT, ODT, VEC><<<unsigned(blocks), 256, 0, st>>>(sorted, a.tokens_count, p.chunk,
-                                                                  static_cast<O *>(a.dtable), a.dtable_stride, a.vocab,
-                                                                  a.dim, a.scale, a.accumulate, part, p.ld);
-  return ks::map_cuda(cudaGetLastError());
+  return ks::launch_kernel(true, emb_grad_kernel<DT, ODT, VEC>, dim3(unsigned(blocks)), dim3(256), 0, st, g);
 }
 
 template <int DT, int ODT>
@@ -472,13 +572,8 @@ int lookup_launch(const ks_embedding_args &a, cudaStream_t st) {
   const int grid = int(std::min<int64_t>((total + 7) / 8, int64_t(ks::sm_count()) * 64));
   auto t = static_cast<const T *>(a.table);
   auto o = static_cast<T *>(a.out);
-  if (vec)
-    emb_lookup_kernel<DT, true><<<grid, 256, 0, st>>>(a.tokens, a.tokens_count, t, a.table_stride, o, a.out_stride,
-                                                      a.vocab, a.dim, a.scale);
-  else
-    emb_lookup_kernel<DT, false><<<grid, 256, 0, st>>>(a.tokens, a.tokens_count, t, a.table_stride, o, a.out_stride,
-                                                       a.vocab, a.dim, a.scale);
-  return ks::map_cuda(cudaGetLastError());
+  return ks::launch_kernel(false, vec ? emb_lookup_kernel<DT, true> : emb_lookup_kernel<DT, false>, dim3(grid), dim3(256), 0, st,
+                         a.tokens, a.tokens_count, t, a.table_stride, o, a.out_stride, a.vocab, a.dim, a.scale);
 }
 
 }  // namespace
@@ -548,7 +643,7 @@ int ks_embedding_grad_launch(const ks_embedding_grad_config *cfg, const ks_embed
     zero_ctas = unsigned(std::min<int64_t>(want, ks::sm_count() - kCluster));
     zero_ctas = std::max(1u, zero_ctas / kCluster) * kCluster;
   }
-  const size_t shm = (size_t(kSortWarps) + 2) * (size_t(1) << p.bits) * 4;
+  const size_t shm = std::max<size_t>((size_t(kSortWarps) + 2) * (size_t(1) << p.bits) * 4, kZeroBytes);
   cudaError_t e = cudaFuncSetAttribute(emb_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shm));
   if (e != cudaSuccess) return ks::map_cuda(e);
   cudaLaunchAttribute attr[1];
@@ -565,7 +660,7 @@ int ks_embedding_grad_launch(const ks_embedding_grad_config *cfg, const ks_embed
   lc.numAttrs = 1;
   e = cudaLaunchKernelEx(&lc, emb_sort_kernel, a->tokens, a->tokens_count, a->vocab, a->padding_idx, p.passes, p.bits,
                          reinterpret_cast<uint2 *>(ws + p.o_buf0), reinterpret_cast<uint2 *>(ws + p.o_buf1),
-                         static_cast<char *>(a->dtable), zrows, zbytes, a->dtable_stride * osz);
+                         reinterpret_cast<uint32_t *>(ws + p.o_count), p.counters, static_cast<char *>(a->dtable), zrows, zbytes, a->dtable_stride * osz);
   if (e != cudaSuccess) return ks::map_cuda(e);
   if (a->dtype == KS_BF16)
     return a->out_dtype == KS_F32 ? grad_launch_vec<KS_BF16, KS_F32>(*a, p, st)

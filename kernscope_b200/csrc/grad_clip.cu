@@ -114,18 +114,27 @@ KS_DEV void scale_chunk(const Chunk &c, float k) {
   const int head = head_of<DT>(g, c.count), vecs = (c.count - head) / Y::per, tail = c.count - head - vecs * Y::per;
   auto v = reinterpret_cast<const uint4 *>(g + head);
   const bool same = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < vecs; i += kThreads) {
-    float f[8];
-    unpack<DT>(v[i], f);
-    typename Y::T y[Y::per];
+  constexpr int U = 4;  // loads in flight: a store to `out` keeps the compiler from moving loads past it
+  for (int i0 = threadIdx.x; i0 < vecs; i0 += U * kThreads) {
+    uint4 x[U];
 #pragma unroll
-    for (int j = 0; j < Y::per; ++j) y[j] = Y::put(f[j] * k);
-    if (same) {
-      *reinterpret_cast<uint4 *>(o + head + i * Y::per) = *reinterpret_cast<const uint4 *>(y);
-    } else {
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * kThreads < vecs) x[u] = v[i0 + u * kThreads];
 #pragma unroll
-      for (int j = 0; j < Y::per; ++j) o[head + i * Y::per + j] = y[j];
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads;
+      if (i >= vecs) break;
+      float f[8];
+      unpack<DT>(x[u], f);
+      alignas(16) typename Y::T y[Y::per];
+#pragma unroll
+      for (int j = 0; j < Y::per; ++j) y[j] = Y::put(f[j] * k);
+      if (same) {
+        *reinterpret_cast<uint4 *>(o + head + i * Y::per) = *reinterpret_cast<const uint4 *>(y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < Y::per; ++j) o[head + i * Y::per + j] = y[j];
+      }
     }
   }
   if (int(threadIdx.x) < head) o[threadIdx.x] = Y::put(Y::get(g[threadIdx.x]) * k);
@@ -149,6 +158,7 @@ KS_DEV double block_sum(double v, double *sh) {
 __global__ void __launch_bounds__(kThreads) clip_norm_kernel(const Chunk *__restrict__ table, int64_t chunks,
                                                              double *__restrict__ partial) {
   __shared__ double sh[32];
+  ks_pdl_release();
   double acc = 0.0;
   for (int64_t i = blockIdx.x; i < chunks; i += gridDim.x) {
     const Chunk c = table[i];
@@ -164,8 +174,9 @@ __global__ void __launch_bounds__(kThreads)
     clip_scale_kernel(const Chunk *__restrict__ table, int64_t chunks, const double *__restrict__ partial, int partials,
                       float max_norm, float eps, float *__restrict__ norm_out) {
   __shared__ double sh[32];
+  ks_pdl_wait();
   double acc = 0.0;
-  for (int i = threadIdx.x; i < partials; i += kThreads) acc += partial[i];
+  for (int i = threadIdx.x; i < partials; i += kThreads) acc += __ldcg(partial + i);
   const float norm = float(sqrt(block_sum(acc, sh)));
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
   const float r = max_norm / (norm + eps);
@@ -237,9 +248,10 @@ int ks_grad_clip_launch(const ks_grad_clip_args *a, void *stream) {
   const int grid = int(std::max<int64_t>(1, std::min(a->chunks, most)));
   auto table = static_cast<const Chunk *>(a->table);
   auto partial = static_cast<double *>(a->workspace);
-  clip_norm_kernel<<<grid, kThreads, 0, st>>>(table, a->chunks, partial);
-  clip_scale_kernel<<<grid, kThreads, 0, st>>>(table, a->chunks, partial, grid, a->max_norm, a->eps, a->norm);
-  return ks::map_cuda(cudaGetLastError());
+  s = ks::launch_kernel(false, clip_norm_kernel, dim3(grid), dim3(kThreads), 0, st, table, a->chunks, partial);
+  if (s != KS_OK) return s;
+  return ks::launch_kernel(true, clip_scale_kernel, dim3(grid), dim3(kThreads), 0, st, table, a->chunks, partial, grid, a->max_norm,
+                         a->eps, a->norm);
 }
 
 }  // extern "C"

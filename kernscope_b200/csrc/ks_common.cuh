@@ -76,6 +76,20 @@ KS_DEV double ks_warp_sum_f64(double v) {
 }
 
 // ---------------------------------------------------------------------------
+// Programmatic dependent launch, between the kernels of one call: a kernel lets
+// its successor be launched early (its CTAs take their places as SMs free up,
+// and set themselves up), and the successor waits for the completion of its
+// predecessor, memory included, before it reads or writes global memory.  The
+// first kernel of a call is launched plainly and the last does not release, so
+// that the caller's own kernels before and after see ordinary stream order and
+// a call's inputs are constant while its kernels run; what one kernel of a call
+// writes and the next reads is loaded past L1 (__ldcg), since the reader may
+// have been started before the writer finished.
+// ---------------------------------------------------------------------------
+KS_DEV void ks_pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+KS_DEV void ks_pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---------------------------------------------------------------------------
 // Shared-memory addresses, mbarriers, fences
 // ---------------------------------------------------------------------------
 KS_DEV uint32_t ks_smem_u32(const void *p) {
@@ -459,4 +473,21 @@ int symbol_address(const void *symbol, void **out);
 // address resolved once per device, limit from ks_set_wait_limit_ns).
 KsWait wait_ctx();
 void set_reason(char *buf, size_t len, const char *fmt, ...);
+
+// Launch `kernel`; `next`: as the successor of this call's previous kernel, it
+// may be set up while that one still runs and calls ks_pdl_wait() itself.
+template <typename... P, typename... A>
+int launch_kernel(bool next, void (*kernel)(P...), dim3 grid, dim3 block, size_t shm, cudaStream_t st, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = grid;
+  lc.blockDim = block;
+  lc.dynamicSmemBytes = shm;
+  lc.stream = st;
+  lc.attrs = attr;
+  lc.numAttrs = next ? 1 : 0;
+  return map_cuda(cudaLaunchKernelEx(&lc, kernel, static_cast<P>(args)...));
+}
 }  // namespace ks

@@ -85,6 +85,7 @@ struct CeGemm {
   CeScalars *sc;
   // DH
   int out_f32, accumulate;
+  int release;            // another kernel of the call follows
 };
 
 template <int BN, int STAGES, int ACC, int MH>
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ks_prefetch_tmap(&tma_a);
     ks_prefetch_tmap(&tma_b);
     if (MODE != STATS) ks_prefetch_tmap(&tma_c);
-    if ((MODE == STATS || MODE == STORE) && blockIdx.x == 0) p.sc->counter = 0;  // for the combine kernel that follows
+    if (p.release) ks_pdl_release();
   }
   if (warp == 1) {
     ks_tmem_alloc(tmem_slot, L::tmem_cols);
@@ -219,6 +220,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   ks_tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  ks_pdl_wait();
+  if ((MODE == STATS || MODE == STORE) && blockIdx.x == 0 && threadIdx.x == 0)
+    p.sc->counter = 0;  // for the combine kernel that follows
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------ producer
@@ -347,8 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *stg = smem + L::c_off + (warp - 2) * 2 * kCBuf;
     const bool f16 = p.f16 != 0;
     float escale = 1.f, fscale = 1.f;
-    if (MODE == DH || MODE == DW) escale = p.sc->escale;
-    if (MODE == PROB) fscale = p.sc->fscale;
+    if (MODE == DH || MODE == DW) escale = __ldcg(&p.sc->escale);
+    if (MODE == PROB) fscale = __ldcg(&p.sc->fscale);
     int i = 0;
     uint32_t nstore = 0;
     for (int t = blockIdx.x; t < num_work; t += gridDim.x, ++i) {
@@ -374,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (c >= 0 && c < BN) tcol[h] = int(c);
               if (MODE == PROB) f[h] = p.dloss ? p.dloss[row] * fscale : fscale;
             }
-            if (MODE == PROB) lse2[h] = p.lse[row] * kLog2e;
+            if (MODE == PROB) lse2[h] = __ldcg(p.lse + row) * kLog2e;
           }
         }
       }
@@ -524,7 +528,7 @@ KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool 
     for (; k + 8 <= dim; k += 256) {
       const int64_t at = k + lane * 8;
       if (at + 8 > dim) continue;
-      const uint4 x = *reinterpret_cast<const uint4 *>(h + at), y = *reinterpret_cast<const uint4 *>(w + at);
+      const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(h + at)), y = __ldcg(reinterpret_cast<const uint4 *>(w + at));
       a0 = fmaf(val(x.x, 0), val(y.x, 0), a0);
       a1 = fmaf(val(x.x, 1), val(y.x, 1), a1);
       a0 = fmaf(val(x.y, 0), val(y.y, 0), a0);
@@ -536,7 +540,7 @@ KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool 
     }
     k = dim / 8 * 8;
   }
-  for (k += lane; k < dim; k += 32) a0 = fmaf(val(h[k], 0), val(w[k], 0), a0);
+  for (k += lane; k < dim; k += 32) a0 = fmaf(val(__ldcg(h + k), 0), val(__ldcg(w + k), 0), a0);
   return ks_warp_sum(a0 + a1);
 }
 
@@ -546,11 +550,13 @@ __global__ void __launch_bounds__(256)
                       float *__restrict__ tlogit,
                       const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab, int64_t ignore, int reduction,
                       float grad_scale, const float *dloss, float range, float *__restrict__ loss,
-                      float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc) {
+                      float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc, int release) {
   __shared__ float sm[8][kCombRows], ss[8][kCombRows], dot[kCombRows];
   __shared__ double shl[kCombRows], shn[kCombRows];
   __shared__ bool is_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (release) ks_pdl_release();
+  ks_pdl_wait();
   const int rr = tid & (kCombRows - 1), slice = tid / kCombRows;
   const int64_t row = int64_t(blockIdx.x) * kCombRows + rr;
   float m = -INFINITY, s = 0.f;
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(256)
   };
   if (row < tokens)
     for (int t = slice; t < tiles; t += 256 / kCombRows) {
-      const float2 v = part[int64_t(t) * rows_p + row];
+      const float2 v = __ldcg(part + int64_t(t) * rows_p + row);
       add(v.x, v.y);
     }
   {
@@ -599,7 +605,7 @@ __global__ void __launch_bounds__(256)
       float lt = 0.f;
       if (valid) {  // the target's logit as the dot product, in the sum too
         lt = dot[tid];
-        const float old = tlogit[row];
+        const float old = __ldcg(tlogit + row);
         if (isfinite(lt) && isfinite(old)) s += ex2((lt - m) * kLog2e) - ex2((old - m) * kLog2e);
         tlogit[row] = lt;
       }
@@ -668,13 +674,15 @@ __global__ void __launch_bounds__(256)
                     int64_t tokens, int64_t vocab, int64_t ignore, const CeScalars *__restrict__ sc, int f16) {
   const int lane = threadIdx.x & 31;
   const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  ks_pdl_release();
+  ks_pdl_wait();
   if (row >= tokens) return;
   const int64_t t = targets[row];
   const bool valid = t != ignore && t >= 0 && t < vocab;
-  const float f = valid ? sc->fscale : 0.f, fe = f16 ? f / kF16Exp : f;
-  const float l2 = lse[row] * kLog2e;
+  const float f = valid ? __ldcg(&sc->fscale) : 0.f, fe = f16 ? f / kF16Exp : f;
+  const float l2 = __ldcg(lse + row) * kLog2e;
   uint16_t *dr = d + row * ld;
-  const float dt = valid ? f * ex2(fmaf(tlogit[row], kLog2e, -l2)) - f : 0.f;
+  const float dt = valid ? f * ex2(fmaf(__ldcg(tlogit + row), kLog2e, -l2)) - f : 0.f;
   const int64_t step = int64_t(gridDim.y) * 256;
   for (int64_t c0 = int64_t(blockIdx.y) * 256 + lane * 8; c0 < ld; c0 += 4 * step) {
     uint4 v[4];
@@ -684,8 +692,8 @@ __global__ void __launch_bounds__(256)
       const int64_t c = c0 + j * step;
       k[j] = 0.f;
       if (c < ld && valid) {
-        v[j] = *reinterpret_cast<const uint4 *>(dr + c);
-        if (c < vocab) k[j] = part[(c >> tile_log2) * rows_p + row].x;
+        v[j] = __ldcg(reinterpret_cast<const uint4 *>(dr + c));
+        if (c < vocab) k[j] = __ldcg(&part[(c >> tile_log2) * rows_p + row].x);
       }
     }
 #pragma unroll
@@ -738,6 +746,8 @@ __global__ void __launch_bounds__(1024)
                       float grad_scale, const float *__restrict__ dloss, float range, CeScalars *sc) {
   __shared__ float shm[32];
   __shared__ double shn[32];
+  ks_pdl_release();
+  ks_pdl_wait();
   float mx = 0.f;
   double n = 0.0;
   for (int64_t r = threadIdx.x; r < tokens; r += 1024) {
@@ -780,13 +790,14 @@ __global__ void __launch_bounds__(256)
     ce_dh_finish_kernel(const float *__restrict__ slabs, int count, int64_t slab_elems, int64_t ld, int64_t rows,
                         int64_t cols, const CeScalars *sc, uint16_t *__restrict__ out, int64_t out_stride, int f16,
                         int vec) {
-  const float e = sc->escale;
+  ks_pdl_wait();
+  const float e = __ldcg(&sc->escale);
   const int64_t cv = (cols + 3) / 4, total = rows * cv;
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
     const int64_t r = i / cv, c = (i - r * cv) * 4;
-    float4 a = *reinterpret_cast<const float4 *>(slabs + r * ld + c);
+    float4 a = __ldcg(reinterpret_cast<const float4 *>(slabs + r * ld + c));
     for (int k = 1; k < count; ++k) {
-      const float4 b = *reinterpret_cast<const float4 *>(slabs + k * slab_elems + r * ld + c);
+      const float4 b = __ldcg(reinterpret_cast<const float4 *>(slabs + k * slab_elems + r * ld + c));
       a.x += b.x;
       a.y += b.y;
       a.z += b.z;
@@ -809,7 +820,9 @@ __global__ void __launch_bounds__(256)
 // that both sides move in full 64-byte pieces whatever their alignment.
 __global__ void __launch_bounds__(256)
     ce_copy2d_kernel(const uint16_t *__restrict__ src, int64_t src_stride, uint16_t *__restrict__ dst,
-                     int64_t dst_stride, int64_t rows, int64_t cols) {
+                     int64_t dst_stride, int64_t rows, int64_t cols, int release) {
+  if (release) ks_pdl_release();
+  ks_pdl_wait();
   const int64_t chunks = (cols + 255) / 256, total = rows * chunks;
   const int lane = threadIdx.x & 31;
   for (int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += int64_t(gridDim.x) * 8) {
@@ -820,7 +833,7 @@ __global__ void __launch_bounds__(256)
     uint16_t v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j * 32 + lane < n) v[j] = s[j * 32 + lane];
+      if (j * 32 + lane < n) v[j] = __ldcg(s + j * 32 + lane);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (j * 32 + lane < n) d[j * 32 + lane] = v[j];
@@ -841,12 +854,42 @@ struct Tile {
   int64_t tiles(int64_t m, int64_t n) const { return ((m + tm() - 1) / tm()) * ((n + tm() - 1) / tm()); }
 };
 
-// The large tile reads half as many operand bytes per product; the small one
-// fills the SMs where the large leaves them idle.
-Tile pick(int64_t m, int64_t n, int forced, int sms) {
-  if (forced) return Tile{forced == 256};
-  const int64_t tl = Tile{true}.tiles(m, n);
-  return Tile{tl >= sms};
+// Time of one K-block of one tile on one SM, microseconds, measured: the 256 x
+// 256 tile in a full 4096 x 2048 x 32768 dw product (0.72), the 128 x 128 tile,
+// which reads twice the operand bytes per product, in its dh product (0.29).
+constexpr double kLargeKb = 0.72, kSmallKb = 0.29;
+constexpr double kSlabBytesPerUs = 5e6;  // an fp32 slab is written once and read once
+
+struct Choice {
+  Tile tile;
+  int64_t splits, kb_split;
+};
+
+// Tile and K-splits with the least estimated time: rounds of tiles over the
+// SMs x K-blocks, plus the slabs' traffic where K is split (at least 8
+// K-blocks a split).  The large tile wins wherever it fills the SMs; the small
+// one, and splits, where it leaves them idle (512 x 1000 x 10007, dh: 8 large
+// tiles; split 17 ways 21 us, unsplit 113).
+Choice pick(int64_t m, int64_t n, int64_t kbs, bool may_split, int forced, int sms) {
+  Choice best = {};
+  double least = 0;
+  for (int large = 1; large >= 0; --large) {
+    if (forced && forced != (large ? 256 : 128)) continue;
+    const Tile t{large != 0};
+    const int64_t tiles = t.tiles(m, n);
+    const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>(2 * sms / tiles, kbs / 8)) : 1;
+    for (int64_t s = 1; s <= most; ++s) {
+      const int64_t per = (kbs + s - 1) / s, used = (kbs + per - 1) / per;
+      const double rounds = double((tiles * used + sms - 1) / sms);
+      double us = rounds * double(per) * (large ? kLargeKb : kSmallKb);
+      if (used > 1) us += 4 + double(used) * double(m) * double(n) * 8 / kSlabBytesPerUs;
+      if (best.splits == 0 || us < least) {
+        least = us;
+        best = Choice{t, used, per};
+      }
+    }
+  }
+  return best;
 }
 
 struct Plan {
@@ -904,9 +947,8 @@ int check(const ks_linear_ce_config &c, const ks_linear_ce_args &a, char *reason
 void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t avail, Plan &p) {
   const int sms = ks::sm_count();
   const bool fwd = a.pass != KS_CE_BACKWARD, bwd = a.pass != KS_CE_FORWARD;
-  p.g1 = pick(a.tokens, a.vocab, c.tile_m, sms);
-  p.gh = pick(a.tokens, a.dim, c.tile_m, sms);
-  p.gw = pick(a.vocab, a.dim, c.tile_m, sms);
+  p.g1 = pick(a.tokens, a.vocab, (a.dim + kBK - 1) / kBK, false, c.tile_m, sms).tile;
+  p.gw = pick(a.vocab, a.dim, (a.tokens + kBK - 1) / kBK, false, c.tile_m, sms).tile;
   p.pack_h = !tma_ok(a.h, a.h_stride);
   p.pack_w = !tma_ok(a.w, a.w_stride);
   p.pad_dh = bwd && !tma_ok(a.dh, a.dh_stride);
@@ -938,11 +980,10 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
       o = from;
       p.piece = piece;
       p.pieces = (a.vocab + piece - 1) / piece;
-      // few output tiles: split the piece's columns until the SMs are filled, at least 8 K-blocks each
-      const int64_t tiles = p.gh.tiles(a.tokens, a.dim), kbs = (std::min(piece, a.vocab) + kBK - 1) / kBK;
-      const int64_t s = std::max<int64_t>(1, std::min<int64_t>(sms / tiles, kbs / 8));
-      p.kb_split = int((kbs + s - 1) / s);
-      p.splits = int((kbs + p.kb_split - 1) / p.kb_split);
+      const Choice h = pick(a.tokens, a.dim, (std::min(piece, a.vocab) + kBK - 1) / kBK, true, c.tile_m, sms);
+      p.gh = h.tile;
+      p.splits = int(h.splits);
+      p.kb_split = int(h.kb_split);
       p.slabs = p.splits > 1 || p.pieces > 1;
       p.slab_ld = up(a.dim, 32);
       p.slab_elems = p.rows_p * p.slab_ld;
@@ -970,7 +1011,8 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
 }
 
 template <int MODE, int BN, int STAGES, int ACC, int MH>
-int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g, cudaStream_t st) {
+int launch(bool next, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g,
+           cudaStream_t st) {
   using L = Layout<BN, STAGES, ACC, MH>;
   auto kern = ce_gemm_kernel<MODE, BN, STAGES, ACC, MH>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(L::request));
@@ -978,14 +1020,15 @@ int launch(const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, 
   const int64_t work = int64_t((g.M + kBM * MH - 1) / (kBM * MH)) * ((g.N + BN - 1) / BN) * g.splits;
   if (work > (int64_t(1) << 30)) return KS_ERR_INVALID_ARGS;
   const int sms = ks::sm_count();
-  kern<<<int(std::min<int64_t>(work, sms)), kThreads, L::request, st>>>(ta, tb, tc, g, ks::wait_ctx());
-  return ks::map_cuda(cudaGetLastError());
+  return ks::launch_kernel(next, kern, dim3(unsigned(std::min<int64_t>(work, sms))), dim3(kThreads), L::request, st, ta,
+                           tb, tc, g, ks::wait_ctx());
 }
 
 template <int MODE>
-int launch_tile(Tile t, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g,
+int launch_tile(bool next, Tile t, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g,
                 cudaStream_t st) {
-  return t.large ? launch<MODE, 256, 3, 1, 2>(ta, tb, tc, g, st) : launch<MODE, 128, 5, 2, 1>(ta, tb, tc, g, st);
+  return t.large ? launch<MODE, 256, 3, 1, 2>(next, ta, tb, tc, g, st)
+                 : launch<MODE, 128, 5, 2, 1>(next, ta, tb, tc, g, st);
 }
 
 CUtensorMapDataType tm_type(int dtype) {
@@ -1018,12 +1061,12 @@ int map_out(CUtensorMap *m, int dtype, void *p, int64_t rows, int64_t cols, int6
                             CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-int copy2d(const void *src, int64_t ss, void *dst, int64_t ds, int64_t rows, int64_t cols, cudaStream_t st) {
+int copy2d(bool next, bool release, const void *src, int64_t ss, void *dst, int64_t ds, int64_t rows, int64_t cols,
+           cudaStream_t st) {
   const int64_t items = rows * ((cols + 255) / 256);
   const int grid = int(std::min<int64_t>((items + 7) / 8, int64_t(ks::sm_count()) * 8));
-  ce_copy2d_kernel<<<grid, 256, 0, st>>>(static_cast<const uint16_t *>(src), ss, static_cast<uint16_t *>(dst), ds, rows,
-                                         cols);
-  return ks::map_cuda(cudaGetLastError());
+  return ks::launch_kernel(next, ce_copy2d_kernel, dim3(grid), dim3(256), 0, st, static_cast<const uint16_t *>(src), ss,
+                           static_cast<uint16_t *>(dst), ds, rows, cols, int(release));
 }
 
 int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
@@ -1032,15 +1075,18 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   auto sc = reinterpret_cast<CeScalars *>(ws + p.o_sc);
   const float range = a.dtype == KS_F16 ? kF16Range : 1.f;
   int s;
+  bool next = false;  // a kernel of this call has been launched
   const void *h = a.h, *w = a.w;
   int64_t hs = a.h_stride, wst = a.w_stride;
   if (p.pack_h) {
-    if ((s = copy2d(a.h, a.h_stride, ws + p.o_h, p.ld, a.tokens, a.dim, st)) != KS_OK) return s;
+    if ((s = copy2d(next, true, a.h, a.h_stride, ws + p.o_h, p.ld, a.tokens, a.dim, st)) != KS_OK) return s;
+    next = true;
     h = ws + p.o_h;
     hs = p.ld;
   }
   if (p.pack_w) {
-    if ((s = copy2d(a.w, a.w_stride, ws + p.o_w, p.ld, a.vocab, a.dim, st)) != KS_OK) return s;
+    if ((s = copy2d(next, true, a.w, a.w_stride, ws + p.o_w, p.ld, a.vocab, a.dim, st)) != KS_OK) return s;
+    next = true;
     w = ws + p.o_w;
     wst = p.ld;
   }
@@ -1052,7 +1098,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   g.ignore = a.ignore_index;
   g.rows_p = p.rows_p;
   g.sc = sc;
-  g.splits = 1;
+  g.splits = g.release = 1;
   const int64_t kd = (a.dim + kBK - 1) / kBK;
   CUtensorMap th, tw;
   const int t1 = p.g1.tm();
@@ -1071,23 +1117,23 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
       CUtensorMap te;  // [tokens, whole tiles]: the columns past the vocabulary are -inf logits, zeros
       if ((s = map_out(&te, a.dtype, ws + p.o_d, a.tokens, up(a.vocab, 256), up(a.vocab, 256))) != KS_OK) return s;
       g.N = int(up(a.vocab, 256));
-      s = launch_tile<STORE>(p.g1, th, tw, te, g, st);
+      s = launch_tile<STORE>(next, p.g1, th, tw, te, g, st);
     } else {
-      s = launch_tile<STATS>(p.g1, th, tw, th, g, st);
+      s = launch_tile<STATS>(next, p.g1, th, tw, th, g, st);
     }
     if (s != KS_OK) return s;
     const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
-    ce_combine_kernel<<<blocks, 256, 0, st>>>(
-        g.part, int(p.n_tiles), p.rows_p, static_cast<const uint16_t *>(h), hs, static_cast<const uint16_t *>(w), wst,
-        a.dim, g.f16, g.tlogit, a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale, a.dloss, range,
-        a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc);
-    if ((s = ks::map_cuda(cudaGetLastError())) != KS_OK) return s;
+    s = ks::launch_kernel(
+        true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, g.part, int(p.n_tiles), p.rows_p,
+        static_cast<const uint16_t *>(h), hs, static_cast<const uint16_t *>(w), wst, a.dim, g.f16, g.tlogit, a.targets,
+        a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc, int(bwd));
+    if (s != KS_OK) return s;
   }
   if (!bwd) return KS_OK;
   if (!fwd) {
-    ce_scalars_kernel<<<1, 1024, 0, st>>>(a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale,
-                                          a.dloss, range, sc);
-    if ((s = ks::map_cuda(cudaGetLastError())) != KS_OK) return s;
+    s = ks::launch_kernel(next, ce_scalars_kernel, dim3(1), dim3(1024), 0, st, a.targets, a.tokens, a.vocab, a.ignore_index,
+                        a.reduction, a.grad_scale, a.dloss, range, sc);
+    if (s != KS_OK) return s;
   }
   char *d = ws + p.o_d;
   float *slabs = reinterpret_cast<float *>(ws + p.o_slab);
@@ -1096,8 +1142,6 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     const char *wp = static_cast<const char *>(w) + v0 * wst * 2;
     CUtensorMap ta, tb, tc;
     // d of the piece: [tokens, vpad], columns past the vocabulary zero
-    if ((s = map_k(&tw, a.dtype, wp, vp, a.dim, wst, t1)) != KS_OK) return s;
-    if ((s = map_out(&tc, a.dtype, d, a.tokens, vpad, vpad)) != KS_OK) return s;
     g.M = int(a.tokens);
     g.N = int(vpad);
     g.kb_total = g.kb_split = int(kd);
@@ -1109,12 +1153,13 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     if (p.store) {
       const unsigned rows8 = unsigned((a.tokens + 7) / 8);
       const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, std::max<int64_t>(1, 8192 / rows8)));
-      ce_scale_kernel<<<dim3(rows8, cols), 256, 0, st>>>(reinterpret_cast<uint16_t *>(d), vpad, g.part, p.rows_p,
-                                                         t1 == 256 ? 8 : 7, lse, g.tlogit, a.targets, a.tokens, a.vocab,
-                                                         a.ignore_index, sc, g.f16);
-      s = ks::map_cuda(cudaGetLastError());
+      s = ks::launch_kernel(true, ce_scale_kernel, dim3(rows8, cols), dim3(256), 0, st, reinterpret_cast<uint16_t *>(d), vpad, g.part,
+                          p.rows_p, t1 == 256 ? 8 : 7, lse, g.tlogit, a.targets, a.tokens, a.vocab, a.ignore_index, sc,
+                          g.f16);
     } else {
-      s = launch_tile<PROB>(p.g1, th, tw, tc, g, st);
+      if ((s = map_k(&tw, a.dtype, wp, vp, a.dim, wst, t1)) != KS_OK) return s;
+      if ((s = map_out(&tc, a.dtype, d, a.tokens, vpad, vpad)) != KS_OK) return s;
+      s = launch_tile<PROB>(true, p.g1, th, tw, tc, g, st);
     }
     if (s != KS_OK) return s;
     // dh (+)= d w
@@ -1135,7 +1180,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.group = 8;
     g.out_f32 = slabbed;
     g.accumulate = slabbed && i > 0;
-    if ((s = launch_tile<DH>(p.gh, ta, tb, tc, g, st)) != KS_OK) return s;
+    if ((s = launch_tile<DH>(true, p.gh, ta, tb, tc, g, st)) != KS_OK) return s;
     // rows v0.. of dw = d^T h
     const int tw_ = p.gw.tm();
     int a3d = 0;
@@ -1149,18 +1194,20 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.kb_total = g.kb_split = int((a.tokens + kBK - 1) / kBK);
     g.splits = 1;
     g.out_f32 = g.accumulate = 0;
-    if ((s = launch_tile<DW>(p.gw, ta, tb, tc, g, st)) != KS_OK) return s;
-    if (p.pad_dw && (s = copy2d(ws + p.o_dw, p.ld, dwp, a.dw_stride, vp, a.dim, st)) != KS_OK) return s;
+    const bool last = i + 1 == p.pieces && !p.slabs && !p.pad_dh;
+    g.release = !last || p.pad_dw;
+    if ((s = launch_tile<DW>(true, p.gw, ta, tb, tc, g, st)) != KS_OK) return s;
+    g.release = 1;
+    if (p.pad_dw && (s = copy2d(true, !last, ws + p.o_dw, p.ld, dwp, a.dw_stride, vp, a.dim, st)) != KS_OK) return s;
   }
   if (p.slabs) {
     const int64_t items = a.tokens * ((a.dim + 3) / 4);
     const int grid = int(std::min<int64_t>((items + 255) / 256, int64_t(ks::sm_count()) * 8));
     const int vec = reinterpret_cast<uintptr_t>(a.dh) % 8 == 0 && a.dh_stride % 4 == 0;
-    ce_dh_finish_kernel<<<grid, 256, 0, st>>>(slabs, p.splits, p.slab_elems, p.slab_ld, a.tokens, a.dim, sc,
-                                              static_cast<uint16_t *>(a.dh), a.dh_stride, a.dtype == KS_F16, vec);
-    return ks::map_cuda(cudaGetLastError());
+    return ks::launch_kernel(true, ce_dh_finish_kernel, dim3(grid), dim3(256), 0, st, slabs, p.splits, p.slab_elems, p.slab_ld,
+                           a.tokens, a.dim, sc, static_cast<uint16_t *>(a.dh), a.dh_stride, int(a.dtype == KS_F16), vec);
   }
-  if (p.pad_dh) return copy2d(ws + p.o_dh, p.ld, a.dh, a.dh_stride, a.tokens, a.dim, st);
+  if (p.pad_dh) return copy2d(true, false, ws + p.o_dh, p.ld, a.dh, a.dh_stride, a.tokens, a.dim, st);
   return KS_OK;
 }
 

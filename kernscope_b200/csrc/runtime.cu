@@ -36,12 +36,22 @@ int map_cuda(cudaError_t e) {
   }
 }
 
-int check_arch_sm100() {
+// An attribute of the current device that never changes, asked for once per
+// device (the smallest launches take a few microseconds in all).
+static cudaError_t device_attribute(cudaDeviceAttr attr, std::atomic<int> (&cache)[64], int *value) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return map_cuda(e);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (*value = cache[dev].load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+  e = cudaDeviceGetAttribute(value, attr, dev);
+  if (e == cudaSuccess && dev < 64) cache[dev].store(*value, std::memory_order_relaxed);
+  return e;
+}
+
+int check_arch_sm100() {
+  static std::atomic<int> cache[64];
   int major = 0;
-  e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+  const cudaError_t e = device_attribute(cudaDevAttrComputeCapabilityMajor, cache, &major);
   if (e != cudaSuccess) return map_cuda(e);
   return major == 10 ? KS_OK : KS_ERR_ARCH;
 }
@@ -107,9 +117,9 @@ KsWait wait_ctx() {
 }
 
 int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  static std::atomic<int> cache[64];
+  int n = 0;
+  if (device_attribute(cudaDevAttrMultiProcessorCount, cache, &n) != cudaSuccess || n <= 0) return 148;
   return n;
 }
 

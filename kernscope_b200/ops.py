@@ -214,62 +214,69 @@ def flash_attention(q, k, v, causal: bool = True, scale: float = 0.0, out=None, 
 
 
 # ---------------------------------------------------------------------------
-# Training operators at the vocabulary end of a language model
+# Training operators at the vocabulary end of a language model.
+#
+# The smallest of these calls take a few microseconds on the GPU, so the host
+# side is kept short: one pass of checks, raw stream handles, sizes of scratch
+# remembered per problem size (never per tensor).
 # ---------------------------------------------------------------------------
 _DT_TRAIN = {torch.bfloat16: N.KS_BF16, torch.float16: N.KS_F16, torch.float32: N.KS_F32}
+_DT_HALF = {torch.bfloat16: N.KS_BF16, torch.float16: N.KS_F16}
 _REDUCTIONS = {"none": N.KS_CE_NONE, "mean": N.KS_CE_MEAN, "sum": N.KS_CE_SUM}
 
 
-def _empty(shape, dtype, device, stream) -> torch.Tensor:
-    """torch.empty from the pool of the stream that the launch goes to: scratch
-    freed after the call is then reused only behind the launch."""
+def _raw_stream(stream, dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+
+
+def _empty(like, shape, dtype, stream) -> torch.Tensor:
+    """An uninitialised tensor on `like`'s device, from the pool of the stream
+    that the launch goes to: scratch freed after the call is then reused only
+    behind the launch."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
 
 
-def _check_rows(name, t, dtypes, device=None):
-    """A [rows, cols] CUDA tensor on the current device with dense rows (any row
-    stride of at least cols)."""
-    if not (t.is_cuda and t.dim() == 2 and t.dtype in dtypes):
-        raise ValueError(f"{name} must be a 2-D CUDA tensor of {' or '.join(str(d) for d in dtypes)}")
-    if t.device.index != torch.cuda.current_device() or (device is not None and t.device != device):
-        raise ValueError(f"{name} is on {t.device}, not on the current device")
-    if (t.stride(1) != 1 and t.shape[1] > 1) or (t.stride(0) < t.shape[1] and t.shape[0] > 1):
-        raise ValueError(f"{name} must have dense rows (stride 1 along the last axis) that do not overlap")
+def _zero(t, stream) -> torch.Tensor:
+    if stream is None:
+        return t.zero_()
+    with torch.cuda.stream(stream):
+        return t.zero_()
 
 
-def _row_stride(t) -> int:
-    return max(t.stride(0), t.shape[1])
+def _rows(name, t, dtypes, dev: int) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a 2-D tensor on device `dev` whose rows are
+    dense and do not overlap."""
+    if t.dtype in dtypes and t.get_device() == dev and t.dim() == 2:
+        (r, c), (s0, s1) = t.shape, t.stride()
+        if (s1 == 1 or c <= 1) and (s0 >= c or r <= 1):
+            return r, c, (s0 if s0 > c else c)
+    raise ValueError(f"{name} must be a 2-D tensor of {' or '.join(str(d) for d in dtypes)} on the current CUDA device, "
+                     f"with dense rows that do not overlap (got {t.dtype} {tuple(t.shape)}, strides {t.stride()}, "
+                     f"{t.device})")
 
 
-def _check_ids(name, t, n, device):
-    if not (t.is_cuda and t.device == device and t.dtype == torch.int64 and t.is_contiguous() and t.numel() == n):
-        raise ValueError(f"{name} must be a contiguous int64 tensor of {n} values on {device}")
-
-
-def _check_f32(name, t, n, device):
-    if not (t.is_cuda and t.device == device and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == n):
-        raise ValueError(f"{name} must be a contiguous float32 tensor of {n} values on {device}")
+def _values(name, t, dtype, n: int, dev: int) -> int:
+    """Address of a contiguous tensor of n values on device `dev`."""
+    if t.dtype is dtype and t.get_device() == dev and t.numel() == n and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n} values on the current CUDA device (got "
+                     f"{t.dtype} {tuple(t.shape)}, {t.device})")
 
 
 def _linear_ce_args(h, w, targets, ce_pass, reduction, ignore_index, grad_scale=1.0) -> N.LinearCeArgs:
-    _check_rows("h", h, (torch.bfloat16, torch.float16))
-    _check_rows("w", w, (h.dtype,), h.device)
-    if h.shape[1] != w.shape[1]:
+    dev = torch.cuda.current_device()
+    n, dim, h_stride = _rows("h", h, _DT_HALF, dev)
+    vocab, w_dim, w_stride = _rows("w", w, (h.dtype,), dev)
+    if dim != w_dim:
         raise ValueError("h and w differ in their last dimension")
-    _check_ids("targets", targets, h.shape[0], h.device)
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}")
-    a = N.LinearCeArgs()
-    a.h, a.w, a.targets = h.data_ptr(), w.data_ptr(), targets.data_ptr()
-    a.tokens, a.dim, a.vocab = h.shape[0], h.shape[1], w.shape[0]
-    a.h_stride, a.w_stride = _row_stride(h), _row_stride(w)
-    a.dh_stride = a.dw_stride = a.dim
-    a.dtype, a.ce_pass, a.reduction = _DT_TRAIN[h.dtype], ce_pass, _REDUCTIONS[reduction]
-    a.grad_scale, a.ignore_index = grad_scale, ignore_index
-    return a
+    return N.LinearCeArgs(h.data_ptr(), w.data_ptr(), _values("targets", targets, torch.int64, n, dev), n, dim, vocab,
+                          h_stride, w_stride, _DT_HALF[h.dtype], ce_pass, _REDUCTIONS[reduction], grad_scale,
+                          ignore_index, None, None, None, None, None, dim, dim)
 
 
 # Default bound on the scratch of one call.  Where 2 bytes for every (token,
@@ -288,12 +295,30 @@ def linear_cross_entropy_workspace_bytes(args: N.LinearCeArgs, cfg=None, limit=N
     return least.value, want.value
 
 
-def _linear_ce_run(a, cfg, workspace, device, stream):
-    cfg = cfg or N.LinearCeConfig()
+_CE_DEFAULT = N.LinearCeConfig()
+_ce_scratch: dict = {}  # problem size and alignment -> preferred workspace bytes
+
+
+def _linear_ce_run(a, cfg, workspace, like, stream):
     if workspace is None:
-        workspace = _empty(linear_cross_entropy_workspace_bytes(a, cfg)[1], torch.uint8, device, stream)
-    a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    N.check("ks_linear_ce_launch", N.lib.ks_linear_ce_launch(C.byref(cfg), C.byref(a), _stream_ptr(stream)))
+        if cfg is None:
+            # all that the size depends on
+            aligned = [not ((p or 0) & 15 or stride & 7) for p, stride in
+                       ((a.h, a.h_stride), (a.w, a.w_stride), (a.dh, a.dh_stride), (a.dw, a.dw_stride))]
+            key = (a.tokens, a.dim, a.vocab, a.ce_pass, LINEAR_CE_WORKSPACE_LIMIT, *aligned)
+            size = _ce_scratch.get(key)
+            if size is None:
+                if len(_ce_scratch) >= 4096:
+                    _ce_scratch.clear()
+                size = _ce_scratch[key] = linear_cross_entropy_workspace_bytes(a)[1]
+        else:
+            size = linear_cross_entropy_workspace_bytes(a, cfg)[1]
+        workspace = _empty(like, size, torch.uint8, stream)
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), size
+    else:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    N.check("ks_linear_ce_launch", N.lib.ks_linear_ce_launch(C.byref(cfg or _CE_DEFAULT), C.byref(a),
+                                                             _raw_stream(stream, like.get_device())))
 
 
 def linear_cross_entropy(h, w, targets, ignore_index: int = -100, reduction: str = "none", cfg=None, workspace=None,
@@ -303,23 +328,29 @@ def linear_cross_entropy(h, w, targets, ignore_index: int = -100, reduction: str
     dim] (bf16 or fp16), targets int64.  Returns (loss, lse) in fp32."""
     a = _linear_ce_args(h, w, targets, N.KS_CE_FORWARD, reduction, ignore_index)
     n = a.tokens
-    loss = _empty(n if reduction == "none" else 1, torch.float32, h.device, stream)
-    lse = _empty(n, torch.float32, h.device, stream)
+    loss = _empty(h, n if reduction == "none" else 1, torch.float32, stream)
+    lse = _empty(h, n, torch.float32, stream)
     if n == 0:
-        return loss.zero_(), lse
+        return _zero(loss, stream), lse
     a.loss, a.lse = loss.data_ptr(), lse.data_ptr()
-    _linear_ce_run(a, cfg, workspace, h.device, stream)
+    _linear_ce_run(a, cfg, workspace, h, stream)
     return loss, lse
 
 
 def _linear_ce_grads(a, h, w, dh, dw, stream):
-    dh = _empty(h.shape, h.dtype, h.device, stream) if dh is None else dh
-    dw = _empty(w.shape, w.dtype, w.device, stream) if dw is None else dw
     for name, t, like in (("dh", dh, h), ("dw", dw, w)):
-        _check_rows(name, t, (like.dtype,), like.device)
-        if t.shape != like.shape:
-            raise ValueError(f"{name} must have the shape {tuple(like.shape)}")
-    a.dh, a.dw, a.dh_stride, a.dw_stride = dh.data_ptr(), dw.data_ptr(), _row_stride(dh), _row_stride(dw)
+        if t is None:
+            t = _empty(like, like.shape, like.dtype, stream)
+        else:
+            rows, cols, stride = _rows(name, t, (like.dtype,), like.get_device())
+            if (rows, cols) != tuple(like.shape):
+                raise ValueError(f"{name} must have the shape {tuple(like.shape)}")
+            setattr(a, name + "_stride", stride)
+        setattr(a, name, t.data_ptr())
+        if name == "dh":
+            dh = t
+        else:
+            dw = t
     return dh, dw
 
 
@@ -330,14 +361,14 @@ def linear_cross_entropy_backward(h, w, targets, lse, dloss=None, ignore_index: 
     otherwise; None stands for ones.  Tokens with targets == ignore_index take no
     part, and the mean divides by the number of the others."""
     a = _linear_ce_args(h, w, targets, N.KS_CE_BACKWARD, reduction, ignore_index, grad_scale)
-    _check_f32("lse", lse, a.tokens, h.device)
+    dev = h.get_device()
+    a.lse = _values("lse", lse, torch.float32, a.tokens, dev)
     if dloss is not None:
-        _check_f32("dloss", dloss, a.tokens if reduction == "none" else 1, h.device)
+        a.dloss = _values("dloss", dloss, torch.float32, a.tokens if reduction == "none" else 1, dev)
     dh, dw = _linear_ce_grads(a, h, w, dh, dw, stream)
     if a.tokens == 0:
-        return dh, dw.zero_()
-    a.lse, a.dloss = lse.data_ptr(), dloss.data_ptr() if dloss is not None else None
-    _linear_ce_run(a, cfg, workspace, h.device, stream)
+        return dh, _zero(dw, stream)
+    _linear_ce_run(a, cfg, workspace, h, stream)
     return dh, dw
 
 
@@ -348,35 +379,39 @@ def linear_cross_entropy_grad(h, w, targets, ignore_index: int = -100, reduction
     a = _linear_ce_args(h, w, targets, N.KS_CE_GRAD, reduction, ignore_index, grad_scale)
     if reduction == "none":
         raise ValueError("loss and gradient in one call need reduction 'mean' or 'sum'")
-    loss = _empty(1, torch.float32, h.device, stream)
+    loss = _empty(h, 1, torch.float32, stream)
     dh, dw = _linear_ce_grads(a, h, w, dh, dw, stream)
     if a.tokens == 0:
-        return loss.zero_(), dh, dw.zero_()
+        return _zero(loss, stream), dh, _zero(dw, stream)
     a.loss = loss.data_ptr()
-    _linear_ce_run(a, cfg, workspace, h.device, stream)
+    _linear_ce_run(a, cfg, workspace, h, stream)
     return loss, dh, dw
-
-
-_TRAIN_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def embedding(tokens, table, scale: float = 1.0, out=None, stream=None) -> torch.Tensor:
     """scale * table[tokens] (tokens int64 of any shape, table [vocab, dim] in
     bf16, fp16 or fp32); tokens outside [0, vocab) give rows of zeros."""
-    _check_rows("table", table, _TRAIN_DTYPES)
-    _check_ids("tokens", tokens, tokens.numel(), table.device)
-    n, (vocab, dim) = tokens.numel(), table.shape
-    out = _empty((*tokens.shape, dim), table.dtype, table.device, stream) if out is None else out
-    if out.numel() != n * dim:
-        raise ValueError(f"out must hold {n} rows of {dim}")
-    rows = out if out.dim() == 2 else out.view(n, dim)
-    _check_rows("out", rows, (table.dtype,), table.device)
+    dev = torch.cuda.current_device()
+    vocab, dim, table_stride = _rows("table", table, _DT_TRAIN, dev)
+    n = tokens.numel()
+    ids = _values("tokens", tokens, torch.int64, n, dev)
+    if out is None:
+        out = _empty(table, (*tokens.shape, dim), table.dtype, stream)
+        out_stride = dim
+    else:
+        if out.numel() != n * dim:
+            raise ValueError(f"out must hold {n} rows of {dim}")
+        out_stride = _rows("out", out if out.dim() == 2 else out.view(n, dim), (table.dtype,), dev)[2]
     if n == 0:
         return out
-    args = N.EmbeddingArgs(tokens.data_ptr(), n, table.data_ptr(), out.data_ptr(), vocab, dim, _row_stride(table),
-                           _row_stride(rows), _DT_TRAIN[table.dtype], scale)
-    N.check("ks_embedding_launch", N.lib.ks_embedding_launch(C.byref(args), _stream_ptr(stream)))
+    args = N.EmbeddingArgs(ids, n, table.data_ptr(), out.data_ptr(), vocab, dim, table_stride, out_stride,
+                           _DT_TRAIN[table.dtype], scale)
+    N.check("ks_embedding_launch", N.lib.ks_embedding_launch(C.byref(args), _raw_stream(stream, dev)))
     return out
+
+
+_EMB_DEFAULT = N.EmbeddingGradConfig()
+_emb_scratch: dict = {}  # problem size -> workspace bytes
 
 
 def embedding_backward(tokens, dout, vocab: int, scale: float = 1.0, padding_idx: int = -1, dtable=None, dtype=None,
@@ -385,32 +420,42 @@ def embedding_backward(tokens, dout, vocab: int, scale: float = 1.0, padding_idx
     type or fp32 (`dtype`, or that of `dtable`).  accumulate adds to `dtable`'s
     values and touches the rows of `tokens` alone; otherwise every row is
     written.  Tokens equal to padding_idx or outside [0, vocab) have no part."""
-    n = tokens.numel()
-    rows = dout if dout.dim() == 2 else dout.view(n, dout.shape[-1])
-    _check_rows("dout", rows, _TRAIN_DTYPES)
-    _check_ids("tokens", tokens, rows.shape[0], rows.device)
-    dim = rows.shape[1]
+    dev = torch.cuda.current_device()
+    rows = dout if dout.dim() == 2 else dout.view(tokens.numel(), dout.shape[-1])
+    n, dim, dout_stride = _rows("dout", rows, _DT_TRAIN, dev)
+    ids = _values("tokens", tokens, torch.int64, n, dev)
     if dtable is None:
         if accumulate:
             raise ValueError("accumulate needs the dtable to add to")
-        dtable = _empty((vocab, dim), dtype or dout.dtype, rows.device, stream)
-    _check_rows("dtable", dtable, (dout.dtype, torch.float32), rows.device)
-    if tuple(dtable.shape) != (vocab, dim) or (dtype is not None and dtable.dtype != dtype):
-        raise ValueError(f"dtable must be [{vocab}, {dim}]" + (f" of {dtype}" if dtype is not None else ""))
+        if dtype not in (None, dout.dtype, torch.float32):
+            raise ValueError("the gradient has the type of dout or float32")
+        dtable = _empty(dout, (vocab, dim), dtype or dout.dtype, stream)
+        dtable_stride = dim
+    else:
+        r, c, dtable_stride = _rows("dtable", dtable, (dout.dtype, torch.float32), dev)
+        if (r, c) != (vocab, dim) or (dtype is not None and dtable.dtype != dtype):
+            raise ValueError(f"dtable must be [{vocab}, {dim}]" + (f" of {dtype}" if dtype is not None else ""))
     if n == 0:
-        return dtable if accumulate else dtable.zero_()
-    args = N.EmbeddingGradArgs(tokens.data_ptr(), n, rows.data_ptr(), dtable.data_ptr(), vocab, dim, _row_stride(rows),
-                               _row_stride(dtable), _DT_TRAIN[dout.dtype], _DT_TRAIN[dtable.dtype], int(accumulate),
-                               scale, padding_idx)
-    cfg = cfg or N.EmbeddingGradConfig()
+        return dtable if accumulate else _zero(dtable, stream)
+    args = N.EmbeddingGradArgs(ids, n, rows.data_ptr(), dtable.data_ptr(), vocab, dim, dout_stride, dtable_stride,
+                               _DT_TRAIN[dout.dtype], _DT_TRAIN[dtable.dtype], accumulate, scale, padding_idx)
+    cfg = cfg or _EMB_DEFAULT
     if workspace is None:
-        need = C.c_size_t(0)
-        N.check("ks_embedding_grad_workspace_bytes",
-                N.lib.ks_embedding_grad_workspace_bytes(C.byref(cfg), C.byref(args), C.byref(need)))
-        workspace = _empty(need.value, torch.uint8, rows.device, stream)
-    args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        key = (n, vocab, dim, args.dtype, cfg.chunk)
+        size = _emb_scratch.get(key)
+        if size is None:
+            if len(_emb_scratch) >= 4096:
+                _emb_scratch.clear()
+            need = C.c_size_t(0)
+            N.check("ks_embedding_grad_workspace_bytes",
+                    N.lib.ks_embedding_grad_workspace_bytes(C.byref(cfg), C.byref(args), C.byref(need)))
+            size = _emb_scratch[key] = need.value
+        workspace = _empty(dout, size, torch.uint8, stream)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), size
+    else:
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     N.check("ks_embedding_grad_launch",
-            N.lib.ks_embedding_grad_launch(C.byref(cfg), C.byref(args), _stream_ptr(stream)))
+            N.lib.ks_embedding_grad_launch(C.byref(cfg), C.byref(args), _raw_stream(stream, dev)))
     return dtable
 
 
@@ -438,6 +483,7 @@ class GradClipper:
                     raise ValueError("gradients must be contiguous bf16, fp16 or fp32 tensors on one CUDA device")
             if o.dtype != g.dtype or o.numel() != g.numel():
                 raise ValueError("an output differs in type or size from its gradient")
+        # a tensor twice, or two that overlap, would be counted and scaled twice
         spans = sorted({(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), i)
                         for i, pair in enumerate(zip(self.grads, self.out)) for t in pair if t.numel()})
         if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
@@ -453,16 +499,17 @@ class GradClipper:
         need = C.c_size_t(0)
         N.check("ks_grad_clip_workspace_bytes", N.lib.ks_grad_clip_workspace_bytes(chunks.value, C.byref(need)))
         self._table = host.to(self.device)
-        self._need, self._chunks = need.value, chunks.value
+        self._need, self._chunks, self._index = need.value, chunks.value, self.device.index
 
     def clip(self, max_norm: float, eps: float = 1e-6, stream=None) -> torch.Tensor:
-        if self.device.index != torch.cuda.current_device():
+        if self._index != torch.cuda.current_device():
             raise ValueError(f"the gradients are on {self.device}, not on the current device")
-        norm = _empty(1, torch.float32, self.device, stream)
-        ws = _empty(self._need, torch.uint8, self.device, stream)
+        # the norm in its own small tensor: it may outlive the scratch
+        norm = _empty(self._table, 1, torch.float32, stream)
+        ws = _empty(self._table, self._need, torch.uint8, stream)
         args = N.GradClipArgs(self._table.data_ptr(), self._chunks, max_norm, eps, norm.data_ptr(), ws.data_ptr(),
                               self._need)
-        N.check("ks_grad_clip_launch", N.lib.ks_grad_clip_launch(C.byref(args), _stream_ptr(stream)))
+        N.check("ks_grad_clip_launch", N.lib.ks_grad_clip_launch(C.byref(args), _raw_stream(stream, self._index)))
         return norm
 
 
