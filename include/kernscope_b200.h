@@ -314,7 +314,8 @@ int ks_embedding_launch(const ks_embedding_args *args, void *stream);
  * written, zeros where no token is).  fp32 sums in the order of the positions,
  * one rounding; the same bits every time.  Tokens outside [0, vocab) and
  * those equal to padding_idx have no part.  out_dtype: dout's type or fp32.
- * cfg.chunk: sorted positions per warp, 1..32, 0 = chosen from the sizes.
+ * cfg.chunk: sorted positions after which a token's sum is split, 1..1024, 0 =
+ * chosen from the sizes.
  * The workspace (256-byte aligned) holds the sorted tokens and the partial
  * sums of tokens that lie in several chunks.                                 */
 typedef struct ks_embedding_grad_config { int chunk; } ks_embedding_grad_config;

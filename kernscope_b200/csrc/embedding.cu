@@ -6,10 +6,10 @@
 //
 // Both are bound by memory.  The gradient sums each table row in a fixed
 // order, the order of the positions, whatever the timing: a stable radix sort
-// of the tokens brings equal ones together, then each warp walks `chunk`
-// consecutive sorted positions over one segment of columns, adding in fp32
-// and writing a row when its token ends.  A token whose positions lie in
-// several chunks leaves an fp32 partial sum per chunk, and the warp that
+// of the tokens brings equal ones together, then CTAs walk the sorted
+// positions over one segment of columns each, adding in fp32 and writing a row
+// when its token ends.  A token whose positions lie in several chunks (of
+// `chunk` positions) leaves an fp32 partial sum per chunk, and the CTA that
 // finishes last adds those in order.  No floating-point atomics.
 #include <algorithm>
 #include <cuda_fp16.h>
@@ -45,22 +45,19 @@ struct Elem<KS_F32> {
   KS_DEV static float put(float v) { return v; }
 };
 
-// W values of a lane, still as stored.  VEC: 16-byte pieces at consecutive
-// columns; otherwise columns lane, lane + 32, ...
-template <int DT, int W, bool VEC>
+// A lane's share of a row's segment, still as stored: 16 bytes (VEC), or as many
+// single elements 32 columns apart, for rows that are not 16-byte aligned.
+template <int DT, bool VEC>
 struct Raw {
   using T = typename Elem<DT>::T;
+  static constexpr int W = Elem<DT>::kPer;
   alignas(16) T v[W];
   // p: the row at the segment's first column; c: that column; lanes past `dim` hold zeros
   KS_DEV void load(const T *p, int64_t c, int64_t dim, int lane) {
     if constexpr (VEC) {
-      constexpr int per = Elem<DT>::kPer;
-#pragma unroll
-      for (int j = 0; j < W / per; ++j) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (c + lane * W + j * per < dim) x = __ldg(reinterpret_cast<const uint4 *>(p + lane * W + j * per));
-        *reinterpret_cast<uint4 *>(v + j * per) = x;
-      }
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (c + lane * W < dim) x = __ldg(reinterpret_cast<const uint4 *>(p + lane * W));
+      *reinterpret_cast<uint4 *>(v) = x;
     } else {
 #pragma unroll
       for (int j = 0; j < W; ++j) v[j] = c + lane + j * 32 < dim ? __ldg(p + lane + j * 32) : T(0);
@@ -68,11 +65,7 @@ struct Raw {
   }
   KS_DEV void store(T *p, int64_t c, int64_t dim, int lane) const {
     if constexpr (VEC) {
-      constexpr int per = Elem<DT>::kPer;
-#pragma unroll
-      for (int j = 0; j < W / per; ++j)
-        if (c + lane * W + j * per < dim)
-          *reinterpret_cast<uint4 *>(p + lane * W + j * per) = *reinterpret_cast<const uint4 *>(v + j * per);
+      if (c + lane * W < dim) *reinterpret_cast<uint4 *>(p + lane * W) = *reinterpret_cast<const uint4 *>(v);
     } else {
 #pragma unroll
       for (int j = 0; j < W; ++j)
@@ -94,82 +87,131 @@ __global__ void __launch_bounds__(256)
   constexpr int W = E::kPer, kSeg = 32 * W, U = 4;
   const int lane = threadIdx.x & 31;
   const int64_t segs = (dim + kSeg - 1) / kSeg, groups = (segs + U - 1) / U;
-  const int64_t total = n * groups, step = int64_t(gridDim.x) * 8;
-  for (int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5); i < total; i += step) {
-    const int64_t row = i / groups, c0 = (i - row * groups) * U * kSeg;
-    const int64_t t = __ldg(tokens + row);
-    const bool in = t >= 0 && t < vocab;
-    Raw<DT, W, VEC> x[U];
+  const int64_t i = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (i >= n * groups) return;
+  const int64_t row = i / groups, c0 = (i - row * groups) * U * kSeg;
+  const int64_t t = __ldg(tokens + row);
+  const bool in = t >= 0 && t < vocab;
+  Raw<DT, VEC> x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u].load(table + (in ? t : 0) * table_stride + c0 + u * kSeg, c0 + u * kSeg, in ? dim : 0, lane);
+  for (int u = 0; u < U; ++u)
+    x[u].load(table + (in ? t : 0) * table_stride + c0 + u * kSeg, c0 + u * kSeg, in ? dim : 0, lane);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+  for (int u = 0; u < U; ++u) {
 #pragma unroll
-      for (int j = 0; j < W; ++j) x[u].v[j] = E::put(E::get(x[u].v[j]) * scale);
-      if (!in) {
-#pragma unroll
-        for (int j = 0; j < W; ++j) x[u].v[j] = 0;  // not 0 * inf
-      }
-      x[u].store(out + row * out_stride + c0 + u * kSeg, c0 + u * kSeg, dim, lane);
-    }
+    for (int j = 0; j < W; ++j) x[u].v[j] = in ? E::put(E::get(x[u].v[j]) * scale) : 0;  // outside: not 0 * inf
+    x[u].store(out + row * out_stride + c0 + u * kSeg, c0 + u * kSeg, dim, lane);
   }
+}
+
+KS_DEV uint32_t token_key(int64_t t, int64_t vocab, int64_t padding) {
+  return t < 0 || t >= vocab || t == padding ? uint32_t(vocab) : uint32_t(t);  // the excluded ones sort last
 }
 
 // ---------------------------------------------------------------------------
 // Stable sort of (token, position), and the zeros of the dense gradient.
 //
+// Up to kRankMax positions: each position's place is the number of smaller
+// (token, position) pairs, counted directly, 16 threads a position, every CTA
+// with all keys in shared memory.  (At 8192 positions this and the radix sort took
+// the same 20 us, but the comparisons keep 128 SMs from writing zeros.)
+//
+// More: radix, below.
 // One cluster of 8 CTAs sorts: least-significant-digit radix passes of up to
 // 10 bits, the digit counts exchanged through distributed shared memory (no
 // counters in global memory, no spinning).  Each warp owns a contiguous part
 // of the input and ranks 32 elements at a time with a match over the warp, so
 // equal digits keep their order.  The other clusters of the grid write the
-// zeros meanwhile: the sort is latency-bound and uses no bandwidth to speak of.
+// zeros meanwhile, up to 512 KB a CTA: the sort is latency-bound and uses no bandwidth
+// to speak of.  (With one zeroing CTA per SM the clusters that found no room at
+// first made a second round of it: 134 MB in 36 us, 537 MB in 134.)
 // ---------------------------------------------------------------------------
 constexpr int kCluster = 8;
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kBatch = 8;  // loads in flight per lane
 
-constexpr int kZeroBytes = 32 * 1024;  // one bulk store of zeros
+// What the other CTAs of the sorting kernels zero: rows `stride` apart and
+// `bytes` long (even, as are their addresses), `share` bytes per CTA.
+struct Zeros {
+  char *p;
+  int64_t rows, bytes, stride, share;
+};
 
-KS_DEV void bulk_store(void *dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
-               "r"(ks_smem_u32(src)), "r"(bytes)
-               : "memory");
+KS_DEV void zero_rows(const Zeros &z, int64_t cta) {
+  const int64_t rows = z.rows, bytes = z.bytes, stride = z.stride, first = cta * z.share;
+  char *p = z.p;
+  const int64_t end = min(first + z.share, rows * bytes);
+  for (int64_t at = first; at < end;) {
+    const int64_t r = at / bytes, c = at - r * bytes;
+    const int64_t len = min(bytes - c, end - at);
+    char *q = p + r * stride + c;
+    const int64_t head = min(len, int64_t((16 - (reinterpret_cast<uintptr_t>(q) & 15)) & 15));
+    const int64_t vecs = (len - head) / 16, tail = len - head - vecs * 16;
+    uint4 *v = reinterpret_cast<uint4 *>(q + head);
+    for (int64_t i = threadIdx.x; i < vecs; i += kSortThreads) v[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x < head / 2) reinterpret_cast<uint16_t *>(q)[threadIdx.x] = 0;
+    if (threadIdx.x < tail / 2) reinterpret_cast<uint16_t *>(q + len - tail)[threadIdx.x] = 0;
+    at += len;
+  }
 }
 
-// Zeros over [p, p + bytes) (p and bytes even), the pieces of kZeroBytes dealt
-// out over `ctas` CTAs; the even bytes before and after whole 16-byte words by
-// the first of them.
-KS_DEV void zero_span(char *p, int64_t bytes, const void *zeros, int64_t cta, int64_t ctas) {
-  const int64_t head = min(bytes, int64_t((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15));
-  const int64_t body = (bytes - head) / 16 * 16, tail = bytes - head - body;
-  if (threadIdx.x == 0)
-    for (int64_t at = cta * kZeroBytes; at < body; at += ctas * kZeroBytes)
-      bulk_store(p + head + at, zeros, uint32_t(min(body - at, int64_t(kZeroBytes))));
-  if (cta == 0 && threadIdx.x < head / 2) reinterpret_cast<uint16_t *>(p)[threadIdx.x] = 0;
-  if (cta == 0 && threadIdx.x < tail / 2) reinterpret_cast<uint16_t *>(p + bytes - tail)[threadIdx.x] = 0;
+constexpr int kRankMax = 4096;
+constexpr int kRankBits = 12;
+constexpr int kRankRows = kSortThreads / 16;  // positions per CTA
+
+// FITS: token and position fit one 32-bit key (vocab < 2^20, position < 2^12).
+template <bool FITS>
+__global__ void __launch_bounds__(kSortThreads)
+    emb_rank_kernel(const int64_t *__restrict__ tokens, int n, int64_t vocab, int64_t padding, uint2 *__restrict__ out,
+                    uint32_t *counters, int64_t counters_n, const __grid_constant__ Zeros zeros) {
+  __shared__ __align__(16) uint32_t keys[kRankMax];
+  const int tid = threadIdx.x, ctas = (n + kRankRows - 1) / kRankRows;
+  if (tid == 0) ks_pdl_release();
+  if (int(blockIdx.x) >= ctas) {
+    zero_rows(zeros, int64_t(blockIdx.x) - ctas);
+    return;
+  }
+  for (int64_t i = int64_t(blockIdx.x) * kSortThreads + tid; i < counters_n; i += int64_t(ctas) * kSortThreads)
+    counters[i] = 0;
+  const int padded = (n + 63) / 64 * 64;
+#pragma unroll 4
+  for (int i = tid; i < padded; i += kSortThreads) {
+    uint32_t k = 0xffffffffu;  // sorts behind everything
+    if (i < n) {
+      k = token_key(tokens[i], vocab, padding);
+      if (FITS) k = k << kRankBits | uint32_t(i);
+    }
+    keys[i] = k;
+  }
+  __syncthreads();
+  const int i = blockIdx.x * kRankRows + tid / 16;
+  const uint32_t mine = i < n ? keys[i] : 0;
+  int below = 0;
+  for (int j = tid % 16 * 4; j < padded; j += 64) {
+    const uint4 k = *reinterpret_cast<const uint4 *>(keys + j);
+    if (FITS) {
+      below += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+    } else {
+      below += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+      below += (k.x == mine && j < i) + (k.y == mine && j + 1 < i) + (k.z == mine && j + 2 < i) +
+               (k.w == mine && j + 3 < i);
+    }
+  }
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) below += __shfl_xor_sync(0xffffffffu, below, o);
+  if (tid % 16 == 0 && i < n) out[below] = make_uint2(FITS ? mine >> kRankBits : mine, uint32_t(i));
 }
 
 __global__ void __launch_bounds__(kSortThreads, 1)
     emb_sort_kernel(const int64_t *__restrict__ tokens, int64_t n, int64_t vocab, int64_t padding, int passes, int bits,
-                    uint2 *buf0, uint2 *buf1, uint32_t *counters, int64_t counters_n, char *zero, int64_t zero_rows,
-                    int64_t zero_bytes, int64_t zero_stride) {
-  extern __shared__ __align__(16) uint32_t sh[];
+                    uint2 *buf0, uint2 *buf1, uint32_t *counters, int64_t counters_n,
+                    const __grid_constant__ Zeros zeros) {
+  extern __shared__ uint32_t sh[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) ks_pdl_release();
   if (blockIdx.x >= kCluster) {
-    const int64_t ctas = gridDim.x - kCluster, cta = blockIdx.x - kCluster;
-    for (int i = tid; i < kZeroBytes / 16; i += kSortThreads) reinterpret_cast<uint4 *>(sh)[i] = make_uint4(0, 0, 0, 0);
-    ks_fence_proxy_async();
-    __syncthreads();
-    if (zero_rows == 1)
-      zero_span(zero, zero_bytes, sh, cta, ctas);
-    else
-      for (int64_t r = cta; r < zero_rows; r += ctas) zero_span(zero + r * zero_stride, zero_bytes, sh, 0, 1);
-    if (tid == 0) {
-      ks_bulk_commit_group();
-      ks_bulk_wait_all();
-    }
+    zero_rows(zeros, int64_t(blockIdx.x) - kCluster);
     return;
   }
   for (int64_t i = int64_t(blockIdx.x) * kSortThreads + tid; i < counters_n; i += kCluster * kSortThreads) counters[i] = 0;
@@ -189,12 +231,20 @@ __global__ void __launch_bounds__(kSortThreads, 1)
     auto fetch = [&](int64_t i) {
       if (pass > 0) return __ldcg(in + i);
       const int64_t t = __ldg(tokens + i);
-      return make_uint2(t < 0 || t >= vocab || t == padding ? uint32_t(vocab) : uint32_t(t), uint32_t(i));
+      return make_uint2(token_key(t, vocab, padding), uint32_t(i));
     };
     for (int i = tid; i < kSortWarps * bins; i += kSortThreads) count[i] = 0;
     __syncthreads();
     uint32_t *mine = count + warp * bins;
-    for (int64_t i = lo + lane; i < hi; i += 32) atomicAdd(mine + ((fetch(i).x >> shift) & (bins - 1)), 1u);
+    for (int64_t i = lo + lane; i < hi; i += 32 * kBatch) {
+      uint2 kv[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i + u * 32 < hi) kv[u] = fetch(i + u * 32);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i + u * 32 < hi) atomicAdd(mine + ((kv[u].x >> shift) & (bins - 1)), 1u);
+    }
     __syncthreads();
     if (tid < bins) {
       uint32_t s = 0;
@@ -239,86 +289,52 @@ __global__ void __launch_bounds__(kSortThreads, 1)
     __syncthreads();
     if (tid < bins) base[tid] = before + incl - total + (warp ? wsum[warp - 1] : 0u);
     __syncthreads();
-    for (int64_t i0 = lo; i0 < hi; i0 += 32) {
-      const int64_t i = i0 + lane;
-      const bool have = i < hi;
-      uint2 kv = make_uint2(0, 0);
-      if (have) kv = fetch(i);
-      const uint32_t d = have ? (kv.x >> shift) & (bins - 1) : uint32_t(bins);
-      const uint32_t peers = __match_any_sync(0xffffffffu, d);
-      const uint32_t below = __popc(peers & ((1u << lane) - 1u));
-      if (have) out[base[d] + mine[d] + below] = kv;
-      __syncwarp();
-      if (have && below == 0) mine[d] += __popc(peers);
-      __syncwarp();
+    for (int64_t i0 = lo + lane; i0 - lane < hi; i0 += 32 * kBatch) {
+      uint2 kv[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+        if (i0 + u * 32 < hi) kv[u] = fetch(i0 + u * 32);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (i0 - lane + u * 32 >= hi) break;
+        const bool have = i0 + u * 32 < hi;
+        const uint32_t d = have ? (kv[u].x >> shift) & (bins - 1) : uint32_t(bins);
+        const uint32_t peers = __match_any_sync(0xffffffffu, d);
+        const uint32_t below = __popc(peers & ((1u << lane) - 1u));
+        if (have) out[base[d] + mine[d] + below] = kv[u];
+        __syncwarp();
+        if (have && below == 0) mine[d] += __popc(peers);
+        __syncwarp();
+      }
     }
     ks_cluster_sync();  // out is complete; cta_count may be rewritten
   }
 }
 
 // ---------------------------------------------------------------------------
-// Sums over the sorted positions.  A warp takes `chunk` (at most 32) of them
-// and kSeg columns; U rows' loads are in flight.  part: [chunk][2][ld] fp32,
-// slot 0 for a token that began in an earlier chunk, slot 1 for one that goes
-// on into the next.
+// Sums over the sorted positions.  A CTA takes one chunk of them and one
+// segment of columns (16 bytes a thread); every CTA has the same number of
+// rows to read, whatever the tokens are.  The rows come through a ring of
+// shared memory, kStages stages of kRows rows, filled by bulk copies (one per
+// row, of up to 4 KB), so that about 100 KB a CTA are in flight while the
+// threads add; reading them into registers instead (warps over short windows,
+// 4 to 8 rows in flight each) reached 3.4 TB/s at 131072 x 1024 fp32.  Rows that
+// are not 16-byte aligned are read with plain loads, four rows at a time.
+// part: [chunk][2][ld] fp32, slot 0 for a token that began in an earlier chunk,
+// slot 1 for one that goes on into the next.
 // ---------------------------------------------------------------------------
-template <int DT, int ODT, bool VEC>
-struct Sum {
-  using E = Elem<DT>;
-  using O = Elem<ODT>;
-  static constexpr int W = E::kPer, kSeg = 32 * W;
-  float a[W];
-  KS_DEV void clear() {
-#pragma unroll
-    for (int j = 0; j < W; ++j) a[j] = 0.f;
-  }
-  KS_DEV static int64_t col(int j, int lane) { return VEC ? lane * W + j : lane + j * 32; }
-  KS_DEV void put_part(float *p, int64_t c, int64_t dim, int lane) const {
-    if constexpr (VEC) {
-      if (c + lane * W < dim) {
-#pragma unroll
-        for (int j = 0; j < W; j += 4)
-          *reinterpret_cast<float4 *>(p + c + lane * W + j) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        if (c + col(j, lane) < dim) p[c + col(j, lane)] = a[j];
-    }
-  }
-  KS_DEV void add_part(const float *p, int64_t c, int64_t dim, int lane) {
-    if constexpr (VEC) {
-      if (c + lane * W < dim) {
-#pragma unroll
-        for (int j = 0; j < W; j += 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + c + lane * W + j));
-          a[j] += v.x;
-          a[j + 1] += v.y;
-          a[j + 2] += v.z;
-          a[j + 3] += v.w;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < W; ++j)
-        if (c + col(j, lane) < dim) a[j] += __ldcg(p + c + col(j, lane));
-    }
-  }
-  KS_DEV void finish(typename O::T *row, int64_t c, int64_t dim, int lane, float scale, bool accumulate) {
-    Raw<ODT, W, VEC> o;
-    if (accumulate) o.load(row + c, c, dim, lane);
-#pragma unroll
-    for (int j = 0; j < W; ++j) o.v[j] = O::put(accumulate ? fmaf(a[j], scale, O::get(o.v[j])) : a[j] * scale);
-    o.store(row + c, c, dim, lane);
-  }
-};
+constexpr int kRows = 8;
+constexpr int kStages = 3;
+constexpr int kMaxChunk = 1024;
+constexpr int kSegThreads = 256;  // at most: 4 KB of a row
 
-// What every warp of a launch shares.
+// What every CTA of a launch shares.
 template <int DT, int ODT>
 struct GradArgs {
   const uint2 *sorted;
   int64_t n;
   int chunk;
+  uint32_t segs;
   const typename Elem<DT>::T *dout;
   int64_t dout_stride;
   typename Elem<ODT>::T *dtable;
@@ -327,124 +343,242 @@ struct GradArgs {
   int accumulate;
   float *part;
   int64_t ld;
-  uint32_t *arrived;  // [chunk][2][segment] warps of a group that left their partials, [chunk][segment] groups
+  uint32_t *arrived;  // [chunk][2][segment] CTAs of a group that left their partials, [chunk][segment] groups
   int64_t chunks;
 };
 
-constexpr int64_t kGroup = 64;  // chunks whose partials one warp adds up
-
-// A token of which this warp (chunk ch, segment seg) has just left a partial
-// sum, in slot 1 if it begins here, goes on elsewhere.  The last of the warps
-// that hold a part of it, within each group of 64 chunks, adds the group's
-// partials in order; the last group adds the groups'.  So the order of the sum
-// is that of the chunks, whoever comes last, and a token that fills the whole
-// batch (131072 positions: 4096 partials) is joined in two short chains.
+// A thread's sums: `per` adjacent columns (VEC), or 8 of them blockDim apart.
 template <int DT, int ODT, bool VEC>
-KS_DEV void join(const GradArgs<DT, ODT> &g, uint32_t key, int64_t ch, int64_t seg, int64_t segs, bool begins, bool goes_on,
-                 int lane) {
+struct Sum {
+  using E = Elem<DT>;
+  using O = Elem<ODT>;
+  static constexpr int W = VEC ? E::kPer : 8;
+  float a[W];
+  KS_DEV static int cols() { return blockDim.x * W; }
+  KS_DEV static int col(int j) { return VEC ? threadIdx.x * W + j : threadIdx.x + j * blockDim.x; }
+  KS_DEV void clear() {
+#pragma unroll
+    for (int j = 0; j < W; ++j) a[j] = 0.f;
+  }
+  // c: the segment's first column
+  KS_DEV void put_part(float *p, int64_t c, int64_t dim) const {
+#pragma unroll
+    for (int j = 0; j < W; j += VEC ? 4 : 1) {
+      if (c + col(j) >= dim) continue;
+      if constexpr (VEC)
+        *reinterpret_cast<float4 *>(p + c + col(j)) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
+      else
+        p[c + col(j)] = a[j];
+    }
+  }
+  KS_DEV void add_part(const float *p, int64_t c, int64_t dim) {
+#pragma unroll
+    for (int j = 0; j < W; j += VEC ? 4 : 1) {
+      if (c + col(j) >= dim) continue;
+      if constexpr (VEC) {
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + c + col(j)));
+        a[j] += v.x;
+        a[j + 1] += v.y;
+        a[j + 2] += v.z;
+        a[j + 3] += v.w;
+      } else {
+        a[j] += __ldcg(p + c + col(j));
+      }
+    }
+  }
+  KS_DEV void finish(typename O::T *row, int64_t c, int64_t dim, float scale, bool accumulate) const {
+    constexpr int step = VEC ? W < O::kPer ? W : O::kPer : 1;  // values per 16-byte store
+    static_assert(!VEC || step * sizeof(typename O::T) == 16, "whole vectors");
+#pragma unroll
+    for (int j = 0; j < W; j += step) {
+      if (c + col(j) >= dim) continue;
+      typename O::T *p = row + c + col(j);
+      alignas(16) typename O::T o[step];
+      if (accumulate) {
+        if constexpr (VEC)
+          *reinterpret_cast<uint4 *>(o) = *reinterpret_cast<const uint4 *>(p);
+        else
+          o[0] = *p;
+      }
+#pragma unroll
+      for (int k = 0; k < step; ++k) o[k] = O::put(accumulate ? fmaf(a[j + k], scale, O::get(o[k])) : a[j + k] * scale);
+      if constexpr (VEC)
+        *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(o);
+      else
+        *p = o[0];
+    }
+  }
+};
+
+constexpr int64_t kGroup = 64;  // chunks whose partials one CTA adds up
+
+// A token that lies in chunks a to b, of which this CTA (chunk ch, segment seg)
+// has just left a partial sum.  The last of the CTAs that hold a part of it,
+// within each group of 64 chunks, adds the group's partials in order; the last
+// group adds the groups'.  So the order of the sum is that of the chunks,
+// whoever comes last, and a token that fills the whole batch is joined in two
+// short chains.  (A kernel of its own for the joins cost 4 us more at 777 x 1001
+// and 12 at 131072 x 1024.)
+template <int DT, int ODT, bool VEC>
+KS_DEV void join(const GradArgs<DT, ODT> &g, uint32_t key, int64_t ch, int64_t seg, int64_t a, int64_t b) {
   using S = Sum<DT, ODT, VEC>;
-  const int64_t c = seg * S::kSeg;
-  int64_t a = ch, b = ch;  // the token's first and last chunk
-  if (!begins) {
-    for (int64_t j = ch - 1;; j -= 32) {  // lane l: does it begin before chunk j - l?
-      const int64_t at = (j - lane) * g.chunk;
-      const bool on = at > 0 && __ldcg(&g.sorted[at - 1].x) == key;
-      const uint32_t stop = __ballot_sync(0xffffffffu, !on);
-      if (stop) {
-        a = j - (__ffs(stop) - 1);
-        break;
-      }
-    }
-  }
-  if (goes_on) {
-    for (int64_t j = ch + 1;; j += 32) {  // lane l: does it go on past chunk j + l?
-      const int64_t end = (j + lane + 1) * g.chunk;
-      const bool on = end < g.n && __ldcg(&g.sorted[end].x) == key;
-      const uint32_t stop = __ballot_sync(0xffffffffu, !on);
-      if (stop) {
-        b = j + (__ffs(stop) - 1);
-        break;
-      }
-    }
-  }
+  __shared__ bool last_one;
+  const int64_t c = seg * S::cols(), segs = g.segs;
   auto slot = [&](int64_t chunk) { return g.part + (chunk * 2 + (chunk == a ? 1 : 0)) * g.ld; };
   auto last_of = [&](uint32_t *counter, int64_t expected) {
     __threadfence();
-    __syncwarp();
-    uint32_t before = 0;
-    if (lane == 0) before = atomicAdd(counter, 1u);
-    before = __shfl_sync(0xffffffffu, before, 0);
+    __syncthreads();
+    if (threadIdx.x == 0) last_one = int64_t(atomicAdd(counter, 1u)) == expected - 1;
+    __syncthreads();
+    const bool l = last_one;
     __threadfence();
-    return int64_t(before) == expected - 1;
+    __syncthreads();  // last_one may be written again
+    return l;
   };
   const int64_t first = max(a, ch / kGroup * kGroup), last = min(b, ch / kGroup * kGroup + kGroup - 1);
   if (!last_of(g.arrived + (first * 2 + (first == a ? 1 : 0)) * segs + seg, last - first + 1)) return;
   S sum;
   sum.clear();
 #pragma unroll 4
-  for (int64_t j = first; j <= last; ++j) sum.add_part(slot(j), c, g.dim, lane);
+  for (int64_t j = first; j <= last; ++j) sum.add_part(slot(j), c, g.dim);
   const int64_t ga = a / kGroup, gb = b / kGroup;
   if (ga != gb) {
-    sum.put_part(slot(first), c, g.dim, lane);
+    sum.put_part(slot(first), c, g.dim);
     if (!last_of(g.arrived + g.chunks * 2 * segs + a * segs + seg, gb - ga + 1)) return;
     sum.clear();
 #pragma unroll 4
-    for (int64_t j = ga; j <= gb; ++j) sum.add_part(slot(max(a, j * kGroup)), c, g.dim, lane);
+    for (int64_t j = ga; j <= gb; ++j) sum.add_part(slot(max(a, j * kGroup)), c, g.dim);
   }
-  sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, lane, g.scale, g.accumulate != 0);
+  sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, g.scale, g.accumulate != 0);
 }
 
 template <int DT, int ODT, bool VEC>
-__global__ void __launch_bounds__(256) emb_grad_kernel(const __grid_constant__ GradArgs<DT, ODT> g) {
+__global__ void __launch_bounds__(kSegThreads)
+    emb_grad_kernel(const __grid_constant__ GradArgs<DT, ODT> g, KsWait wait) {
   using S = Sum<DT, ODT, VEC>;
-  constexpr int U = 8;
-  ks_pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t segs = (g.dim + S::kSeg - 1) / S::kSeg;
-  const int64_t id = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t ch = id / segs, seg = id - ch * segs, c = seg * S::kSeg;
+  using E = Elem<DT>;
+  using T = typename E::T;
+  extern __shared__ __align__(128) uint8_t ring[];  // VEC: [kStages][kRows][16 * blockDim]
+  __shared__ uint2 kv[kMaxChunk];
+  __shared__ uint64_t full[kStages];
+  __shared__ int gave_up;
+  const int tid = threadIdx.x;
+  const int64_t ch = blockIdx.x / g.segs, seg = blockIdx.x - ch * g.segs, c = seg * S::cols();
   const int64_t lo = ch * g.chunk;
-  if (lo >= g.n) return;
-  const int cnt = int(min(int64_t(g.chunk), g.n - lo));
-  uint2 kv = make_uint2(0, 0);
-  if (lane < cnt) kv = __ldcg(g.sorted + lo + lane);
-  const uint32_t none = 0xffffffffu;  // no token: vocab < 2^31
+  const int held = int(min(int64_t(g.chunk), g.n - lo));
+  if (VEC && tid == 0) {
+    for (int s = 0; s < kStages; ++s) ks_mbar_init(full + s, 1);
+    gave_up = 0;
+    ks_fence_mbar_init();
+  }
+  ks_pdl_wait();
+  for (int i = tid; i < held; i += blockDim.x) kv[i] = __ldcg(g.sorted + lo + i);
+  constexpr uint32_t none = 0xffffffffu;  // no token: vocab < 2^31
   const uint32_t prev = lo > 0 ? __ldcg(&g.sorted[lo - 1].x) : none;
-  const uint32_t next = lo + cnt < g.n ? __ldcg(&g.sorted[lo + cnt].x) : none;
-  bool from_before = prev == __shfl_sync(0xffffffffu, kv.x, 0);
-  float *slots = g.part + ch * 2 * g.ld;
-  S sum;
-  sum.clear();
-  for (int i0 = 0; i0 < cnt; i0 += U) {
-    Raw<DT, S::W, VEC> x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t key = __shfl_sync(0xffffffffu, kv.x, (i0 + u) & 31);
-      const int64_t pos = __shfl_sync(0xffffffffu, kv.y, (i0 + u) & 31);
-      const bool take = i0 + u < cnt && key < g.vocab;
-      x[u].load(g.dout + (take ? pos * g.dout_stride : 0) + c, c, take ? g.dim : 0, lane);
+  uint32_t next = lo + held < g.n ? __ldcg(&g.sorted[lo + held].x) : none;
+  __syncthreads();
+  int cnt = held;  // the excluded tokens come last
+  if (kv[held - 1].x >= g.vocab) {
+    int a = 0, b = held - 1;  // the first of them
+    while (a < b) {
+      const int m = (a + b) / 2;
+      if (kv[m].x >= g.vocab) b = m;
+      else a = m + 1;
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u;
-      if (i >= cnt) break;
-      const uint32_t key = __shfl_sync(0xffffffffu, kv.x, i);
-      if (key >= g.vocab) return;  // the excluded tokens come last
-      const uint32_t after = i + 1 < cnt ? __shfl_sync(0xffffffffu, kv.x, (i + 1) & 31) : next;
-#pragma unroll
-      for (int j = 0; j < S::W; ++j) sum.a[j] += S::E::get(x[u].v[j]);
-      if (after != key || i + 1 == cnt) {
-        if (from_before || after == key) {
-          sum.put_part(from_before ? slots : slots + g.ld, c, g.dim, lane);
-          join<DT, ODT, VEC>(g, key, ch, seg, segs, !from_before, after == key, lane);
-        } else {
-          sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, lane, g.scale, g.accumulate != 0);
-        }
-        sum.clear();
-        from_before = false;
+    cnt = a;
+    next = none;
+  }
+  if (cnt == 0) return;
+  constexpr int R = VEC ? kRows : 4;  // plain loads: 8 x 4 registers in flight
+  const int stages = (cnt + R - 1) / R;
+  const uint32_t row_bytes = uint32_t(min(int64_t(S::cols()), g.dim - c) * int64_t(sizeof(T)));
+  const uint32_t pitch = blockDim.x * 16;
+  // rows of stage st into its place of the ring, one copy per lane
+  auto fill = [&](int st) {
+    if (st >= stages || tid >= 32) return;
+    const int rows = min(kRows, cnt - st * kRows), s = st % kStages;
+    if (tid == 0) ks_mbar_arrive_expect_tx(full + s, rows * row_bytes);
+    __syncwarp();
+    if (tid < rows)
+      ks_bulk_load(ring + (s * kRows + tid) * pitch, g.dout + int64_t(kv[st * kRows + tid].y) * g.dout_stride + c, row_bytes,
+                   full + s);
+  };
+  if constexpr (VEC)
+    for (int s = 0; s < kStages; ++s) fill(s);
+  // chunks that the first and the last token reach to, searched for while the
+  // first rows are on their way: 32 chunk edges at a time, by every warp for itself
+  int64_t first_chunk = ch, last_chunk = ch;
+  bool from_before = prev == kv[0].x;
+  if (from_before) {
+    for (int64_t j = ch - 1;; j -= 32) {  // lane l: does the token begin before chunk j - l?
+      const int64_t at = (j - (tid & 31)) * g.chunk;
+      const uint32_t stop = __ballot_sync(0xffffffffu, !(at > 0 && __ldcg(&g.sorted[at - 1].x) == prev));
+      if (stop) {
+        first_chunk = j - (__ffs(stop) - 1);
+        break;
       }
     }
   }
+  if (next == kv[cnt - 1].x) {
+    for (int64_t j = ch + 1;; j += 32) {  // lane l: does it go on past chunk j + l?
+      const int64_t end = (j + (tid & 31) + 1) * g.chunk;
+      const uint32_t stop = __ballot_sync(0xffffffffu, !(end < g.n && __ldcg(&g.sorted[end].x) == next));
+      if (stop) {
+        last_chunk = j + (__ffs(stop) - 1);
+        break;
+      }
+    }
+  }
+  uint32_t head = none, tail = none;  // tokens of which this CTA leaves a partial sum
+  bool head_goes_on = false;
+  S sum;
+  sum.clear();
+  for (int st = 0; st < stages; ++st) {
+    T x[R][S::W];
+    if constexpr (VEC) {
+      if (!ks_mbar_wait(full + st % kStages, (st / kStages) & 1, &gave_up, wait)) return;
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool in = st * R + r < cnt;
+        const T *p = g.dout + (in ? int64_t(kv[st * R + r].y) * g.dout_stride : 0) + c;
+#pragma unroll
+        for (int j = 0; j < S::W; ++j) x[r][j] = in && c + S::col(j) < g.dim ? __ldg(p + S::col(j)) : T(0);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int i = st * R + r;
+      if (i >= cnt) break;
+      if constexpr (VEC) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(ring + ((st % kStages) * kRows + r) * pitch + tid * 16);
+        *reinterpret_cast<uint4 *>(x[r]) = v;
+      }
+#pragma unroll
+      for (int j = 0; j < S::W; ++j) sum.a[j] += E::get(x[r][j]);
+      const uint32_t key = kv[i].x, after = i + 1 < cnt ? kv[i + 1].x : next;
+      const bool goes_on = after == key;
+      if (goes_on && i + 1 < cnt) continue;
+      if (from_before) {
+        sum.put_part(g.part + ch * 2 * g.ld, c, g.dim);
+        head = key;
+        head_goes_on = goes_on;
+      } else if (goes_on) {
+        sum.put_part(g.part + (ch * 2 + 1) * g.ld, c, g.dim);
+        tail = key;
+      } else {
+        sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, g.scale, g.accumulate != 0);
+      }
+      sum.clear();
+      from_before = false;
+    }
+    if constexpr (VEC) {
+      __syncthreads();  // the stage has been read
+      fill(st + kStages);
+    }
+  }
+  if (head != none) join<DT, ODT, VEC>(g, head, ch, seg, first_chunk, head_goes_on ? last_chunk : ch);
+  if (tail != none) join<DT, ODT, VEC>(g, tail, ch, seg, ch, last_chunk);
 }
 
 // ---------------------------------------------------------------------------
@@ -473,6 +607,10 @@ int check_sizes(const char *what, int64_t n, int64_t vocab, int64_t dim, int dt,
 
 struct GradPlan {
   int chunk;
+  bool vec;
+  int threads;           // of a CTA of emb_grad_kernel
+  int64_t segs;          // segments of columns
+  size_t shm;            // its ring
   int64_t chunks, ld;
   int bits, passes;
   int64_t counters;
@@ -482,8 +620,8 @@ struct GradPlan {
 int grad_check(const ks_embedding_grad_config &c, const ks_embedding_grad_args &a, char *reason, size_t len) {
   int s = check_sizes("embedding_grad", a.tokens_count, a.vocab, a.dim, a.dtype, reason, len);
   if (s != KS_OK) return s;
-  if (c.chunk < 0 || c.chunk > 32) {
-    ks::set_reason(reason, len, "embedding_grad: chunk must be 0 (chosen) or 1..32");
+  if (c.chunk < 0 || c.chunk > kMaxChunk) {
+    ks::set_reason(reason, len, "embedding_grad: chunk must be 0 (chosen) or 1..%d", kMaxChunk);
     return KS_ERR_INVALID_CONFIG;
   }
   if (a.out_dtype != a.dtype && a.out_dtype != KS_F32) {
@@ -501,19 +639,34 @@ int grad_check(const ks_embedding_grad_config &c, const ks_embedding_grad_args &
 GradPlan grad_plan(const ks_embedding_grad_config &c, const ks_embedding_grad_args &a) {
   GradPlan p;
   const int64_t n = a.tokens_count;
-  const int64_t segs = (a.dim * elem_size(a.dtype) + 511) / 512;
-  // 32 positions a warp where that leaves 16 warps for every SM, fewer positions otherwise
-  p.chunk = c.chunk;
-  if (p.chunk == 0) {
-    p.chunk = 32;
-    while (p.chunk > 4 && (n + p.chunk - 1) / p.chunk * segs < 16LL * ks::sm_count()) p.chunk /= 2;
-  }
-  p.chunks = (n + p.chunk - 1) / p.chunk;
+  const int esz = elem_size(a.dtype);
   p.ld = (a.dim + 63) / 64 * 64;
+  int64_t most_chunks = 0, most_counters = 0;  // of both kinds of rows: the workspace's size goes by the sizes alone
+  const bool vec = aligned16(a.dout, a.dout_stride, a.dim, esz) &&
+                   aligned16(a.dtable, a.dtable_stride, a.dim, elem_size(a.out_dtype)) && a.dim % (16 / esz) == 0;
+  for (const bool v : {!vec, vec}) {
+    p.vec = v;
+    const int64_t want = v ? (a.dim * esz + 15) / 16 : (a.dim + 7) / 8;  // threads for a whole row
+    p.segs = (want + kSegThreads - 1) / kSegThreads;
+    p.threads = int(((want + p.segs - 1) / p.segs + 31) / 32 * 32);
+    p.segs = (want + p.threads - 1) / p.threads;
+    p.shm = v ? size_t(kStages) * kRows * p.threads * 16 : 0;
+    // one round of CTAs, as many as the SMs hold; two where chunks stay long
+    // (131072 x 1024 fp32: 242 us in one round of 448 positions, 222 in two)
+    const int64_t per_sm = std::min<int64_t>({int64_t(227 * 1024 / (p.shm + 9 * 1024 + 512)), 1024 / p.threads, 16});
+    int64_t even = (n * p.segs + per_sm * ks::sm_count() - 1) / (per_sm * ks::sm_count());
+    if (even >= 256) even = (even + 1) / 2;
+    p.chunk = c.chunk ? c.chunk : int(std::min<int64_t>(kMaxChunk, (even + kRows - 1) / kRows * kRows));
+    p.chunks = (n + p.chunk - 1) / p.chunk;
+    p.counters = p.chunks * 3 * p.segs;
+    most_chunks = std::max(most_chunks, p.chunks);
+    most_counters = std::max(most_counters, p.counters);
+  }
   int b = 1;
   while ((int64_t(1) << b) <= a.vocab) ++b;  // keys 0..vocab
   p.passes = (b + 9) / 10;
   p.bits = (b + p.passes - 1) / p.passes;
+  if (n <= kRankMax) p.passes = 1;  // one pass of comparisons instead
   size_t o = 0;
   auto take = [&](size_t bytes) {
     const size_t at = o;
@@ -522,23 +675,42 @@ GradPlan grad_plan(const ks_embedding_grad_config &c, const ks_embedding_grad_ar
   };
   p.o_buf0 = take(size_t(n) * 8);
   p.o_buf1 = take(p.passes > 1 ? size_t(n) * 8 : 0);
-  // (segments of the narrower lane-strided path are as many: 512 bytes or 32 x per elements alike)
-  p.counters = p.chunks * 3 * segs;
-  p.o_count = take(size_t(p.counters) * 4);
-  p.o_part = take(size_t(p.chunks) * 2 * p.ld * 4);
+  p.o_count = take(size_t(most_counters) * 4);
+  p.o_part = take(size_t(most_chunks) * 2 * p.ld * 4);
   p.bytes = o;
   return p;
 }
 
+int sort_launch(const ks_embedding_grad_args &a, const GradPlan &p, uint2 *buf0, uint2 *buf1, uint32_t *counters,
+                const Zeros &zeros, unsigned zero_ctas, cudaStream_t st) {
+  const size_t shm = (size_t(kSortWarps) + 2) * (size_t(1) << p.bits) * 4;
+  cudaError_t e = cudaFuncSetAttribute(emb_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shm));
+  if (e != cudaSuccess) return ks::map_cuda(e);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(kCluster + (zero_ctas + kCluster - 1) / kCluster * kCluster);
+  lc.blockDim = dim3(kSortThreads);
+  lc.dynamicSmemBytes = shm;
+  lc.stream = st;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  return ks::map_cuda(cudaLaunchKernelEx(&lc, emb_sort_kernel, a.tokens, a.tokens_count, a.vocab, a.padding_idx, p.passes,
+                                         p.bits, buf0, buf1, counters, p.counters, zeros));
+}
+
 template <int DT, int ODT, bool VEC>
 int grad_launch(const ks_embedding_grad_args &a, const GradPlan &p, cudaStream_t st) {
-  using S = Sum<DT, ODT, VEC>;
   using T = typename Elem<DT>::T;
   using O = typename Elem<ODT>::T;
   char *ws = static_cast<char *>(a.workspace);
   const GradArgs<DT, ODT> g = {reinterpret_cast<const uint2 *>(ws + (p.passes & 1 ? p.o_buf0 : p.o_buf1)),
                                a.tokens_count,
                                p.chunk,
+                               uint32_t(p.segs),
                                static_cast<const T *>(a.dout),
                                a.dout_stride,
                                static_cast<O *>(a.dtable),
@@ -551,16 +723,18 @@ int grad_launch(const ks_embedding_grad_args &a, const GradPlan &p, cudaStream_t
                                p.ld,
                                reinterpret_cast<uint32_t *>(ws + p.o_count),
                                p.chunks};
-  const int64_t segs = (a.dim + S::kSeg - 1) / S::kSeg, blocks = (p.chunks * segs + 7) / 8;
-  if (blocks > 0x7fffffff) return KS_ERR_INVALID_ARGS;
-  return ks::launch_kernel(true, emb_grad_kernel<DT, ODT, VEC>, dim3(unsigned(blocks)), dim3(256), 0, st, g);
+  if (p.chunks * p.segs > 0x7fffffff) return KS_ERR_INVALID_ARGS;
+  auto kern = emb_grad_kernel<DT, ODT, VEC>;
+  if (p.shm > 32 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(p.shm));
+    if (e != cudaSuccess) return ks::map_cuda(e);
+  }
+  return ks::launch_kernel(true, kern, dim3(unsigned(p.chunks * p.segs)), dim3(p.threads), p.shm, st, g, ks::wait_ctx());
 }
 
 template <int DT, int ODT>
 int grad_launch_vec(const ks_embedding_grad_args &a, const GradPlan &p, cudaStream_t st) {
-  const bool vec = aligned16(a.dout, a.dout_stride, a.dim, elem_size(DT)) &&
-                   aligned16(a.dtable, a.dtable_stride, a.dim, elem_size(ODT)) && a.dim % Elem<DT>::kPer == 0;
-  return vec ? grad_launch<DT, ODT, true>(a, p, st) : grad_launch<DT, ODT, false>(a, p, st);
+  return p.vec ? grad_launch<DT, ODT, true>(a, p, st) : grad_launch<DT, ODT, false>(a, p, st);
 }
 
 template <int DT>
@@ -569,7 +743,8 @@ int lookup_launch(const ks_embedding_args &a, cudaStream_t st) {
   const int esz = elem_size(DT);
   const bool vec = aligned16(a.table, a.table_stride, a.dim, esz) && aligned16(a.out, a.out_stride, a.dim, esz);
   const int64_t groups = ((a.dim * esz + 511) / 512 + 3) / 4, total = a.tokens_count * groups;
-  const int grid = int(std::min<int64_t>((total + 7) / 8, int64_t(ks::sm_count()) * 64));
+  if ((total + 7) / 8 > 0x7fffffff) return KS_ERR_INVALID_ARGS;
+  const unsigned grid = unsigned((total + 7) / 8);
   auto t = static_cast<const T *>(a.table);
   auto o = static_cast<T *>(a.out);
   return ks::launch_kernel(false, vec ? emb_lookup_kernel<DT, true> : emb_lookup_kernel<DT, false>, dim3(grid), dim3(256), 0, st,
@@ -634,34 +809,30 @@ int ks_embedding_grad_launch(const ks_embedding_grad_config *cfg, const ks_embed
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char *ws = static_cast<char *>(a->workspace);
 
-  int64_t zrows = 0, zbytes = 0;
+  Zeros zeros = {};
   unsigned zero_ctas = 0;
   if (!a->accumulate) {
-    zrows = a->dtable_stride == a->dim ? 1 : a->vocab;
-    zbytes = (zrows == 1 ? a->vocab : 1) * a->dim * osz;
-    const int64_t want = (a->vocab * a->dim * osz + 65535) / 65536;  // 64 KB a CTA at least
-    zero_ctas = unsigned(std::min<int64_t>(want, ks::sm_count() - kCluster));
-    zero_ctas = std::max(1u, zero_ctas / kCluster) * kCluster;
+    // a dense table is one long row
+    const int64_t rows = a->dtable_stride == a->dim ? 1 : a->vocab;
+    const int64_t bytes = (rows == 1 ? a->vocab : 1) * a->dim * osz;
+    // two CTAs for every SM, 512 KB each at most: more rounds of CTAs even out
+    const int64_t share = std::min<int64_t>(512 * 1024, std::max<int64_t>(16 * 1024, rows * bytes / (2 * ks::sm_count())));
+    zeros = Zeros{static_cast<char *>(a->dtable), rows, bytes, a->dtable_stride * osz, (share + 15) / 16 * 16};
+    const int64_t ctas = (rows * bytes + zeros.share - 1) / zeros.share;
+    if (ctas > (1 << 30)) return KS_ERR_INVALID_ARGS;
+    zero_ctas = unsigned(ctas);
   }
-  const size_t shm = std::max<size_t>((size_t(kSortWarps) + 2) * (size_t(1) << p.bits) * 4, kZeroBytes);
-  cudaError_t e = cudaFuncSetAttribute(emb_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shm));
-  if (e != cudaSuccess) return ks::map_cuda(e);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kCluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(kCluster + zero_ctas);
-  lc.blockDim = dim3(kSortThreads);
-  lc.dynamicSmemBytes = shm;
-  lc.stream = st;
-  lc.attrs = attr;
-  lc.numAttrs = 1;
-  e = cudaLaunchKernelEx(&lc, emb_sort_kernel, a->tokens, a->tokens_count, a->vocab, a->padding_idx, p.passes, p.bits,
-                         reinterpret_cast<uint2 *>(ws + p.o_buf0), reinterpret_cast<uint2 *>(ws + p.o_buf1),
-                         reinterpret_cast<uint32_t *>(ws + p.o_count), p.counters, static_cast<char *>(a->dtable), zrows, zbytes, a->dtable_stride * osz);
-  if (e != cudaSuccess) return ks::map_cuda(e);
+  auto counters = reinterpret_cast<uint32_t *>(ws + p.o_count);
+  auto buf0 = reinterpret_cast<uint2 *>(ws + p.o_buf0), buf1 = reinterpret_cast<uint2 *>(ws + p.o_buf1);
+  if (a->tokens_count <= kRankMax) {
+    const unsigned grid = unsigned((a->tokens_count + kRankRows - 1) / kRankRows) + zero_ctas;
+    s = ks::launch_kernel(false, a->vocab < (1 << (32 - kRankBits)) ? emb_rank_kernel<true> : emb_rank_kernel<false>, dim3(grid),
+                          dim3(kSortThreads), 0, st, a->tokens, int(a->tokens_count), a->vocab, a->padding_idx, buf0,
+                          counters, p.counters, zeros);
+  } else {
+    s = sort_launch(*a, p, buf0, buf1, counters, zeros, zero_ctas, st);
+  }
+  if (s != KS_OK) return s;
   if (a->dtype == KS_BF16)
     return a->out_dtype == KS_F32 ? grad_launch_vec<KS_BF16, KS_F32>(*a, p, st)
                                   : grad_launch_vec<KS_BF16, KS_BF16>(*a, p, st);

@@ -525,9 +525,8 @@ KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool 
   float a0 = 0.f, a1 = 0.f;
   int64_t k = 0;
   if (((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15) == 0) {
-    for (; k + 8 <= dim; k += 256) {
-      const int64_t at = k + lane * 8;
-      if (at + 8 > dim) continue;
+#pragma unroll 4
+    for (int64_t at = lane * 8; at + 8 <= dim; at += 256) {
       const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(h + at)), y = __ldcg(reinterpret_cast<const uint4 *>(w + at));
       a0 = fmaf(val(x.x, 0), val(y.x, 0), a0);
       a1 = fmaf(val(x.x, 1), val(y.x, 1), a1);
@@ -665,9 +664,9 @@ __global__ void __launch_bounds__(256)
 }
 
 // STORE's exponentials e -> d in place: d = f (e exp(tile maximum - lse) -
-// [target]).  A warp takes 256 columns (16 bytes a lane) of one row at a time,
-// four of them in flight; a block's eight warps take eight rows, whose tile
-// maxima share 32-byte sectors.  Reads and writes 2 bytes a value.
+// [target]).  A warp takes 1024 columns of one row, four 16-byte loads a lane
+// in flight; a block's eight warps take eight rows, whose tile maxima share
+// 32-byte sectors.  Reads and writes 2 bytes a value.
 __global__ void __launch_bounds__(256)
     ce_scale_kernel(uint16_t *__restrict__ d, int64_t ld, const float2 *__restrict__ part, int64_t rows_p, int tile_log2,
                     const float *__restrict__ lse, const float *__restrict__ tlogit, const int64_t *__restrict__ targets,
@@ -683,8 +682,8 @@ __global__ void __launch_bounds__(256)
   const float l2 = __ldcg(lse + row) * kLog2e;
   uint16_t *dr = d + row * ld;
   const float dt = valid ? f * ex2(fmaf(__ldcg(tlogit + row), kLog2e, -l2)) - f : 0.f;
-  const int64_t step = int64_t(gridDim.y) * 256;
-  for (int64_t c0 = int64_t(blockIdx.y) * 256 + lane * 8; c0 < ld; c0 += 4 * step) {
+  constexpr int step = 256;
+  for (int64_t c0 = int64_t(blockIdx.y) * (4 * step) + lane * 8; c0 < ld; c0 += int64_t(gridDim.y) * (4 * step)) {
     uint4 v[4];
     float k[4];
 #pragma unroll
@@ -1152,7 +1151,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.dloss = a.reduction == KS_CE_NONE ? a.dloss : nullptr;
     if (p.store) {
       const unsigned rows8 = unsigned((a.tokens + 7) / 8);
-      const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, std::max<int64_t>(1, 8192 / rows8)));
+      const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, 65535));
       s = ks::launch_kernel(true, ce_scale_kernel, dim3(rows8, cols), dim3(256), 0, st, reinterpret_cast<uint16_t *>(d), vpad, g.part,
                           p.rows_p, t1 == 256 ? 8 : 7, lse, g.tlogit, a.targets, a.tokens, a.vocab, a.ignore_index, sc,
                           g.f16);

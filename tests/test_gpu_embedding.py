@@ -95,7 +95,8 @@ def _check_grad(torch, got, tokens, dout, vocab, scale, out_name, base=None, pad
 
 
 GRAD_SHAPES = [(1, 1, 1), (1, 512, 5), (31, 64, 3), (32, 65, 1), (33, 256, 40), (200, 1001, 50), (777, 264, 5003),
-               (5000, 128, 1023), (5000, 40, 1024), (9000, 96, 70000), (20000, 72, 1100000)]
+               (4096, 48, 1048575), (4096, 48, 1048576), (4097, 48, 300), (3500, 16, 3000000), (5000, 128, 1023),
+               (5000, 40, 1024), (9000, 96, 70000), (12000, 24, 900), (70000, 8, 5), (20000, 72, 1100000)]
 
 
 @pytest.mark.parametrize("names", [("bf16", "bf16"), ("bf16", "fp32"), ("fp16", "fp16"), ("fp16", "fp32"), ("fp32", "fp32")],
@@ -113,17 +114,17 @@ def test_gradient(ks, shape, names):
     _check_grad(torch, got, tokens, dout, vocab, 0.75, names[1])
 
 
-@pytest.mark.parametrize("chunk", [0, 1, 2, 5, 8, 31, 32])
-@pytest.mark.parametrize("kind", ["one", "two", "few", "sorted", "all different", "outside"])
+@pytest.mark.parametrize("chunk", [0, 1, 7, 8, 31, 32, 100, 1024])
+@pytest.mark.parametrize("kind", ["one", "two", "few", "sorted", "all different", "edges", "outside"])
 def test_runs_and_chunk_edges(ks, kind, chunk):
     """Tokens that fill many chunks, end at chunk edges or inside them."""
     N, ops, torch = ks
-    n, dim, vocab = 3000, 136, 4000
+    n, dim, vocab = 9001, (136, 1000)[chunk % 4 == 0], 4000
     g = _gen(torch, 1)
     dout = _rows(torch, g, n, dim, 0, torch.bfloat16)
     i = torch.arange(n, device="cuda")
     tokens = {"one": torch.full_like(i, 3999), "two": i % 2, "few": (i * 7919) % 13, "sorted": i // 32,
-              "all different": (i * 1009) % 4000, "outside": torch.full_like(i, 4000)}[kind]
+              "all different": (i * 1009) % 4000, "edges": i // 128 * 2 + (i % 128 >= 8), "outside": torch.full_like(i, 4000)}[kind]
     cfg = N.EmbeddingGradConfig(chunk)
     args = dict(dtype=torch.float32, cfg=cfg)
     got = ops.embedding_backward(tokens, dout, vocab, 1.0, **args)
@@ -237,6 +238,7 @@ def test_no_tokens_and_refusals(ks):
     ]:
         with pytest.raises(ValueError):
             bad()
-    with pytest.raises(N.KsError) as e:
-        ops.embedding_backward(tokens, dout, 10, cfg=N.EmbeddingGradConfig(33))
-    assert e.value.status == N.KS_ERR_INVALID_CONFIG
+    for chunk in (-1, 1025):
+        with pytest.raises(N.KsError) as e:
+            ops.embedding_backward(tokens, dout, 10, cfg=N.EmbeddingGradConfig(chunk))
+        assert e.value.status == N.KS_ERR_INVALID_CONFIG
