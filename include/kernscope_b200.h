@@ -273,15 +273,15 @@ int ks_flash_attention_launch(const ks_flash_attention_config *cfg,
  * workspace, in pieces of the vocabulary, from logits taken a second time;
  * KS_CE_GRAD with a workspace that holds d whole keeps 16-bit exponentials
  * there in the first pass and saves the second.
- * cfg.tile_m: 0 = chosen from the sizes, 128 = 128 x 128 tiles, 256 = 256 x
- * 256 tiles.  cfg.piece: vocabulary columns per piece of the backward pass, a
+ * cfg.tile_m x cfg.tile_n: 0 x 0 = chosen from the sizes for each product,
+ * 128 x 128, 128 x 256 or 256 x 256.  cfg.piece: vocabulary columns per piece of the backward pass, a
  * multiple of 256; 0 = as many as the workspace holds.
  * ks_linear_ce_workspace_bytes() gives the least size that works and the
  * size that the call makes use of (at most about limit bytes, or `least`
  * where that is more); the workspace is 256-byte aligned.                    */
 typedef enum ks_ce_pass { KS_CE_FORWARD = 0, KS_CE_BACKWARD = 1, KS_CE_GRAD = 2 } ks_ce_pass;
 typedef enum ks_ce_reduction { KS_CE_NONE = 0, KS_CE_MEAN = 1, KS_CE_SUM = 2 } ks_ce_reduction;
-typedef struct ks_linear_ce_config { int tile_m; int64_t piece; } ks_linear_ce_config;
+typedef struct ks_linear_ce_config { int tile_m; int tile_n; int64_t piece; } ks_linear_ce_config;
 typedef struct ks_linear_ce_args {
   const void *h; const void *w; const int64_t *targets;
   int64_t tokens; int64_t dim; int64_t vocab; int64_t h_stride; int64_t w_stride;

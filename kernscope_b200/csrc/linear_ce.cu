@@ -6,7 +6,7 @@
 //   dh = d w;  dw = d^T h
 //
 // The logits [tokens, vocab] are never written.  Five GEMM-shaped passes share
-// one persistent kernel (TMA producer warp, one MMA-issuing thread, four
+// one persistent kernel (TMA producer warp, one MMA-issuing thread, eight
 // epilogue warps; tcgen05.mma kind::f16, fp32 accumulators in TMEM):
 //   STATS  l = h w^T; the epilogue reduces each tile's row to (max, sum of
 //          exponentials) and picks the target's logit out of the accumulator;
@@ -48,10 +48,11 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kBK = 64;                        // one 128-byte swizzle row of 16-bit values
 constexpr int kUmmaK = 16;
-constexpr int kThreads = 192;                  // producer, MMA, 4 x epilogue
+constexpr int kEpiWarps = 8;                    // two per TMEM lane quadrant, each with half of the columns
+constexpr int kThreads = 64 + kEpiWarps * 32;  // producer, MMA, epilogue
 constexpr uint32_t kABox = kBM * kBK * 2;      // 128 rows x 64 K (or two boxes of 64 K x 64 columns): 16 KB
 constexpr uint32_t kBBox = kBK * 64 * 2;       // 64 K-rows x 64 columns: 8 KB
-constexpr uint32_t kCBuf = 32 * 128;           // one epilogue block: 32 rows x 32 columns, up to 4 bytes each
+constexpr uint32_t kCStage = 32 * 128;         // an epilogue warp's staging: two 32 x 32 blocks of 16 bits, or one of 32
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kF16Range = 1024.f;            // factor on fp16 d
 constexpr float kF16Exp = 32768.f;             // factor on STORE's fp16 exponentials, which are at most 1
@@ -77,7 +78,7 @@ struct CeGemm {
   int64_t v0;             // first vocabulary column of the piece (PROB)
   const int64_t *targets;
   int64_t ignore;
-  float2 *part;           // [N-tiles][rows_p] (max, sum)
+  float2 *part;           // [half tiles][rows_p] (max, sum)
   float *tlogit;          // [rows_p]
   int64_t rows_p;
   const float *lse;
@@ -95,7 +96,7 @@ struct Layout {
   static constexpr uint32_t a_off = 0;
   static constexpr uint32_t b_off = a_off + STAGES * a_bytes;
   static constexpr uint32_t c_off = b_off + STAGES * b_bytes;
-  static constexpr uint32_t bar_off = c_off + 8 * kCBuf;  // 4 warps x 2 buffers
+  static constexpr uint32_t bar_off = c_off + kEpiWarps * kCStage;
   static constexpr uint32_t n_bars = 2 * STAGES + ACC + ACC * MH + 1;
   static constexpr uint32_t misc_off = bar_off + n_bars * 8;
   static constexpr uint32_t bytes = misc_off + 16;
@@ -155,22 +156,36 @@ KS_DEV float max32(const uint32_t (&r)[32]) {
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
 }
 
-// Maximum over this lane's row of one accumulator half, `left` columns of it
+// tcgen05.wait::ld that the loaded registers depend on, so that their uses
+// cannot move ahead of it.
+KS_DEV void wait_loaded(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+
+// Maximum over COLS columns of this lane's accumulator row, `left` of them
 // inside the vocabulary.
-template <int BN>
-KS_DEV float half_max(uint32_t t_addr, int64_t left) {
+template <int COLS>
+KS_DEV float cols_max(uint32_t t_addr, int64_t left) {
+  static_assert(COLS % 64 == 0, "pairs of blocks");
   float m = -INFINITY;
 #pragma unroll 1
-  for (int c = 0; c < BN; c += 32) {
-    uint32_t r[32];
-    ks_tmem_ld32(t_addr + c, r);
-    ks_tmem_wait_ld();
-    if (left - c < 32) {
+  for (int c = 0; c < COLS; c += 64) {
+    uint32_t r[2][32];
+    ks_tmem_ld32(t_addr + c, r[0]);
+    ks_tmem_ld32(t_addr + c + 32, r[1]);
+    wait_loaded(r[0]);
+    wait_loaded(r[1]);
+    if (left - c < 64) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (j >= left - c) r[j] = __float_as_uint(-INFINITY);
+      for (int j = 0; j < 64; ++j)
+        if (j >= left - c) r[j / 32][j % 32] = __float_as_uint(-INFINITY);
     }
-    m = fmaxf(m, max32(r));
+    m = fmaxf(m, fmaxf(max32(r[0]), max32(r[1])));
   }
   return m;
 }
@@ -203,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ks_mbar_init(empty + s, 1);
     }
     for (int a = 0; a < ACC; ++a) ks_mbar_init(tfull + a, 1);
-    for (int a = 0; a < ACC * MH; ++a) ks_mbar_init(tempty + a, 4);
+    for (int a = 0; a < ACC * MH; ++a) ks_mbar_init(tempty + a, kEpiWarps);
     ks_mbar_init(drain, 1);
     *abort = 0;
     ks_fence_mbar_init();
@@ -347,11 +362,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     ks_mbar_wait(drain, 0, nullptr, wait);
   } else if (warp >= 2) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;  // TMEM lane quadrant this warp may access
-    uint8_t *stg = smem + L::c_off + (warp - 2) * 2 * kCBuf;
+    constexpr int kCols = BN / 2;        // columns of a tile that one warp drains, of each 128-row half
+    constexpr int kBlocks = kCols / 32;  // 32-column blocks in them
+    const int q = warp & 3;              // TMEM lane quadrant this warp may access
+    const int cg = (warp - 2) / 4 * kCols;  // its first column
+    uint8_t *stg = smem + L::c_off + (warp - 2) * kCStage;
     const bool f16 = p.f16 != 0;
+    const bool wide = MODE == DH && p.out_f32;  // 32-bit blocks
     float escale = 1.f, fscale = 1.f;
-    if (MODE == DH || MODE == DW) escale = __ldcg(&p.sc->escale);
+    if (MODE == DH || MODE == DW) escale = wide ? 1.f : __ldcg(&p.sc->escale);
     if (MODE == PROB) fscale = __ldcg(&p.sc->fscale);
     int i = 0;
     uint32_t nstore = 0;
@@ -384,32 +403,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ks_mbar_wait(tfull + acc, acc_phase, abort, wait)) break;
       ks_tc_fence_after();
-      const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + acc * BN * MH;
-      const int64_t col0 = p.v0 + int64_t(tn) * BN;  // first vocabulary column of the tile (STATS, PROB)
+      const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + acc * BN * MH + cg;
+      const int64_t col0 = p.v0 + int64_t(tn) * BN;  // first vocabulary column of the tile (STATS, STORE, PROB)
       float m = -INFINITY, s = 0.f;
-#pragma unroll 1
-      for (int cc = 0; cc < MH * (BN / 32); ++cc) {
-        const int h = cc / (BN / 32);
-        const int cb = (cc % (BN / 32)) * 32;  // first column of the block inside the tile
-        if (MODE == STORE && cb == 0) m = half_max<BN>(t_addr + cc * 32, p.vocab - col0);
-        uint32_t r[32];
-        ks_tmem_ld32(t_addr + cc * 32, r);
-        ks_tmem_wait_ld();
-        if ((cc + 1) % (BN / 32) == 0) {  // this half is free for the next tile's MMAs
+      // block k: half k / kBlocks, columns cg + k % kBlocks * 32.  `next` is loaded while `r` is worked on.
+      auto step = [&](int k, uint32_t (&r)[32], uint32_t (&next)[32]) {
+        const int h = k / kBlocks, cb = cg + k % kBlocks * 32;
+        wait_loaded(r);
+        if (k + 1 < MH * kBlocks) ks_tmem_ld32(t_addr + (k + 1) / kBlocks * BN + (k + 1) % kBlocks * 32, next);
+        if ((MODE == STATS || MODE == STORE) && k % kBlocks == 0) {
+          s = 0.f;
+          m = MODE == STORE ? cols_max<kCols>(t_addr + h * BN, p.vocab - col0 - cg) : -INFINITY;
+        }
+        if ((k + 1) % kBlocks == 0) {  // this warp's part of the half is in registers
           ks_tc_fence_before();
           __syncwarp();
           if (lane == 0) ks_mbar_arrive(tempty + acc * MH + h);
         }
+        const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
+        const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cb;  // the target inside the block
+        const int64_t left = p.vocab - (col0 + cb);             // columns of the block inside the vocabulary
         if constexpr (MODE == STATS || MODE == STORE) {
-          const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cb;
           if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
             float v = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               if (j == tc) v = __uint_as_float(r[j]);
-            if (tc >= 0 && tc < 32) p.tlogit[int64_t(tm) * kTM + h * kBM + q * 32 + lane] = v;
+            if (tc >= 0 && tc < 32) p.tlogit[row] = v;
           }
-          const int64_t left = p.vocab - (col0 + cb);  // columns of the block inside the vocabulary
           if (left < 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
@@ -423,44 +444,50 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 32; ++j) {
             const float x = ex2(fmaf(__uint_as_float(r[j]), kLog2e, -base));
             a4[j & 3] += x;
-            if (MODE == STORE) r[j] = __float_as_uint(f16 ? x * kF16Exp : x);
+            if (MODE == STORE) r[j] = __float_as_uint(x);
           }
           if (MODE == STATS) s *= ex2(fmaf(m, kLog2e, -base));
           s += (a4[0] + a4[1]) + (a4[2] + a4[3]);
           m = mn;
-          if (cb + 32 == BN) {
-            const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
-            if (row < p.tokens) p.part[int64_t(tn) * p.rows_p + row] = make_float2(m, s);
-            m = -INFINITY;
-            s = 0.f;
+          if ((k + 1) % kBlocks == 0 && row < p.tokens)
+            p.part[(int64_t(tn) * 2 + cg / kCols) * p.rows_p + row] = make_float2(m, s);
+        }
+        if constexpr (MODE == STORE) {
+          if (f16) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * kF16Exp);
           }
+        } else if constexpr (MODE == PROB) {
+          const float fr = h == 0 ? f[0] : f[MH - 1];
+          const float l2 = h == 0 ? lse2[0] : lse2[MH - 1];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(fr * ex2(fmaf(__uint_as_float(r[j]), kLog2e, -l2)));
+          if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j == tc) r[j] = __float_as_uint(__uint_as_float(r[j]) - fr);
+          }
+          if (left < 32 || fr == 0.f) {  // columns past the vocabulary, rows without gradient: zeros, whatever the logits
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (j >= left || fr == 0.f) r[j] = 0u;
+          }
+        } else if constexpr (MODE == DH || MODE == DW) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
         }
         if constexpr (MODE != STATS) {
-          uint8_t *buf = stg + (nstore & 1) * kCBuf;
-          if (lane == 0) ks_bulk_wait_read<1>();  // the store two blocks back has read this buffer
-          __syncwarp();
-          if constexpr (MODE == PROB) {
-            const float fr = h == 0 ? f[0] : f[MH - 1];
-            const float l2 = h == 0 ? lse2[0] : lse2[MH - 1];
-            const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cb;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(fr * ex2(fmaf(__uint_as_float(r[j]), kLog2e, -l2)));
-            if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j == tc) r[j] = __float_as_uint(__uint_as_float(r[j]) - fr);
-            }
-            const int64_t left = p.vocab - (col0 + cb);
-            if (left < 32 || fr == 0.f) {  // columns past the vocabulary, rows without gradient: zeros, whatever the logits
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (j >= left || fr == 0.f) r[j] = 0u;
-            }
-          } else if (MODE == DW || !p.out_f32) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
+          const int c0 = tn * BN + cb;
+          const int64_t r0 = int64_t(tm) * kTM + h * kBM + q * 32;
+          if (c0 >= p.N || r0 >= p.M) return;  // blocks past the edge hold nothing
+          // the store that last used this buffer has read it
+          uint8_t *buf = stg + (wide ? 0 : (nstore & 1) * (kCStage / 2));
+          if (lane == 0) {
+            if (wide) ks_bulk_wait_read<0>();
+            else ks_bulk_wait_read<1>();
           }
-          if (MODE == DH && p.out_f32) {
+          __syncwarp();
+          if (wide) {
             // row = lane: eight 16-byte chunks, chunk v at position v ^ (lane & 7) (128-byte swizzle)
 #pragma unroll
             for (int v = 0; v < 8; ++v)
@@ -480,19 +507,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           ks_fence_proxy_async();
           __syncwarp();
-          const int c0 = tn * BN + cb;
-          const int64_t r0 = int64_t(tm) * kTM + h * kBM + q * 32;
-          if (c0 < p.N && r0 < p.M) {  // blocks past the edge hold nothing
-            if (lane == 0) {
-              if (MODE == DH && p.accumulate)
-                tma_reduce_add_2d(&tma_c, buf, c0, int(split * p.rows_p + r0));
-              else
-                ks_tma_store_2d(&tma_c, buf, c0, int((MODE == DH ? split * p.rows_p : 0) + r0));
-              ks_bulk_commit_group();
-            }
-            ++nstore;
+          if (lane == 0) {
+            if (MODE == DH && p.accumulate)
+              tma_reduce_add_2d(&tma_c, buf, c0, int(split * p.rows_p + r0));
+            else
+              ks_tma_store_2d(&tma_c, buf, c0, int((MODE == DH ? split * p.rows_p : 0) + r0));
+            ks_bulk_commit_group();
           }
+          ++nstore;
         }
+      };
+      uint32_t ra[32], rb[32];
+      ks_tmem_ld32(t_addr, ra);
+#pragma unroll 1
+      for (int k = 0; k < MH * kBlocks; k += 2) {
+        step(k, ra, rb);
+        step(k + 1, rb, ra);
       }
     }
     if (MODE != STATS && lane == 0) ks_bulk_wait_all();
@@ -846,17 +876,20 @@ int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 bool tma_ok(const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0; }
 
-// One GEMM's tile: 256 x 256 (one CTA, two M=128 MMAs per B tile) or 128 x 128.
+// One GEMM's tile: 256 x 256 (one CTA, two M=128 MMAs per B tile, one
+// accumulator drained by halves), 128 x 256 or 128 x 128 (two accumulators).
 struct Tile {
-  bool large;
-  int tm() const { return large ? 256 : 128; }
-  int64_t tiles(int64_t m, int64_t n) const { return ((m + tm() - 1) / tm()) * ((n + tm() - 1) / tm()); }
+  int tm, tn;
+  int64_t tiles(int64_t m, int64_t n) const { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
 };
 
-// Time of one K-block of one tile on one SM, microseconds, measured: the 256 x
-// 256 tile in a full 4096 x 2048 x 32768 dw product (0.72), the 128 x 128 tile,
-// which reads twice the operand bytes per product, in its dh product (0.29).
-constexpr double kLargeKb = 0.72, kSmallKb = 0.29;
+// What a tile costs, microseconds, measured: one K-block on one SM, and what a
+// tile's epilogue adds where the MMAs cannot run beside it.
+struct Cost {
+  Tile tile;
+  double kb, tail;
+};
+constexpr Cost kCosts[] = {{{256, 256}, 0.72, 1.5}, {{128, 256}, 0.40, 0.3}, {{128, 128}, 0.29, 0.3}};
 constexpr double kSlabBytesPerUs = 5e6;  // an fp32 slab is written once and read once
 
 struct Choice {
@@ -867,24 +900,23 @@ struct Choice {
 // Tile and K-splits with the least estimated time: rounds of tiles over the
 // SMs x K-blocks, plus the slabs' traffic where K is split (at least 8
 // K-blocks a split).  The large tile wins wherever it fills the SMs; the small
-// one, and splits, where it leaves them idle (512 x 1000 x 10007, dh: 8 large
-// tiles; split 17 ways 21 us, unsplit 113).
-Choice pick(int64_t m, int64_t n, int64_t kbs, bool may_split, int forced, int sms) {
+// ones, and splits, where it leaves them idle (333 x 1000 over 10007 columns,
+// dh: 8 large tiles; split 17 ways 21 us, unsplit 113).
+Choice pick(int64_t m, int64_t n, int64_t kbs, bool may_split, int tm, int tn, int sms) {
   Choice best = {};
   double least = 0;
-  for (int large = 1; large >= 0; --large) {
-    if (forced && forced != (large ? 256 : 128)) continue;
-    const Tile t{large != 0};
-    const int64_t tiles = t.tiles(m, n);
+  for (const Cost &c : kCosts) {
+    if ((tm && tm != c.tile.tm) || (tn && tn != c.tile.tn)) continue;
+    const int64_t tiles = c.tile.tiles(m, n);
     const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>(2 * sms / tiles, kbs / 8)) : 1;
     for (int64_t s = 1; s <= most; ++s) {
       const int64_t per = (kbs + s - 1) / s, used = (kbs + per - 1) / per;
       const double rounds = double((tiles * used + sms - 1) / sms);
-      double us = rounds * double(per) * (large ? kLargeKb : kSmallKb);
+      double us = rounds * (double(per) * c.kb + c.tail);
       if (used > 1) us += 4 + double(used) * double(m) * double(n) * 8 / kSlabBytesPerUs;
       if (best.splits == 0 || us < least) {
         least = us;
-        best = Choice{t, used, per};
+        best = Choice{c.tile, used, per};
       }
     }
   }
@@ -896,7 +928,7 @@ struct Plan {
   bool pack_h, pack_w, pad_dh, pad_dw;
   int64_t ld;            // row stride of packed h / w / padded outputs
   int64_t rows_p;        // tokens rounded up to 256
-  int64_t n_tiles;       // vocabulary tiles of STATS
+  int64_t n_tiles;       // vocabulary half tiles of STATS or STORE
   int64_t piece, pieces; // vocabulary columns per piece, pieces
   int splits, kb_split;  // K-splits of DH, K-blocks in each
   bool slabs;            // DH goes through fp32 slabs
@@ -907,8 +939,9 @@ struct Plan {
 };
 
 int check(const ks_linear_ce_config &c, const ks_linear_ce_args &a, char *reason, size_t len) {
-  if (c.tile_m != 0 && c.tile_m != 128 && c.tile_m != 256) {
-    ks::set_reason(reason, len, "linear_ce: tile_m must be 0 (chosen), 128 or 256");
+  if (!((c.tile_m == 0 && c.tile_n == 0) || (c.tile_m == 128 && (c.tile_n == 128 || c.tile_n == 256)) ||
+        (c.tile_m == 256 && c.tile_n == 256))) {
+    ks::set_reason(reason, len, "linear_ce: tile_m x tile_n must be 0 x 0 (chosen), 128 x 128, 128 x 256 or 256 x 256");
     return KS_ERR_INVALID_CONFIG;
   }
   if (c.piece < 0 || c.piece % 256 != 0) {
@@ -946,15 +979,16 @@ int check(const ks_linear_ce_config &c, const ks_linear_ce_args &a, char *reason
 void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t avail, Plan &p) {
   const int sms = ks::sm_count();
   const bool fwd = a.pass != KS_CE_BACKWARD, bwd = a.pass != KS_CE_FORWARD;
-  p.g1 = pick(a.tokens, a.vocab, (a.dim + kBK - 1) / kBK, false, c.tile_m, sms).tile;
-  p.gw = pick(a.vocab, a.dim, (a.tokens + kBK - 1) / kBK, false, c.tile_m, sms).tile;
+  p.g1 = pick(a.tokens, a.vocab, (a.dim + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
+  p.gw = pick(a.vocab, a.dim, (a.tokens + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
   p.pack_h = !tma_ok(a.h, a.h_stride);
   p.pack_w = !tma_ok(a.w, a.w_stride);
   p.pad_dh = bwd && !tma_ok(a.dh, a.dh_stride);
   p.pad_dw = bwd && !tma_ok(a.dw, a.dw_stride);
   p.ld = up(a.dim, 8);
   p.rows_p = up(a.tokens, 256);
-  p.n_tiles = up(a.vocab, 256) / p.g1.tm();  // of STORE, which runs over whole 256-column blocks
+  const int half = p.g1.tn / 2;               // columns that share a maximum
+  p.n_tiles = up(a.vocab, 256) / half;        // of STORE, which runs over whole 256-column blocks
   size_t o = 0;
   auto take = [&](size_t bytes) {
     const size_t at = o;
@@ -979,7 +1013,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
       o = from;
       p.piece = piece;
       p.pieces = (a.vocab + piece - 1) / piece;
-      const Choice h = pick(a.tokens, a.dim, (std::min(piece, a.vocab) + kBK - 1) / kBK, true, c.tile_m, sms);
+      const Choice h = pick(a.tokens, a.dim, (std::min(piece, a.vocab) + kBK - 1) / kBK, true, c.tile_m, c.tile_n, sms);
       p.gh = h.tile;
       p.splits = int(h.splits);
       p.kb_split = int(h.kb_split);
@@ -1006,7 +1040,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   } else {
     p.fixed = p.bytes = o;
   }
-  if (!p.store) p.n_tiles = (a.vocab + p.g1.tm() - 1) / p.g1.tm();
+  if (!p.store) p.n_tiles = up(a.vocab, p.g1.tn) / half;
 }
 
 template <int MODE, int BN, int STAGES, int ACC, int MH>
@@ -1026,8 +1060,9 @@ int launch(bool next, const CUtensorMap &ta, const CUtensorMap &tb, const CUtens
 template <int MODE>
 int launch_tile(bool next, Tile t, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g,
                 cudaStream_t st) {
-  return t.large ? launch<MODE, 256, 3, 1, 2>(next, ta, tb, tc, g, st)
-                 : launch<MODE, 128, 5, 2, 1>(next, ta, tb, tc, g, st);
+  if (t.tm == 256) return launch<MODE, 256, 3, 1, 2>(next, ta, tb, tc, g, st);
+  return t.tn == 256 ? launch<MODE, 256, 4, 2, 1>(next, ta, tb, tc, g, st)
+                     : launch<MODE, 128, 5, 2, 1>(next, ta, tb, tc, g, st);
 }
 
 CUtensorMapDataType tm_type(int dtype) {
@@ -1100,12 +1135,11 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   g.splits = g.release = 1;
   const int64_t kd = (a.dim + kBK - 1) / kBK;
   CUtensorMap th, tw;
-  const int t1 = p.g1.tm();
-  if ((s = map_k(&th, a.dtype, h, a.tokens, a.dim, hs, t1)) != KS_OK) return s;
+  if ((s = map_k(&th, a.dtype, h, a.tokens, a.dim, hs, p.g1.tm)) != KS_OK) return s;
   float *lse = a.lse;
   if (fwd) {
     if (!lse) lse = reinterpret_cast<float *>(ws + p.o_lse);
-    if ((s = map_k(&tw, a.dtype, w, a.vocab, a.dim, wst, t1)) != KS_OK) return s;
+    if ((s = map_k(&tw, a.dtype, w, a.vocab, a.dim, wst, p.g1.tn)) != KS_OK) return s;
     g.M = int(a.tokens);
     g.N = int(a.vocab);
     g.kb_total = g.kb_split = int(kd);
@@ -1153,18 +1187,17 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
       const unsigned rows8 = unsigned((a.tokens + 7) / 8);
       const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, 65535));
       s = ks::launch_kernel(true, ce_scale_kernel, dim3(rows8, cols), dim3(256), 0, st, reinterpret_cast<uint16_t *>(d), vpad, g.part,
-                          p.rows_p, t1 == 256 ? 8 : 7, lse, g.tlogit, a.targets, a.tokens, a.vocab, a.ignore_index, sc,
+                          p.rows_p, p.g1.tn == 256 ? 7 : 6, lse, g.tlogit, a.targets, a.tokens, a.vocab, a.ignore_index, sc,
                           g.f16);
     } else {
-      if ((s = map_k(&tw, a.dtype, wp, vp, a.dim, wst, t1)) != KS_OK) return s;
+      if ((s = map_k(&tw, a.dtype, wp, vp, a.dim, wst, p.g1.tn)) != KS_OK) return s;
       if ((s = map_out(&tc, a.dtype, d, a.tokens, vpad, vpad)) != KS_OK) return s;
       s = launch_tile<PROB>(true, p.g1, th, tw, tc, g, st);
     }
     if (s != KS_OK) return s;
     // dh (+)= d w
-    const int th_ = p.gh.tm();
-    if ((s = map_k(&ta, a.dtype, d, a.tokens, vp, vpad, th_)) != KS_OK) return s;
-    if ((s = map_mn(&tb, a.dtype, wp, vp, a.dim, wst, th_, &g.b3d)) != KS_OK) return s;
+    if ((s = map_k(&ta, a.dtype, d, a.tokens, vp, vpad, p.gh.tm)) != KS_OK) return s;
+    if ((s = map_mn(&tb, a.dtype, wp, vp, a.dim, wst, p.gh.tn, &g.b3d)) != KS_OK) return s;
     const bool slabbed = p.slabs;
     if (slabbed)
       s = ks::encode_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, slabs, uint64_t(p.slab_ld),
@@ -1181,11 +1214,10 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.accumulate = slabbed && i > 0;
     if ((s = launch_tile<DH>(true, p.gh, ta, tb, tc, g, st)) != KS_OK) return s;
     // rows v0.. of dw = d^T h
-    const int tw_ = p.gw.tm();
     int a3d = 0;
-    if ((s = map_mn(&ta, a.dtype, d, a.tokens, vpad, vpad, tw_, &a3d)) != KS_OK) return s;
+    if ((s = map_mn(&ta, a.dtype, d, a.tokens, vpad, vpad, p.gw.tm, &a3d)) != KS_OK) return s;
     if (!a3d) return KS_ERR_OTHER;
-    if ((s = map_mn(&tb, a.dtype, h, a.tokens, a.dim, hs, tw_, &g.b3d)) != KS_OK) return s;
+    if ((s = map_mn(&tb, a.dtype, h, a.tokens, a.dim, hs, p.gw.tn, &g.b3d)) != KS_OK) return s;
     char *dwp = static_cast<char *>(a.dw) + v0 * a.dw_stride * 2;
     if ((s = map_out(&tc, a.dtype, p.pad_dw ? ws + p.o_dw : dwp, vp, a.dim, p.pad_dw ? p.ld : a.dw_stride)) != KS_OK)
       return s;

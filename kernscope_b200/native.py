@@ -97,7 +97,7 @@ class FlashAttentionArgs(C.Structure):
 
 
 class LinearCeConfig(C.Structure):
-    _fields_ = [("tile_m", C.c_int), ("piece", C.c_int64)]
+    _fields_ = [("tile_m", C.c_int), ("tile_n", C.c_int), ("piece", C.c_int64)]
 
 
 class LinearCeArgs(C.Structure):

@@ -43,6 +43,11 @@ def _dt(torch, name):
     return {"bf16": torch.bfloat16, "fp16": torch.float16}[name]
 
 
+def _cfg(N, tile, piece=0):
+    tile_m, tile_n = tile if isinstance(tile, tuple) else (tile, tile)
+    return N.LinearCeConfig(tile_m, tile_n, piece)
+
+
 def _make(torch, n, dim, vocab, dtype, seed=0, h_pad=0, w_pad=0, lean=6.0):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -105,14 +110,14 @@ SHAPES = [  # tokens, dim, vocab: one of each, tile edges, odd, long rows, more 
 ]
 
 
-@pytest.mark.parametrize("tile", [0, 128, 256])
+@pytest.mark.parametrize("tile", [0, 128, (128, 256), 256])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
 def test_loss_and_gradients(ks, shape, dtype, tile):
     N, ops, torch = ks
     n, dim, vocab = shape
     h, w, t = _make(torch, n, dim, vocab, _dt(torch, dtype), seed=n + dim + vocab)
-    cfg = N.LinearCeConfig(tile, 0)
+    cfg = _cfg(N, tile)
     count = max(1, int((t != IGNORE).sum()))
     ref = _exact(torch, h, w, t, torch.full((n,), 1.0 / count, device="cuda"))
     loss, lse = ops.linear_cross_entropy(h, w, t, cfg=cfg)
@@ -127,7 +132,7 @@ def test_loss_and_gradients(ks, shape, dtype, tile):
     assert ops.device_error_take() == 0
 
 
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [128, (128, 256), 256])
 @pytest.mark.parametrize("h_pad,w_pad", [(0, 0), (8, 16), (3, 0), (0, 5), (1, 1)])
 def test_strides_and_output_rows(ks, h_pad, w_pad, tile):
     """Row strides of inputs and outputs, those TMA cannot address among them;
@@ -138,7 +143,7 @@ def test_strides_and_output_rows(ks, h_pad, w_pad, tile):
     dh_all = torch.full((n, dim + h_pad), 7.0, dtype=torch.bfloat16, device="cuda")
     dw_all = torch.full((vocab, dim + w_pad), 7.0, dtype=torch.bfloat16, device="cuda")
     ref = _exact(torch, h, w, t, torch.ones(n, device="cuda"))
-    cfg = N.LinearCeConfig(tile, 256)  # three pieces
+    cfg = _cfg(N, tile, 256)  # three pieces
     loss, dh, dw = ops.linear_cross_entropy_grad(h, w, t, reduction="sum", dh=dh_all[:, :dim], dw=dw_all[:, :dim], cfg=cfg)
     _near(torch, dh, ref["dh"], ref["dh_tol"], "dh")
     _near(torch, dw, ref["dw"], ref["dw_tol"], "dw")
@@ -183,7 +188,7 @@ def test_backward_with_incoming_gradient(ks, reduction, dtype, piece):
         dloss = torch.full((1,), 3.0, device="cuda")
         f = torch.full((n,), 1.5, device="cuda") / (int((t != IGNORE).sum()) if reduction == "mean" else 1)
     ref = _exact(torch, h, w, t, f)
-    cfg = N.LinearCeConfig(0, piece)
+    cfg = _cfg(N, 0, piece)
     dh, dw = ops.linear_cross_entropy_backward(h, w, t, lse, dloss, reduction=reduction, grad_scale=0.5, cfg=cfg)
     _near(torch, dh, ref["dh"], ref["dh_tol"], "dh")
     _near(torch, dw, ref["dw"], ref["dw_tol"], "dw")
@@ -207,14 +212,14 @@ def test_large_and_small_incoming_gradients_keep_fp16_range(ks):
         assert torch.equal(dw.double(), base)  # powers of two change no rounding
 
 
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [128, (128, 256), 256])
 def test_workspace_least_and_dirty(ks, tile):
     """The least workspace, full of NaN: the same loss, and gradients within the
     bounds (more pieces, another order of the sum)."""
     N, ops, torch = ks
     n, dim, vocab = 333, 160, 3000
     h, w, t = _make(torch, n, dim, vocab, torch.bfloat16, seed=21)
-    cfg = N.LinearCeConfig(tile, 0)
+    cfg = _cfg(N, tile)
     a = ops._linear_ce_args(h, w, t, N.KS_CE_GRAD, "sum", IGNORE)
     least, want = ops.linear_cross_entropy_workspace_bytes(a, cfg)
     assert least < want
@@ -231,7 +236,7 @@ def test_workspace_least_and_dirty(ks, tile):
     assert e.value.status == N.KS_ERR_WORKSPACE
 
 
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [128, (128, 256), 256])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_loss_of_one_large_logit(ks, dtype, tile):
     """Logits of a few hundred, targets with probability near one: the loss is a
@@ -240,7 +245,7 @@ def test_loss_of_one_large_logit(ks, dtype, tile):
     N, ops, torch = ks
     n, dim, vocab = 64, 2048, 1000
     h, w, t = _make(torch, n, dim, vocab, _dt(torch, dtype), seed=31, lean=300.0)
-    loss, lse = ops.linear_cross_entropy(h, w, t, cfg=N.LinearCeConfig(tile, 0))
+    loss, lse = ops.linear_cross_entropy(h, w, t, cfg=_cfg(N, tile))
     ref = _exact(torch, h, w, t)
     _near(torch, lse, ref["lse"], ref["lse_tol"], "lse")
     valid = ref["valid"]
@@ -382,10 +387,10 @@ def test_refusals(ks):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(N.KsError) as e:
-        ops.linear_cross_entropy(h, w, t, cfg=N.LinearCeConfig(64, 0))
+        ops.linear_cross_entropy(h, w, t, cfg=N.LinearCeConfig(256, 128, 0))
     assert e.value.status == N.KS_ERR_INVALID_CONFIG
     with pytest.raises(N.KsError) as e:
-        ops.linear_cross_entropy_grad(h, w, t, cfg=N.LinearCeConfig(0, 100))
+        ops.linear_cross_entropy_grad(h, w, t, cfg=_cfg(N, 0, 100))
     assert e.value.status == N.KS_ERR_INVALID_CONFIG
     a = ops._linear_ce_args(h, w, t, N.KS_CE_FORWARD, "none", IGNORE)
     cfg = N.LinearCeConfig()
