@@ -412,31 +412,32 @@ struct Sum {
 
 constexpr int64_t kGroup = 64;  // chunks whose partials one CTA adds up
 
-// A token that lies in chunks a to b, of which this CTA (chunk ch, segment seg)
-// has just left a partial sum.  The last of the CTAs that hold a part of it,
-// within each group of 64 chunks, adds the group's partials in order; the last
-// group adds the groups'.  So the order of the sum is that of the chunks,
-// whoever comes last, and a token that fills the whole batch is joined in two
-// short chains.  (A kernel of its own for the joins cost 4 us more at 777 x 1001
-// and 12 at 131072 x 1024.)
+// A token that lies in chunks a to b, of which this CTA has left a partial sum.
+// The last of the CTAs that hold a part of it, within each group of 64 chunks,
+// adds the group's partials in order; the last group adds the groups'.  So the
+// order of the sum is that of the chunks, whoever comes last, and a token that
+// fills the whole batch is joined in two short chains.  (A kernel of its own
+// for the joins cost 4 us more at 777 x 1001 and 12 at 131072 x 1024.)
+struct Part {
+  uint32_t key;
+  int64_t a, b;
+};
+
+// What a CTA (chunk ch, segment seg) waits for in `arrived`, and whether it is last.
+template <int DT, int ODT>
+KS_DEV bool arrive_group(const GradArgs<DT, ODT> &g, const Part &t, int64_t ch, int64_t seg) {
+  const int64_t first = max(t.a, ch / kGroup * kGroup), last = min(t.b, ch / kGroup * kGroup + kGroup - 1);
+  uint32_t *counter = g.arrived + (first * 2 + (first == t.a ? 1 : 0)) * g.segs + seg;
+  return int64_t(atomicAdd(counter, 1u)) == last - first;
+}
+
 template <int DT, int ODT, bool VEC>
-KS_DEV void join(const GradArgs<DT, ODT> &g, uint32_t key, int64_t ch, int64_t seg, int64_t a, int64_t b) {
+KS_DEV void join(const GradArgs<DT, ODT> &g, const Part &t, int64_t ch, int64_t seg) {
   using S = Sum<DT, ODT, VEC>;
-  __shared__ bool last_one;
-  const int64_t c = seg * S::cols(), segs = g.segs;
+  __shared__ bool last_group;
+  const int64_t c = seg * S::cols(), a = t.a, b = t.b;
   auto slot = [&](int64_t chunk) { return g.part + (chunk * 2 + (chunk == a ? 1 : 0)) * g.ld; };
-  auto last_of = [&](uint32_t *counter, int64_t expected) {
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) last_one = int64_t(atomicAdd(counter, 1u)) == expected - 1;
-    __syncthreads();
-    const bool l = last_one;
-    __threadfence();
-    __syncthreads();  // last_one may be written again
-    return l;
-  };
   const int64_t first = max(a, ch / kGroup * kGroup), last = min(b, ch / kGroup * kGroup + kGroup - 1);
-  if (!last_of(g.arrived + (first * 2 + (first == a ? 1 : 0)) * segs + seg, last - first + 1)) return;
   S sum;
   sum.clear();
 #pragma unroll 4
@@ -444,12 +445,18 @@ KS_DEV void join(const GradArgs<DT, ODT> &g, uint32_t key, int64_t ch, int64_t s
   const int64_t ga = a / kGroup, gb = b / kGroup;
   if (ga != gb) {
     sum.put_part(slot(first), c, g.dim);
-    if (!last_of(g.arrived + g.chunks * 2 * segs + a * segs + seg, gb - ga + 1)) return;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0)
+      last_group = int64_t(atomicAdd(g.arrived + g.chunks * 2 * g.segs + a * g.segs + seg, 1u)) == gb - ga;
+    __syncthreads();
+    if (!last_group) return;
+    __threadfence();
     sum.clear();
 #pragma unroll 4
     for (int64_t j = ga; j <= gb; ++j) sum.add_part(slot(max(a, j * kGroup)), c, g.dim);
   }
-  sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, g.scale, g.accumulate != 0);
+  sum.finish(g.dtable + int64_t(t.key) * g.dtable_stride, c, g.dim, g.scale, g.accumulate != 0);
 }
 
 template <int DT, int ODT, bool VEC>
@@ -577,8 +584,19 @@ __global__ void __launch_bounds__(kSegThreads)
       fill(st + kStages);
     }
   }
-  if (head != none) join<DT, ODT, VEC>(g, head, ch, seg, first_chunk, head_goes_on ? last_chunk : ch);
-  if (tail != none) join<DT, ODT, VEC>(g, tail, ch, seg, ch, last_chunk);
+  if (head == none && tail == none) return;
+  // both arrivals at once: a fence and an atomic take about a microsecond each
+  __shared__ bool last[2];
+  const Part h{head, first_chunk, head_goes_on ? last_chunk : ch}, t{tail, ch, last_chunk};
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last[0] = head != none && arrive_group(g, h, ch, seg);
+  if (tid == blockDim.x - 1) last[1] = tail != none && arrive_group(g, t, ch, seg);
+  __syncthreads();
+  const bool join_head = last[0], join_tail = last[1];
+  __threadfence();
+  if (join_head) join<DT, ODT, VEC>(g, h, ch, seg);
+  if (join_tail) join<DT, ODT, VEC>(g, t, ch, seg);
 }
 
 // ---------------------------------------------------------------------------
@@ -656,7 +674,7 @@ GradPlan grad_plan(const ks_embedding_grad_config &c, const ks_embedding_grad_ar
     const int64_t per_sm = std::min<int64_t>({int64_t(227 * 1024 / (p.shm + 9 * 1024 + 512)), 1024 / p.threads, 16});
     int64_t even = (n * p.segs + per_sm * ks::sm_count() - 1) / (per_sm * ks::sm_count());
     if (even >= 256) even = (even + 1) / 2;
-    p.chunk = c.chunk ? c.chunk : int(std::min<int64_t>(kMaxChunk, (even + kRows - 1) / kRows * kRows));
+    p.chunk = c.chunk ? c.chunk : int(std::min<int64_t>(kMaxChunk, std::max<int64_t>(even, kRows)));
     p.chunks = (n + p.chunk - 1) / p.chunk;
     p.counters = p.chunks * 3 * p.segs;
     most_chunks = std::max(most_chunks, p.chunks);

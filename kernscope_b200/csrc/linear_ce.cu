@@ -52,7 +52,7 @@ constexpr int kEpiWarps = 8;                    // two per TMEM lane quadrant, e
 constexpr int kThreads = 64 + kEpiWarps * 32;  // producer, MMA, epilogue
 constexpr uint32_t kABox = kBM * kBK * 2;      // 128 rows x 64 K (or two boxes of 64 K x 64 columns): 16 KB
 constexpr uint32_t kBBox = kBK * 64 * 2;       // 64 K-rows x 64 columns: 8 KB
-constexpr uint32_t kCStage = 32 * 128;         // an epilogue warp's staging: two 32 x 32 blocks of 16 bits, or one of 32
+constexpr uint32_t kCStage = 32 * 128;         // an epilogue warp's staging: 32 rows x 64 columns of 16 bits, or x 32 of 32
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kF16Range = 1024.f;            // factor on fp16 d
 constexpr float kF16Exp = 32768.f;             // factor on STORE's fp16 exponentials, which are at most 1
@@ -79,7 +79,10 @@ struct CeGemm {
   const int64_t *targets;
   int64_t ignore;
   float2 *part;           // [half tiles][rows_p] (max, sum)
-  float *tlogit;          // [rows_p]
+  float *tlogit;          // [rows_p] the target's logit, from the accumulator
+  const uint16_t *h, *w;  // for the target's dot product
+  int64_t h_stride, w_stride, dim;
+  float *tdot;            // [rows_p] that dot product
   int64_t rows_p;
   const float *lse;
   const float *dloss;     // per token, or nullptr
@@ -188,6 +191,36 @@ KS_DEV float cols_max(uint32_t t_addr, int64_t left) {
     m = fmaxf(m, fmaxf(max32(r[0]), max32(r[1])));
   }
   return m;
+}
+
+// <h[row], w[t]> in fp32 by one warp.
+KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool f16, int lane) {
+  auto val = [&](uint32_t v, int hi) {
+    if (f16) {
+      const __half2 x = *reinterpret_cast<const __half2 *>(&v);
+      return hi ? __high2float(x) : __low2float(x);
+    }
+    return hi ? ks_bf16_hi(v) : ks_bf16_lo(v);
+  };
+  float a0 = 0.f, a1 = 0.f;
+  int64_t k = 0;
+  if (((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15) == 0) {
+#pragma unroll 4
+    for (int64_t at = lane * 8; at + 8 <= dim; at += 256) {
+      const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(h + at)), y = __ldcg(reinterpret_cast<const uint4 *>(w + at));
+      a0 = fmaf(val(x.x, 0), val(y.x, 0), a0);
+      a1 = fmaf(val(x.x, 1), val(y.x, 1), a1);
+      a0 = fmaf(val(x.y, 0), val(y.y, 0), a0);
+      a1 = fmaf(val(x.y, 1), val(y.y, 1), a1);
+      a0 = fmaf(val(x.z, 0), val(y.z, 0), a0);
+      a1 = fmaf(val(x.z, 1), val(y.z, 1), a1);
+      a0 = fmaf(val(x.w, 0), val(y.w, 0), a0);
+      a1 = fmaf(val(x.w, 1), val(y.w, 1), a1);
+    }
+    k = dim / 8 * 8;
+  }
+  for (k += lane; k < dim; k += 32) a0 = fmaf(val(__ldcg(h + k), 0), val(__ldcg(w + k), 0), a0);
+  return ks_warp_sum(a0 + a1);
 }
 
 template <int MODE, int BN, int STAGES, int ACC, int MH>
@@ -372,8 +405,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     float escale = 1.f, fscale = 1.f;
     if (MODE == DH || MODE == DW) escale = wide ? 1.f : __ldcg(&p.sc->escale);
     if (MODE == PROB) fscale = __ldcg(&p.sc->fscale);
+    if (MODE == STATS || MODE == STORE) {
+      // these warps have nothing else to do until the first tile is complete
+      for (int64_t row = int64_t(blockIdx.x) * kEpiWarps + warp - 2; row < p.tokens; row += int64_t(gridDim.x) * kEpiWarps) {
+        const int64_t t = p.targets[row];
+        if (t == p.ignore || t < 0 || t >= p.vocab) continue;
+        const float v = target_dot(p.h + row * p.h_stride, p.w + t * p.w_stride, p.dim, f16, lane);
+        if (lane == 0) p.tdot[row] = v;
+      }
+    }
     int i = 0;
-    uint32_t nstore = 0;
     for (int t = blockIdx.x; t < num_work; t += gridDim.x, ++i) {
       const int acc = i % ACC;
       const uint32_t acc_phase = (i / ACC) & 1;
@@ -477,24 +518,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
         }
         if constexpr (MODE != STATS) {
-          const int c0 = tn * BN + cb;
+          // 16 bits: two blocks side by side fill the staging's 128-byte rows, the
+          // second one stores both.  (32-column stores, 64 bytes a row, wrote dw of
+          // 16 tokens x 1024 x 32000 at 3 TB/s.)
+          const bool second = !wide && (k & 1);
+          const int c0 = tn * BN + cb - (second ? 32 : 0);
           const int64_t r0 = int64_t(tm) * kTM + h * kBM + q * 32;
           if (c0 >= p.N || r0 >= p.M) return;  // blocks past the edge hold nothing
-          // the store that last used this buffer has read it
-          uint8_t *buf = stg + (wide ? 0 : (nstore & 1) * (kCStage / 2));
-          if (lane == 0) {
-            if (wide) ks_bulk_wait_read<0>();
-            else ks_bulk_wait_read<1>();
+          if (!second) {
+            if (lane == 0) ks_bulk_wait_read<0>();  // the last store has read the staging
+            __syncwarp();
           }
-          __syncwarp();
+          // row = lane, 128-byte swizzle: 16-byte chunk v at position v ^ (lane & 7)
+          uint8_t *line = stg + lane * 128;
           if (wide) {
-            // row = lane: eight 16-byte chunks, chunk v at position v ^ (lane & 7) (128-byte swizzle)
 #pragma unroll
             for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<uint4 *>(buf + lane * 128 + ((v ^ (lane & 7)) * 16)) =
+              *reinterpret_cast<uint4 *>(line + ((v ^ (lane & 7)) * 16)) =
                   make_uint4(r[v * 4], r[v * 4 + 1], r[v * 4 + 2], r[v * 4 + 3]);
           } else {
-            // row = lane: four 16-byte chunks, chunk v at position v ^ ((lane >> 1) & 3) (64-byte swizzle)
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               uint4 w;
@@ -502,19 +544,19 @@ __global__ void __launch_bounds__(kThreads, 1)
               w.y = pack2(__uint_as_float(r[v * 8 + 2]), __uint_as_float(r[v * 8 + 3]), f16);
               w.z = pack2(__uint_as_float(r[v * 8 + 4]), __uint_as_float(r[v * 8 + 5]), f16);
               w.w = pack2(__uint_as_float(r[v * 8 + 6]), __uint_as_float(r[v * 8 + 7]), f16);
-              *reinterpret_cast<uint4 *>(buf + lane * 64 + ((v ^ ((lane >> 1) & 3)) * 16)) = w;
+              *reinterpret_cast<uint4 *>(line + (((v + (second ? 4 : 0)) ^ (lane & 7)) * 16)) = w;
             }
+            if (!second) return;
           }
           ks_fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
             if (MODE == DH && p.accumulate)
-              tma_reduce_add_2d(&tma_c, buf, c0, int(split * p.rows_p + r0));
+              tma_reduce_add_2d(&tma_c, stg, c0, int(split * p.rows_p + r0));
             else
-              ks_tma_store_2d(&tma_c, buf, c0, int((MODE == DH ? split * p.rows_p : 0) + r0));
+              ks_tma_store_2d(&tma_c, stg, c0, int((MODE == DH ? split * p.rows_p : 0) + r0));
             ks_bulk_commit_group();
           }
-          ++nstore;
         }
       };
       uint32_t ra[32], rb[32];
@@ -543,44 +585,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kCombRows = 8;
 
-// <h[row], w[t]> in fp32 by one warp.
-KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool f16, int lane) {
-  auto val = [&](uint32_t v, int hi) {
-    if (f16) {
-      const __half2 x = *reinterpret_cast<const __half2 *>(&v);
-      return hi ? __high2float(x) : __low2float(x);
-    }
-    return hi ? ks_bf16_hi(v) : ks_bf16_lo(v);
-  };
-  float a0 = 0.f, a1 = 0.f;
-  int64_t k = 0;
-  if (((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w)) & 15) == 0) {
-#pragma unroll 4
-    for (int64_t at = lane * 8; at + 8 <= dim; at += 256) {
-      const uint4 x = __ldcg(reinterpret_cast<const uint4 *>(h + at)), y = __ldcg(reinterpret_cast<const uint4 *>(w + at));
-      a0 = fmaf(val(x.x, 0), val(y.x, 0), a0);
-      a1 = fmaf(val(x.x, 1), val(y.x, 1), a1);
-      a0 = fmaf(val(x.y, 0), val(y.y, 0), a0);
-      a1 = fmaf(val(x.y, 1), val(y.y, 1), a1);
-      a0 = fmaf(val(x.z, 0), val(y.z, 0), a0);
-      a1 = fmaf(val(x.z, 1), val(y.z, 1), a1);
-      a0 = fmaf(val(x.w, 0), val(y.w, 0), a0);
-      a1 = fmaf(val(x.w, 1), val(y.w, 1), a1);
-    }
-    k = dim / 8 * 8;
-  }
-  for (k += lane; k < dim; k += 32) a0 = fmaf(val(__ldcg(h + k), 0), val(__ldcg(w + k), 0), a0);
-  return ks_warp_sum(a0 + a1);
-}
-
 __global__ void __launch_bounds__(256)
-    ce_combine_kernel(const float2 *__restrict__ part, int tiles, int64_t rows_p, const uint16_t *__restrict__ h,
-                      int64_t h_stride, const uint16_t *__restrict__ w, int64_t w_stride, int64_t dim, int f16,
-                      float *__restrict__ tlogit,
+    ce_combine_kernel(const float2 *__restrict__ part, int tiles, int64_t rows_p, const float *__restrict__ tlogit,
+                      const float *__restrict__ tdot,
                       const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab, int64_t ignore, int reduction,
                       float grad_scale, const float *dloss, float range, float *__restrict__ loss,
                       float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc, int release) {
-  __shared__ float sm[8][kCombRows], ss[8][kCombRows], dot[kCombRows];
+  __shared__ float sm[8][kCombRows], ss[8][kCombRows];
   __shared__ double shl[kCombRows], shn[kCombRows];
   __shared__ bool is_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -588,6 +599,14 @@ __global__ void __launch_bounds__(256)
   ks_pdl_wait();
   const int rr = tid & (kCombRows - 1), slice = tid / kCombRows;
   const int64_t row = int64_t(blockIdx.x) * kCombRows + rr;
+  // the row's own values, loaded beside the partial sums
+  int64_t t = ignore;
+  float lt = 0.f, old = 0.f;
+  if (tid < kCombRows && row < tokens) {
+    t = targets[row];
+    lt = __ldcg(tdot + row);
+    old = __ldcg(tlogit + row);
+  }
   float m = -INFINITY, s = 0.f;
   auto add = [&](float m2, float s2) {  // (m, s) (+) (m2, s2); a side with no finite maximum adds its sum as it is
     const float mn = fmaxf(m, m2);
@@ -599,19 +618,11 @@ __global__ void __launch_bounds__(256)
     m = mn;
   };
   if (row < tokens)
+#pragma unroll 4
     for (int t = slice; t < tiles; t += 256 / kCombRows) {
       const float2 v = __ldcg(part + int64_t(t) * rows_p + row);
       add(v.x, v.y);
     }
-  {
-    static_assert(kCombRows == 8, "one warp per row");
-    const int64_t r = int64_t(blockIdx.x) * kCombRows + warp;
-    const int64_t t = r < tokens ? targets[r] : -1;
-    if (t != ignore && t >= 0 && t < vocab) {
-      const float v = target_dot(h + r * h_stride, w + t * w_stride, dim, f16 != 0, lane);
-      if (lane == 0) dot[warp] = v;
-    }
-  }
 #pragma unroll
   for (int o = kCombRows; o < 32; o <<= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
@@ -629,15 +640,9 @@ __global__ void __launch_bounds__(256)
     for (int w = 1; w < 8; ++w) add(sm[w][tid], ss[w][tid]);
     double l = 0.0, n = 0.0;
     if (row < tokens) {
-      const int64_t t = targets[row];
       const bool valid = t != ignore && t >= 0 && t < vocab;
-      float lt = 0.f;
-      if (valid) {  // the target's logit as the dot product, in the sum too
-        lt = dot[tid];
-        const float old = __ldcg(tlogit + row);
-        if (isfinite(lt) && isfinite(old)) s += ex2((lt - m) * kLog2e) - ex2((old - m) * kLog2e);
-        tlogit[row] = lt;
-      }
+      // the target's logit as the dot product, in the sum too
+      if (valid && isfinite(lt) && isfinite(old)) s += ex2((lt - m) * kLog2e) - ex2((old - m) * kLog2e);
       const float lse = m + logf(s);  // -inf + log 0: a row of -inf logits
       lse_out[row] = lse;
       float v = 0.f;
@@ -661,7 +666,7 @@ __global__ void __launch_bounds__(256)
     }
     sums[blockIdx.x] = make_double2(l, n);
     __threadfence();
-    is_last = atomicAdd(&sc->counter, 1u) == gridDim.x - 1;
+    is_last = gridDim.x == 1 || atomicAdd(&sc->counter, 1u) == gridDim.x - 1;
   }
   __syncthreads();
   if (!is_last) return;
@@ -699,7 +704,7 @@ __global__ void __launch_bounds__(256)
 // 32-byte sectors.  Reads and writes 2 bytes a value.
 __global__ void __launch_bounds__(256)
     ce_scale_kernel(uint16_t *__restrict__ d, int64_t ld, const float2 *__restrict__ part, int64_t rows_p, int tile_log2,
-                    const float *__restrict__ lse, const float *__restrict__ tlogit, const int64_t *__restrict__ targets,
+                    const float *__restrict__ lse, const float *__restrict__ tdot, const int64_t *__restrict__ targets,
                     int64_t tokens, int64_t vocab, int64_t ignore, const CeScalars *__restrict__ sc, int f16) {
   const int lane = threadIdx.x & 31;
   const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(256)
   const float f = valid ? __ldcg(&sc->fscale) : 0.f, fe = f16 ? f / kF16Exp : f;
   const float l2 = __ldcg(lse + row) * kLog2e;
   uint16_t *dr = d + row * ld;
-  const float dt = valid ? f * ex2(fmaf(__ldcg(tlogit + row), kLog2e, -l2)) - f : 0.f;
+  const float dt = valid ? f * ex2(fmaf(__ldcg(tdot + row), kLog2e, -l2)) - f : 0.f;
   constexpr int step = 256;
   for (int64_t c0 = int64_t(blockIdx.y) * (4 * step) + lane * 8; c0 < ld; c0 += int64_t(gridDim.y) * (4 * step)) {
     uint4 v[4];
@@ -825,6 +830,7 @@ __global__ void __launch_bounds__(256)
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += int64_t(gridDim.x) * 256) {
     const int64_t r = i / cv, c = (i - r * cv) * 4;
     float4 a = __ldcg(reinterpret_cast<const float4 *>(slabs + r * ld + c));
+#pragma unroll 8
     for (int k = 1; k < count; ++k) {
       const float4 b = __ldcg(reinterpret_cast<const float4 *>(slabs + k * slab_elems + r * ld + c));
       a.x += b.x;
@@ -884,12 +890,16 @@ struct Tile {
 };
 
 // What a tile costs, microseconds, measured: one K-block on one SM, and what a
-// tile's epilogue adds where the MMAs cannot run beside it.
+// tile's epilogue adds where the MMAs cannot run beside it.  The logits'
+// epilogue (exponentials) is the long one: 4096 x 1024 x 65536 scores took 467
+// us in 256 x 256 tiles, 402 in 128 x 256, 724 in 128 x 128; at dim 4096 the
+// large tile's smaller operand traffic wins.
 struct Cost {
   Tile tile;
   double kb, tail;
 };
-constexpr Cost kCosts[] = {{{256, 256}, 0.72, 1.5}, {{128, 256}, 0.40, 0.3}, {{128, 128}, 0.29, 0.3}};
+constexpr Cost kLogitCosts[] = {{{256, 256}, 0.77, 3.8}, {{128, 256}, 0.43, 0.3}, {{128, 128}, 0.36, 0.5}};
+constexpr Cost kProductCosts[] = {{{256, 256}, 0.74, 1.5}, {{128, 256}, 0.41, 0.5}, {{128, 128}, 0.29, 0.4}};
 constexpr double kSlabBytesPerUs = 5e6;  // an fp32 slab is written once and read once
 
 struct Choice {
@@ -902,10 +912,10 @@ struct Choice {
 // K-blocks a split).  The large tile wins wherever it fills the SMs; the small
 // ones, and splits, where it leaves them idle (333 x 1000 over 10007 columns,
 // dh: 8 large tiles; split 17 ways 21 us, unsplit 113).
-Choice pick(int64_t m, int64_t n, int64_t kbs, bool may_split, int tm, int tn, int sms) {
+Choice pick(const Cost (&costs)[3], int64_t m, int64_t n, int64_t kbs, bool may_split, int tm, int tn, int sms) {
   Choice best = {};
   double least = 0;
-  for (const Cost &c : kCosts) {
+  for (const Cost &c : costs) {
     if ((tm && tm != c.tile.tm) || (tn && tn != c.tile.tn)) continue;
     const int64_t tiles = c.tile.tiles(m, n);
     const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>(2 * sms / tiles, kbs / 8)) : 1;
@@ -934,7 +944,7 @@ struct Plan {
   bool slabs;            // DH goes through fp32 slabs
   bool store;            // one piece, from STORE's exponentials
   int64_t slab_ld, slab_elems;
-  size_t o_sc, o_sums, o_part, o_tlogit, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
+  size_t o_sc, o_sums, o_part, o_tlogit, o_tdot, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
   size_t fixed, bytes;   // bytes: fixed + the piece's d (and padded dw)
 };
 
@@ -979,8 +989,8 @@ int check(const ks_linear_ce_config &c, const ks_linear_ce_args &a, char *reason
 void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t avail, Plan &p) {
   const int sms = ks::sm_count();
   const bool fwd = a.pass != KS_CE_BACKWARD, bwd = a.pass != KS_CE_FORWARD;
-  p.g1 = pick(a.tokens, a.vocab, (a.dim + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
-  p.gw = pick(a.vocab, a.dim, (a.tokens + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
+  p.g1 = pick(kLogitCosts, a.tokens, a.vocab, (a.dim + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
+  p.gw = pick(kProductCosts, a.vocab, a.dim, (a.tokens + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
   p.pack_h = !tma_ok(a.h, a.h_stride);
   p.pack_w = !tma_ok(a.w, a.w_stride);
   p.pad_dh = bwd && !tma_ok(a.dh, a.dh_stride);
@@ -999,6 +1009,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   p.o_sums = take(fwd ? size_t((a.tokens + kCombRows - 1) / kCombRows) * 16 : 0);
   p.o_part = take(fwd ? size_t(p.n_tiles) * p.rows_p * 8 : 0);
   p.o_tlogit = take(fwd ? size_t(p.rows_p) * 4 : 0);
+  p.o_tdot = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_lse = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_h = take(p.pack_h ? size_t(a.tokens) * p.ld * 2 : 0);
   p.o_w = take(p.pack_w ? size_t(a.vocab) * p.ld * 2 : 0);
@@ -1013,7 +1024,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
       o = from;
       p.piece = piece;
       p.pieces = (a.vocab + piece - 1) / piece;
-      const Choice h = pick(a.tokens, a.dim, (std::min(piece, a.vocab) + kBK - 1) / kBK, true, c.tile_m, c.tile_n, sms);
+      const Choice h = pick(kProductCosts, a.tokens, a.dim, (std::min(piece, a.vocab) + kBK - 1) / kBK, true, c.tile_m, c.tile_n, sms);
       p.gh = h.tile;
       p.splits = int(h.splits);
       p.kb_split = int(h.kb_split);
@@ -1089,10 +1100,10 @@ int map_mn(CUtensorMap *m, int dtype, const void *p, int64_t rows, int64_t cols,
                             CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// Output [rows, cols] of 16-bit values: 32 x 32 blocks, 64-byte swizzle.
+// Output [rows, cols] of 16-bit values: blocks of 32 rows x 64 columns, 128-byte swizzle.
 int map_out(CUtensorMap *m, int dtype, void *p, int64_t rows, int64_t cols, int64_t stride) {
-  return ks::encode_tmap_2d(m, tm_type(dtype), p, uint64_t(cols), uint64_t(rows), uint64_t(stride) * 2, 32, 32,
-                            CU_TENSOR_MAP_SWIZZLE_64B);
+  return ks::encode_tmap_2d(m, tm_type(dtype), p, uint64_t(cols), uint64_t(rows), uint64_t(stride) * 2, 64, 32,
+                            CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int copy2d(bool next, bool release, const void *src, int64_t ss, void *dst, int64_t ds, int64_t rows, int64_t cols,
@@ -1146,6 +1157,12 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.group = -8;
     g.part = reinterpret_cast<float2 *>(ws + p.o_part);
     g.tlogit = reinterpret_cast<float *>(ws + p.o_tlogit);
+    g.tdot = reinterpret_cast<float *>(ws + p.o_tdot);
+    g.h = static_cast<const uint16_t *>(h);
+    g.w = static_cast<const uint16_t *>(w);
+    g.h_stride = hs;
+    g.w_stride = wst;
+    g.dim = a.dim;
     if (p.store) {
       CUtensorMap te;  // [tokens, whole tiles]: the columns past the vocabulary are -inf logits, zeros
       if ((s = map_out(&te, a.dtype, ws + p.o_d, a.tokens, up(a.vocab, 256), up(a.vocab, 256))) != KS_OK) return s;
@@ -1157,9 +1174,8 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     if (s != KS_OK) return s;
     const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
     s = ks::launch_kernel(
-        true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, g.part, int(p.n_tiles), p.rows_p,
-        static_cast<const uint16_t *>(h), hs, static_cast<const uint16_t *>(w), wst, a.dim, g.f16, g.tlogit, a.targets,
-        a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc, int(bwd));
+        true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, g.part, int(p.n_tiles), p.rows_p, g.tlogit,
+        g.tdot, a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc, int(bwd));
     if (s != KS_OK) return s;
   }
   if (!bwd) return KS_OK;
@@ -1187,7 +1203,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
       const unsigned rows8 = unsigned((a.tokens + 7) / 8);
       const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, 65535));
       s = ks::launch_kernel(true, ce_scale_kernel, dim3(rows8, cols), dim3(256), 0, st, reinterpret_cast<uint16_t *>(d), vpad, g.part,
-                          p.rows_p, p.g1.tn == 256 ? 7 : 6, lse, g.tlogit, a.targets, a.tokens, a.vocab, a.ignore_index, sc,
+                          p.rows_p, p.g1.tn == 256 ? 7 : 6, lse, g.tdot, a.targets, a.tokens, a.vocab, a.ignore_index, sc,
                           g.f16);
     } else {
       if ((s = map_k(&tw, a.dtype, wp, vp, a.dim, wst, p.g1.tn)) != KS_OK) return s;
@@ -1222,6 +1238,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     if ((s = map_out(&tc, a.dtype, p.pad_dw ? ws + p.o_dw : dwp, vp, a.dim, p.pad_dw ? p.ld : a.dw_stride)) != KS_OK)
       return s;
     g.M = int(vp);
+    g.group = -16;  // the column tiles of a block of dw's rows side by side: whole rows are written at about one time
     g.kb_total = g.kb_split = int((a.tokens + kBK - 1) / kBK);
     g.splits = 1;
     g.out_f32 = g.accumulate = 0;
