@@ -5,7 +5,7 @@
 //   d[r,v] = f[r] (exp(l[r,v] - lse[r]) - [v == t[r]])
 //   dh = d w;  dw = d^T h
 //
-// The logits [tokens, vocab] are never written.  Five GEMM-shaped passes share
+// The logits [tokens, vocab] are never written.  Four GEMM-shaped passes share
 // one persistent kernel (TMA producer warp, one MMA-issuing thread, eight
 // epilogue warps; tcgen05.mma kind::f16, fp32 accumulators in TMEM):
 //   STATS  l = h w^T; the epilogue reduces each tile's row to (max, sum of
@@ -17,12 +17,15 @@
 //          tokens x vocab x dim operations;
 //   PROB   l = h w^T again for one piece of the vocabulary; the epilogue
 //          writes d in 16 bits to the workspace (every other gradient call);
-//   DH     dh (+)= d w over the piece's columns (split over K when there are
-//          few tiles; fp32 slabs, added up in a fixed order);
-//   DW     dw rows of the piece = d^T h, complete after one pass over the
-//          tokens, so each is rounded and written once.
-// Operand layouts: h and w K-major in STATS/PROB; d K-major and w MN-major in
-// DH; d MN-major (M = the vocabulary) and h MN-major in DW -- all straight
+//   GRADS  dh (+)= d w over the piece's columns (split over K when there are
+//          few tiles; fp32 slabs, added up in a fixed order) and the piece's
+//          rows of dw = d^T h, complete after one pass over the tokens, so each
+//          is rounded and written once.  Both products in one launch: their
+//          tiles are dealt out so that every SM has the same K-blocks to do,
+//          where dh alone (128 tiles of 256 x 256 at 4096 x 2048) leaves 20 of
+//          148 SMs idle.
+// Operand layouts: h and w K-major in the logits' passes; for dh d K-major and w
+// MN-major, for dw d MN-major (M = the vocabulary) and h MN-major -- all straight
 // from the row-major tensors, no transpose pass.
 //
 // Rounding: products and sums are fp32; d is rounded to the inputs' type
@@ -57,21 +60,30 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kF16Range = 1024.f;            // factor on fp16 d
 constexpr float kF16Exp = 32768.f;             // factor on STORE's fp16 exponentials, which are at most 1
 
-enum Mode { STATS = 0, PROB = 1, DH = 2, DW = 3, STORE = 4 };
+enum Mode { STATS, STORE, PROB, GRADS };
 
 // Scalars between the kernels of one call, in the workspace.
 struct CeScalars {
   float fscale;  // on every row's f: the range factor of d
-  float escale;  // on the accumulators of DH and DW
+  float escale;  // on the accumulators of GRADS
   unsigned int counter;
 };
 
+// One product: output M x N over kb_total K-blocks of 64.
+struct CeSide {
+  int M, N;
+  int kb_total, splits, kb_split;  // K-splits and K-blocks per split (dh)
+  int group;                       // raster: > 0 groups of M-tiles, < 0 bands of N-tiles
+  int b3d;                         // MN-major B map is (64 columns, K, blocks)
+};
+
+struct CeMaps {
+  CUtensorMap a[2], b[2], c[2];
+};
+
 struct CeGemm {
-  int M, N;               // output rows and columns
-  int kb_total;           // K-blocks of 64
-  int splits, kb_split;   // K-splits and K-blocks per split (DH)
-  int group;              // raster: > 0 groups of M-tiles, < 0 bands of N-tiles
-  int b3d;                // MN-major B map is (64 columns, K, blocks)
+  CeSide side[2];         // GRADS: dh, dw; otherwise the first
+  int n1, s1, s2;         // GRADS: the first n1 CTAs share dw tiles [s2, s2 + s1), the others [0, s2)
   int f16;
   // STATS / PROB
   int64_t tokens, vocab;
@@ -87,8 +99,7 @@ struct CeGemm {
   const float *lse;
   const float *dloss;     // per token, or nullptr
   CeScalars *sc;
-  // DH
-  int out_f32, accumulate;
+  int out_f32, accumulate;  // dh goes to fp32 slabs, is added to them
   int release;            // another kernel of the call follows
 };
 
@@ -130,9 +141,9 @@ KS_DEV void tma_reduce_add_2d(const CUtensorMap *m, const void *src, int c0, int
                : "memory");
 }
 
-// Work item t -> output tile and K-split; splits outermost, tiles rastered as
-// in matmul.cu (group > 0: groups of M-tiles, M fastest; group < 0: bands of
-// N-tiles, N fastest).
+// Work item t of a product -> output tile and K-split; splits outermost, tiles
+// rastered as in matmul.cu (group > 0: groups of M-tiles, M fastest; group < 0:
+// bands of N-tiles, N fastest).
 KS_DEV void work_coords(int t, int num_m, int num_n, int group, int &tm, int &tn, int &split) {
   const int tiles = num_m * num_n;
   split = t / tiles;
@@ -148,6 +159,48 @@ KS_DEV void work_coords(int t, int num_m, int num_n, int group, int &tm, int &tn
     tm = first + r % gm;
     tn = r / gm;
   }
+}
+
+// A CTA's work: items of the first product dealt round robin, then (GRADS) tiles
+// of the second, dealt round robin within each of the two classes of CTAs, so
+// that the tiles in work at one time lie side by side and share operands in L2
+// (runs of neighbouring tiles per CTA read d from DRAM once per column tile:
+// 745 instead of 667 us for the two products of 4096 x 2048 x 32768).
+template <bool TWO, int TM, int TN>
+struct Work {
+  int count, first;  // items in all, of the first product
+  int second, step;  // tiles of the second: second, second + step, ...
+  KS_DEV explicit Work(const CeGemm &p) {
+    const CeSide &d = p.side[0];
+    const int items = ((d.M + TM - 1) / TM) * ((d.N + TN - 1) / TN) * d.splits;
+    const int cta = blockIdx.x, ctas = gridDim.x;
+    first = cta < items ? (items - 1 - cta) / ctas + 1 : 0;
+    count = first;
+    second = step = 0;
+    if (TWO) {
+      const bool more = cta < p.n1;
+      const int j = more ? cta : cta - p.n1, s = more ? p.s1 : p.s2;
+      step = more ? p.n1 : ctas - p.n1;
+      second = (more ? p.s2 : 0) + j;
+      if (j < s) count += (s - 1 - j) / step + 1;
+    }
+  }
+};
+
+struct Item {
+  int side, tm, tn, split, kb0, kb1;
+};
+
+template <bool TWO, int TM, int TN>
+KS_DEV Item item_at(const CeGemm &p, const Work<TWO, TM, TN> &w, int i) {
+  Item x;
+  x.side = TWO && i >= w.first;
+  const CeSide &d = p.side[TWO ? x.side : 0];
+  const int t = x.side ? w.second + (i - w.first) * w.step : int(blockIdx.x) + i * int(gridDim.x);
+  work_coords(t, (d.M + TM - 1) / TM, (d.N + TN - 1) / TN, d.group, x.tm, x.tn, x.split);
+  x.kb0 = x.split * d.kb_split;
+  x.kb1 = min(x.kb0 + d.kb_split, d.kb_total);
+  return x;
 }
 
 KS_DEV float max32(const uint32_t (&r)[32]) {
@@ -225,11 +278,9 @@ KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool 
 
 template <int MODE, int BN, int STAGES, int ACC, int MH>
 __global__ void __launch_bounds__(kThreads, 1)
-    ce_gemm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
-                   const __grid_constant__ CUtensorMap tma_c, const __grid_constant__ CeGemm p, KsWait wait) {
+    ce_gemm_kernel(const __grid_constant__ CeMaps maps, const __grid_constant__ CeGemm p, KsWait wait) {
   using L = Layout<BN, STAGES, ACC, MH>;
-  constexpr bool kAMn = MODE == DW;                // A is MN-major (d^T)
-  constexpr bool kBMn = MODE == DH || MODE == DW;  // B is MN-major
+  constexpr bool kGrads = MODE == GRADS;  // two products; B is MN-major, and A in the second
   constexpr int kTM = kBM * MH;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ks_smem_u32(smem_raw);
@@ -242,8 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int *abort = reinterpret_cast<volatile int *>(smem + L::misc_off + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_m = (p.M + kTM - 1) / kTM, num_n = (p.N + BN - 1) / BN;
-  const int num_work = num_m * num_n * p.splits;
+  const Work<kGrads, kTM, BN> work(p);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -255,9 +305,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     ks_mbar_init(drain, 1);
     *abort = 0;
     ks_fence_mbar_init();
-    ks_prefetch_tmap(&tma_a);
-    ks_prefetch_tmap(&tma_b);
-    if (MODE != STATS) ks_prefetch_tmap(&tma_c);
+    for (int d = 0; d < (kGrads ? 2 : 1); ++d) {
+      ks_prefetch_tmap(&maps.a[d]);
+      ks_prefetch_tmap(&maps.b[d]);
+      if (MODE != STATS) ks_prefetch_tmap(&maps.c[d]);
+    }
     if (p.release) ks_pdl_release();
   }
   if (warp == 1) {
@@ -277,11 +329,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0;
     uint32_t phase = 0, armed = 0, armed_parity = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < num_work && ok; t += gridDim.x) {
-      int tm, tn, split;
-      work_coords(t, num_m, num_n, p.group, tm, tn, split);
-      const int kb0 = split * p.kb_split, kb1 = min(kb0 + p.kb_split, p.kb_total);
-      for (int kb = kb0; kb < kb1; ++kb) {
+    for (int i = 0; i < work.count && ok; ++i) {
+      const Item x = item_at(p, work, i);
+      const CUtensorMap *ma = &maps.a[x.side], *mb = &maps.b[x.side];
+      const int b3d = p.side[kGrads ? x.side : 0].b3d;
+      for (int kb = x.kb0; kb < x.kb1; ++kb) {
         if (!ks_mbar_wait(empty + stage, phase ^ 1u, abort, wait)) {
           ok = false;
           break;
@@ -289,18 +341,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t *a_dst = smem + L::a_off + stage * L::a_bytes;
         uint8_t *b_dst = smem + L::b_off + stage * L::b_bytes;
         ks_mbar_arrive_expect_tx(full + stage, L::a_bytes + L::b_bytes);
-        if (kAMn)  // boxes of 64 K-rows x 64 columns, one copy for all of them
-          ks_tma_load_3d(a_dst, &tma_a, full + stage, 0, kb * kBK, tm * (kTM / 64));
+        if (kGrads && x.side)  // boxes of 64 K-rows x 64 columns, one copy for all of them
+          ks_tma_load_3d(a_dst, ma, full + stage, 0, kb * kBK, x.tm * (kTM / 64));
         else
-          ks_tma_load_2d(a_dst, &tma_a, full + stage, kb * kBK, tm * kTM);
-        if (!kBMn) {
-          ks_tma_load_2d(b_dst, &tma_b, full + stage, kb * kBK, tn * BN);
-        } else if (p.b3d) {
-          ks_tma_load_3d(b_dst, &tma_b, full + stage, 0, kb * kBK, tn * (BN / 64));
+          ks_tma_load_2d(a_dst, ma, full + stage, kb * kBK, x.tm * kTM);
+        if (!kGrads) {
+          ks_tma_load_2d(b_dst, mb, full + stage, kb * kBK, x.tn * BN);
+        } else if (b3d) {
+          ks_tma_load_3d(b_dst, mb, full + stage, 0, kb * kBK, x.tn * (BN / 64));
         } else {
 #pragma unroll
           for (int j = 0; j < BN / 64; ++j)
-            ks_tma_load_2d(b_dst + j * kBBox, &tma_b, full + stage, tn * BN + j * 64, kb * kBK);
+            ks_tma_load_2d(b_dst + j * kBBox, mb, full + stage, x.tn * BN + j * 64, kb * kBK);
         }
         armed |= 1u << stage;
         armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
@@ -315,34 +367,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (armed & (1u << s)) ks_mbar_wait(full + s, (armed_parity >> s) & 1u, nullptr, wait);
   } else if (warp == 1 && lane == 0) {
     // ------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = p.f16 ? (ks_idesc_bf16_f32(kBM, BN, kAMn, kBMn) & ~((7u << 7) | (7u << 10)))  // f16 operands: format 0
-                                 : ks_idesc_bf16_f32(kBM, BN, kAMn, kBMn);
+    const uint32_t fmt = p.f16 ? (7u << 7) | (7u << 10) : 0;  // f16 operands: format 0
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    int i = 0;
-    auto issue = [&](int st, bool first_kb, uint32_t d_tmem, int h0, int h1) {
+    auto issue = [&](bool a_mn, int st, bool first_kb, uint32_t d_tmem, int h0, int h1) {
+      const uint32_t idesc = (a_mn ? ks_idesc_bf16_f32(kBM, BN, true, kGrads) : ks_idesc_bf16_f32(kBM, BN, false, kGrads)) & ~fmt;
       const uint32_t a_addr = ks_smem_u32(smem + L::a_off + st * L::a_bytes);
       const uint32_t b_addr = ks_smem_u32(smem + L::b_off + st * L::b_bytes);
 #pragma unroll
       for (int k = 0; k < kBK / kUmmaK; ++k) {
         // K-major: 128-byte rows, 8-row groups 1024 bytes apart, 32 bytes per K=16.
         // MN-major: 64-column boxes kBBox apart (LBO), 8 K-rows 1024 bytes apart (SBO), 2048 bytes per K=16.
-        const uint64_t bdesc = kBMn ? ks_umma_desc_sw128(b_addr + k * 2048, kBBox, 1024)
-                                    : ks_umma_desc_sw128(b_addr + k * 32, 16, 1024);
+        const uint64_t bdesc = kGrads ? ks_umma_desc_sw128(b_addr + k * 2048, kBBox, 1024)
+                                      : ks_umma_desc_sw128(b_addr + k * 32, 16, 1024);
 #pragma unroll
         for (int h = 0; h < MH; ++h) {
           if (h < h0 || h >= h1) continue;
-          const uint64_t adesc = kAMn ? ks_umma_desc_sw128(a_addr + h * kABox + k * 2048, kBBox, 1024)
+          const uint64_t adesc = a_mn ? ks_umma_desc_sw128(a_addr + h * kABox + k * 2048, kBBox, 1024)
                                       : ks_umma_desc_sw128(a_addr + h * kABox + k * 32, 16, 1024);
           ks_umma_ss(d_tmem + h * BN, adesc, bdesc, idesc, !first_kb || k != 0);
         }
       }
     };
-    for (int t = blockIdx.x; t < num_work && ok; t += gridDim.x, ++i) {
-      int tm, tn, split;
-      work_coords(t, num_m, num_n, p.group, tm, tn, split);
-      const int kb0 = split * p.kb_split, kb1 = min(kb0 + p.kb_split, p.kb_total);
+    for (int i = 0; i < work.count && ok; ++i) {
+      const Item x = item_at(p, work, i);
+      const bool a_mn = kGrads && x.side;
       const int acc = i % ACC;
       const uint32_t acc_phase = (i / ACC) & 1;
       // The epilogue frees the accumulator one 128-row half at a time: half
@@ -353,15 +403,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t d_tmem = tmem_base + acc * BN * MH;
       bool rest_free = MH == 1;
       int pend = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = x.kb0; kb < x.kb1; ++kb) {
         if (!ks_mbar_wait(full + stage, phase, abort, wait)) {
           ok = false;
           break;
         }
         ks_tc_fence_after();
-        issue(stage, kb == kb0, d_tmem, 0, 1);
+        issue(a_mn, stage, kb == x.kb0, d_tmem, 0, 1);
         if (!rest_free) {
-          if (pend + 1 < STAGES && kb + 1 < kb1 &&
+          if (pend + 1 < STAGES && kb + 1 < x.kb1 &&
               !ks_mbar_test_wait(ks_smem_u32(tempty + acc * MH + 1), acc_phase ^ 1u)) {
             ++pend;
             if (++stage == STAGES) {
@@ -376,12 +426,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           rest_free = true;
           for (int q = pend; q > 0; --q) {
             const int sp = (stage + STAGES - q) % STAGES;
-            issue(sp, kb - q == kb0, d_tmem, 1, MH);
+            issue(a_mn, sp, kb - q == x.kb0, d_tmem, 1, MH);
             ks_umma_commit(empty + sp);
           }
           pend = 0;
         }
-        issue(stage, kb == kb0, d_tmem, 1, MH);
+        issue(a_mn, stage, kb == x.kb0, d_tmem, 1, MH);
         ks_umma_commit(empty + stage);
         if (++stage == STAGES) {
           stage = 0;
@@ -401,9 +451,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int cg = (warp - 2) / 4 * kCols;  // its first column
     uint8_t *stg = smem + L::c_off + (warp - 2) * kCStage;
     const bool f16 = p.f16 != 0;
-    const bool wide = MODE == DH && p.out_f32;  // 32-bit blocks
-    float escale = 1.f, fscale = 1.f;
-    if (MODE == DH || MODE == DW) escale = wide ? 1.f : __ldcg(&p.sc->escale);
+    float scale = 1.f, fscale = 1.f;
+    if (kGrads) scale = __ldcg(&p.sc->escale);
     if (MODE == PROB) fscale = __ldcg(&p.sc->fscale);
     if (MODE == STATS || MODE == STORE) {
       // these warps have nothing else to do until the first tile is complete
@@ -414,12 +463,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) p.tdot[row] = v;
       }
     }
-    int i = 0;
-    for (int t = blockIdx.x; t < num_work; t += gridDim.x, ++i) {
+    for (int i = 0; i < work.count; ++i) {
       const int acc = i % ACC;
       const uint32_t acc_phase = (i / ACC) & 1;
-      int tm, tn, split;
-      work_coords(t, num_m, num_n, p.group, tm, tn, split);
+      const Item x = item_at(p, work, i);
+      const int tm = x.tm, tn = x.tn;
+      const bool wide = kGrads && !x.side && p.out_f32;        // 32-bit blocks, not scaled yet
+      const bool add = kGrads && !x.side && p.accumulate;
+      const float escale = wide ? 1.f : scale;
+      const int out_m = p.side[kGrads ? x.side : 0].M, out_n = p.side[kGrads ? x.side : 0].N;
+      const int64_t slab = kGrads && !x.side ? x.split * p.rows_p : 0;  // first row of the split's slab
       // what this lane's rows need, loaded while the MMAs still run
       int tcol[MH];       // target column relative to the tile, or one outside it
       float lse2[MH], f[MH];
@@ -513,7 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 32; ++j)
               if (j >= left || fr == 0.f) r[j] = 0u;
           }
-        } else if constexpr (MODE == DH || MODE == DW) {
+        } else if constexpr (kGrads) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
         }
@@ -524,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool second = !wide && (k & 1);
           const int c0 = tn * BN + cb - (second ? 32 : 0);
           const int64_t r0 = int64_t(tm) * kTM + h * kBM + q * 32;
-          if (c0 >= p.N || r0 >= p.M) return;  // blocks past the edge hold nothing
+          if (c0 >= out_n || r0 >= out_m) return;  // blocks past the edge hold nothing
           if (!second) {
             if (lane == 0) ks_bulk_wait_read<0>();  // the last store has read the staging
             __syncwarp();
@@ -551,10 +604,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           ks_fence_proxy_async();
           __syncwarp();
           if (lane == 0) {
-            if (MODE == DH && p.accumulate)
-              tma_reduce_add_2d(&tma_c, stg, c0, int(split * p.rows_p + r0));
+            if (add)
+              tma_reduce_add_2d(&maps.c[x.side], stg, c0, int(slab + r0));
             else
-              ks_tma_store_2d(&tma_c, stg, c0, int((MODE == DH ? split * p.rows_p : 0) + r0));
+              ks_tma_store_2d(&maps.c[x.side], stg, c0, int(slab + r0));
             ks_bulk_commit_group();
           }
         }
@@ -905,43 +958,81 @@ constexpr double kSlabBytesPerUs = 5e6;  // an fp32 slab is written once and rea
 struct Choice {
   Tile tile;
   int64_t splits, kb_split;
+  double item, other;  // GRADS: time of an item of dh, of a tile of dw
 };
 
-// Tile and K-splits with the least estimated time: rounds of tiles over the
-// SMs x K-blocks, plus the slabs' traffic where K is split (at least 8
-// K-blocks a split).  The large tile wins wherever it fills the SMs; the small
-// ones, and splits, where it leaves them idle (333 x 1000 over 10007 columns,
-// dh: 8 large tiles; split 17 ways 21 us, unsplit 113).
-Choice pick(const Cost (&costs)[3], int64_t m, int64_t n, int64_t kbs, bool may_split, int tm, int tn, int sms) {
+bool allowed(const Cost &c, const ks_linear_ce_config &cfg) {
+  return (!cfg.tile_m || cfg.tile_m == c.tile.tm) && (!cfg.tile_n || cfg.tile_n == c.tile.tn);
+}
+
+// Tile of the logits' passes with the least estimated time: rounds of tiles over
+// the SMs x K-blocks.
+Tile pick_logits(const ks_linear_ce_config &cfg, int64_t m, int64_t n, int64_t kbs, int sms) {
+  const Cost *best = nullptr;
+  double least = 0;
+  for (const Cost &c : kLogitCosts) {
+    if (!allowed(c, cfg)) continue;
+    const double us = double((c.tile.tiles(m, n) + sms - 1) / sms) * (double(kbs) * c.kb + c.tail);
+    if (!best || us < least) {
+      least = us;
+      best = &c;
+    }
+  }
+  return best->tile;
+}
+
+// Tile and K-splits of dh [m, n] over kbs K-blocks beside dw [vocab, n] over
+// kb2: all work evenly over the SMs, but no less than the longest item, plus
+// the slabs' traffic where K is split (at least 8 K-blocks a split).  (333 x
+// 1000 over 10007 columns, dh alone: 8 large tiles; split 17 ways 21 us,
+// unsplit 113.)
+Choice pick_grads(const ks_linear_ce_config &cfg, int64_t m, int64_t n, int64_t kbs, int64_t vocab, int64_t kb2, int sms) {
   Choice best = {};
   double least = 0;
-  for (const Cost &c : costs) {
-    if ((tm && tm != c.tile.tm) || (tn && tn != c.tile.tn)) continue;
+  for (const Cost &c : kProductCosts) {
+    if (!allowed(c, cfg)) continue;
     const int64_t tiles = c.tile.tiles(m, n);
-    const int64_t most = may_split ? std::max<int64_t>(1, std::min<int64_t>(2 * sms / tiles, kbs / 8)) : 1;
+    const double other = double(kb2) * c.kb + c.tail, dw = double(c.tile.tiles(vocab, n)) * other;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(2 * sms / tiles, kbs / 8));
     for (int64_t s = 1; s <= most; ++s) {
       const int64_t per = (kbs + s - 1) / s, used = (kbs + per - 1) / per;
-      const double rounds = double((tiles * used + sms - 1) / sms);
-      double us = rounds * (double(per) * c.kb + c.tail);
+      const double item = double(per) * c.kb + c.tail;
+      double us = std::max(item, (double(tiles * used) * item + dw) / sms);
       if (used > 1) us += 4 + double(used) * double(m) * double(n) * 8 / kSlabBytesPerUs;
       if (best.splits == 0 || us < least) {
         least = us;
-        best = Choice{c.tile, used, per};
+        best = Choice{c.tile, used, per, item, other};
       }
     }
   }
   return best;
 }
 
+// GRADS on `ctas` CTAs: those with one item of dh more than the others (the
+// first n1) take fewer tiles of dw, s1 in all against s2.
+void share(const Choice &c, int64_t items, int64_t tiles, int ctas, CeGemm &g) {
+  const int64_t n1 = items % ctas, n2 = ctas - n1;
+  const double hi = double(items / ctas + 1) * c.item, lo = double(items / ctas) * c.item;
+  // level t: n1 (t - hi)+ + n2 (t - lo)+ = the tiles' time
+  const double all = double(tiles) * c.other;
+  double t = lo + all / double(n2);
+  if (t > hi && n1) t = (all + double(n1) * hi + double(n2) * lo) / double(ctas);
+  int64_t s1 = n1 ? int64_t(std::max(0.0, double(n1) * (t - hi) / c.other) + 0.5) : 0;
+  s1 = std::min(s1, tiles);
+  g.n1 = int(n1);
+  g.s1 = int(s1);
+  g.s2 = int(tiles - s1);
+}
+
 struct Plan {
-  Tile g1, gh, gw;
+  Tile g1;               // tiles of the logits' passes
+  Choice grads;
   bool pack_h, pack_w, pad_dh, pad_dw;
   int64_t ld;            // row stride of packed h / w / padded outputs
   int64_t rows_p;        // tokens rounded up to 256
   int64_t n_tiles;       // vocabulary half tiles of STATS or STORE
   int64_t piece, pieces; // vocabulary columns per piece, pieces
-  int splits, kb_split;  // K-splits of DH, K-blocks in each
-  bool slabs;            // DH goes through fp32 slabs
+  bool slabs;            // dh goes through fp32 slabs
   bool store;            // one piece, from STORE's exponentials
   int64_t slab_ld, slab_elems;
   size_t o_sc, o_sums, o_part, o_tlogit, o_tdot, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
@@ -989,8 +1080,7 @@ int check(const ks_linear_ce_config &c, const ks_linear_ce_args &a, char *reason
 void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t avail, Plan &p) {
   const int sms = ks::sm_count();
   const bool fwd = a.pass != KS_CE_BACKWARD, bwd = a.pass != KS_CE_FORWARD;
-  p.g1 = pick(kLogitCosts, a.tokens, a.vocab, (a.dim + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
-  p.gw = pick(kProductCosts, a.vocab, a.dim, (a.tokens + kBK - 1) / kBK, false, c.tile_m, c.tile_n, sms).tile;
+  p.g1 = pick_logits(c, a.tokens, a.vocab, (a.dim + kBK - 1) / kBK, sms);
   p.pack_h = !tma_ok(a.h, a.h_stride);
   p.pack_w = !tma_ok(a.w, a.w_stride);
   p.pad_dh = bwd && !tma_ok(a.dh, a.dh_stride);
@@ -1013,7 +1103,6 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   p.o_lse = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_h = take(p.pack_h ? size_t(a.tokens) * p.ld * 2 : 0);
   p.o_w = take(p.pack_w ? size_t(a.vocab) * p.ld * 2 : 0);
-  p.splits = p.kb_split = 1;
   p.slabs = p.store = false;
   p.piece = p.pieces = 0;
   p.o_dh = p.o_slab = p.o_dw = p.o_d = o;
@@ -1024,15 +1113,13 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
       o = from;
       p.piece = piece;
       p.pieces = (a.vocab + piece - 1) / piece;
-      const Choice h = pick(kProductCosts, a.tokens, a.dim, (std::min(piece, a.vocab) + kBK - 1) / kBK, true, c.tile_m, c.tile_n, sms);
-      p.gh = h.tile;
-      p.splits = int(h.splits);
-      p.kb_split = int(h.kb_split);
-      p.slabs = p.splits > 1 || p.pieces > 1;
+      const int64_t cols = std::min(piece, a.vocab);
+      p.grads = pick_grads(c, a.tokens, a.dim, (cols + kBK - 1) / kBK, cols, (a.tokens + kBK - 1) / kBK, sms);
+      p.slabs = p.grads.splits > 1 || p.pieces > 1;
       p.slab_ld = up(a.dim, 32);
       p.slab_elems = p.rows_p * p.slab_ld;
       p.o_dh = take(p.pad_dh && !p.slabs ? size_t(a.tokens) * p.ld * 2 : 0);
-      p.o_slab = take(p.slabs ? size_t(p.splits) * p.slab_elems * 4 : 0);
+      p.o_slab = take(p.slabs ? size_t(p.grads.splits) * p.slab_elems * 4 : 0);
       p.fixed = o;
       p.o_dw = take(p.pad_dw ? size_t(std::min(piece, a.vocab)) * p.ld * 2 : 0);
       p.o_d = take(size_t(a.tokens) * piece * 2);
@@ -1055,25 +1142,25 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
 }
 
 template <int MODE, int BN, int STAGES, int ACC, int MH>
-int launch(bool next, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g,
-           cudaStream_t st) {
+int launch(bool next, const CeMaps &maps, CeGemm &g, const Choice *c, cudaStream_t st) {
   using L = Layout<BN, STAGES, ACC, MH>;
   auto kern = ce_gemm_kernel<MODE, BN, STAGES, ACC, MH>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(L::request));
   if (e != cudaSuccess) return ks::map_cuda(e);
-  const int64_t work = int64_t((g.M + kBM * MH - 1) / (kBM * MH)) * ((g.N + BN - 1) / BN) * g.splits;
-  if (work > (int64_t(1) << 30)) return KS_ERR_INVALID_ARGS;
-  const int sms = ks::sm_count();
-  return ks::launch_kernel(next, kern, dim3(unsigned(std::min<int64_t>(work, sms))), dim3(kThreads), L::request, st, ta,
-                           tb, tc, g, ks::wait_ctx());
+  const Tile t{kBM * MH, BN};
+  const int64_t items = t.tiles(g.side[0].M, g.side[0].N) * g.side[0].splits;
+  const int64_t tiles = MODE == GRADS ? t.tiles(g.side[1].M, g.side[1].N) : 0;
+  if (items > (int64_t(1) << 30) || tiles > (int64_t(1) << 30)) return KS_ERR_INVALID_ARGS;
+  const int ctas = int(std::min<int64_t>(items + tiles, ks::sm_count()));
+  if (MODE == GRADS) share(*c, items, tiles, ctas, g);
+  return ks::launch_kernel(next, kern, dim3(unsigned(ctas)), dim3(kThreads), L::request, st, maps, g, ks::wait_ctx());
 }
 
 template <int MODE>
-int launch_tile(bool next, Tile t, const CUtensorMap &ta, const CUtensorMap &tb, const CUtensorMap &tc, const CeGemm &g,
-                cudaStream_t st) {
-  if (t.tm == 256) return launch<MODE, 256, 3, 1, 2>(next, ta, tb, tc, g, st);
-  return t.tn == 256 ? launch<MODE, 256, 4, 2, 1>(next, ta, tb, tc, g, st)
-                     : launch<MODE, 128, 5, 2, 1>(next, ta, tb, tc, g, st);
+int launch_tile(bool next, Tile t, const CeMaps &maps, CeGemm &g, const Choice *c, cudaStream_t st) {
+  if (t.tm == 256) return launch<MODE, 256, 3, 1, 2>(next, maps, g, c, st);
+  return t.tn == 256 ? launch<MODE, 256, 4, 2, 1>(next, maps, g, c, st)
+                     : launch<MODE, 128, 5, 2, 1>(next, maps, g, c, st);
 }
 
 CUtensorMapDataType tm_type(int dtype) {
@@ -1143,18 +1230,14 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   g.ignore = a.ignore_index;
   g.rows_p = p.rows_p;
   g.sc = sc;
-  g.splits = g.release = 1;
-  const int64_t kd = (a.dim + kBK - 1) / kBK;
-  CUtensorMap th, tw;
-  if ((s = map_k(&th, a.dtype, h, a.tokens, a.dim, hs, p.g1.tm)) != KS_OK) return s;
+  g.release = 1;
+  const int kd = int((a.dim + kBK - 1) / kBK);
+  CeMaps maps = {};
+  if ((s = map_k(&maps.a[0], a.dtype, h, a.tokens, a.dim, hs, p.g1.tm)) != KS_OK) return s;
   float *lse = a.lse;
   if (fwd) {
     if (!lse) lse = reinterpret_cast<float *>(ws + p.o_lse);
-    if ((s = map_k(&tw, a.dtype, w, a.vocab, a.dim, wst, p.g1.tn)) != KS_OK) return s;
-    g.M = int(a.tokens);
-    g.N = int(a.vocab);
-    g.kb_total = g.kb_split = int(kd);
-    g.group = -8;
+    if ((s = map_k(&maps.b[0], a.dtype, w, a.vocab, a.dim, wst, p.g1.tn)) != KS_OK) return s;
     g.part = reinterpret_cast<float2 *>(ws + p.o_part);
     g.tlogit = reinterpret_cast<float *>(ws + p.o_tlogit);
     g.tdot = reinterpret_cast<float *>(ws + p.o_tdot);
@@ -1163,13 +1246,14 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.h_stride = hs;
     g.w_stride = wst;
     g.dim = a.dim;
+    // STORE: [tokens, whole tiles], the columns past the vocabulary are -inf logits, zeros
+    const int64_t wide = up(a.vocab, 256);
+    g.side[0] = CeSide{int(a.tokens), int(p.store ? wide : a.vocab), kd, 1, kd, -8, 0};
     if (p.store) {
-      CUtensorMap te;  // [tokens, whole tiles]: the columns past the vocabulary are -inf logits, zeros
-      if ((s = map_out(&te, a.dtype, ws + p.o_d, a.tokens, up(a.vocab, 256), up(a.vocab, 256))) != KS_OK) return s;
-      g.N = int(up(a.vocab, 256));
-      s = launch_tile<STORE>(next, p.g1, th, tw, te, g, st);
+      if ((s = map_out(&maps.c[0], a.dtype, ws + p.o_d, a.tokens, wide, wide)) != KS_OK) return s;
+      s = launch_tile<STORE>(next, p.g1, maps, g, nullptr, st);
     } else {
-      s = launch_tile<STATS>(next, p.g1, th, tw, th, g, st);
+      s = launch_tile<STATS>(next, p.g1, maps, g, nullptr, st);
     }
     if (s != KS_OK) return s;
     const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
@@ -1189,62 +1273,51 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, vp = std::min(p.piece, a.vocab - v0), vpad = up(vp, 256);
     const char *wp = static_cast<const char *>(w) + v0 * wst * 2;
-    CUtensorMap ta, tb, tc;
     // d of the piece: [tokens, vpad], columns past the vocabulary zero
-    g.M = int(a.tokens);
-    g.N = int(vpad);
-    g.kb_total = g.kb_split = int(kd);
-    g.splits = 1;
-    g.group = -8;
-    g.v0 = v0;
-    g.lse = lse;
-    g.dloss = a.reduction == KS_CE_NONE ? a.dloss : nullptr;
     if (p.store) {
       const unsigned rows8 = unsigned((a.tokens + 7) / 8);
       const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, 65535));
-      s = ks::launch_kernel(true, ce_scale_kernel, dim3(rows8, cols), dim3(256), 0, st, reinterpret_cast<uint16_t *>(d), vpad, g.part,
-                          p.rows_p, p.g1.tn == 256 ? 7 : 6, lse, g.tdot, a.targets, a.tokens, a.vocab, a.ignore_index, sc,
-                          g.f16);
+      s = ks::launch_kernel(true, ce_scale_kernel, dim3(rows8, cols), dim3(256), 0, st, reinterpret_cast<uint16_t *>(d),
+                            vpad, g.part, p.rows_p, p.g1.tn == 256 ? 7 : 6, lse, g.tdot, a.targets, a.tokens, a.vocab,
+                            a.ignore_index, sc, g.f16);
     } else {
-      if ((s = map_k(&tw, a.dtype, wp, vp, a.dim, wst, p.g1.tn)) != KS_OK) return s;
-      if ((s = map_out(&tc, a.dtype, d, a.tokens, vpad, vpad)) != KS_OK) return s;
-      s = launch_tile<PROB>(true, p.g1, th, tw, tc, g, st);
+      g.side[0] = CeSide{int(a.tokens), int(vpad), kd, 1, kd, -8, 0};
+      g.v0 = v0;
+      g.lse = lse;
+      g.dloss = a.reduction == KS_CE_NONE ? a.dloss : nullptr;
+      if ((s = map_k(&maps.b[0], a.dtype, wp, vp, a.dim, wst, p.g1.tn)) != KS_OK) return s;
+      if ((s = map_out(&maps.c[0], a.dtype, d, a.tokens, vpad, vpad)) != KS_OK) return s;
+      s = launch_tile<PROB>(true, p.g1, maps, g, nullptr, st);
     }
     if (s != KS_OK) return s;
-    // dh (+)= d w
-    if ((s = map_k(&ta, a.dtype, d, a.tokens, vp, vpad, p.gh.tm)) != KS_OK) return s;
-    if ((s = map_mn(&tb, a.dtype, wp, vp, a.dim, wst, p.gh.tn, &g.b3d)) != KS_OK) return s;
-    const bool slabbed = p.slabs;
-    if (slabbed)
-      s = ks::encode_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, slabs, uint64_t(p.slab_ld),
-                             uint64_t(p.splits) * p.rows_p, uint64_t(p.slab_ld) * 4, 32, 32, CU_TENSOR_MAP_SWIZZLE_128B);
+    // dh (+)= d w, and the piece's rows of dw = d^T h
+    const Tile t = p.grads.tile;
+    CeMaps mg = {};
+    const int kv = int((vp + kBK - 1) / kBK), kt = int((a.tokens + kBK - 1) / kBK), per = int(p.grads.kb_split);
+    g.side[0] = CeSide{int(a.tokens), int(a.dim), kv, (kv + per - 1) / per, per, 8, 0};
+    // dw: the column tiles of a block of rows side by side, so that whole rows are written at about one time
+    g.side[1] = CeSide{int(vp), int(a.dim), kt, 1, kt, -16, 0};
+    if ((s = map_k(&mg.a[0], a.dtype, d, a.tokens, vp, vpad, t.tm)) != KS_OK) return s;
+    if ((s = map_mn(&mg.b[0], a.dtype, wp, vp, a.dim, wst, t.tn, &g.side[0].b3d)) != KS_OK) return s;
+    if (p.slabs)
+      s = ks::encode_tmap_2d(&mg.c[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, slabs, uint64_t(p.slab_ld),
+                             uint64_t(p.grads.splits) * p.rows_p, uint64_t(p.slab_ld) * 4, 32, 32,
+                             CU_TENSOR_MAP_SWIZZLE_128B);
     else
-      s = map_out(&tc, a.dtype, p.pad_dh ? ws + p.o_dh : a.dh, a.tokens, a.dim, p.pad_dh ? p.ld : a.dh_stride);
+      s = map_out(&mg.c[0], a.dtype, p.pad_dh ? ws + p.o_dh : a.dh, a.tokens, a.dim, p.pad_dh ? p.ld : a.dh_stride);
     if (s != KS_OK) return s;
-    g.N = int(a.dim);
-    g.kb_total = int((vp + kBK - 1) / kBK);
-    g.kb_split = p.kb_split;
-    g.splits = int((g.kb_total + g.kb_split - 1) / g.kb_split);
-    g.group = 8;
-    g.out_f32 = slabbed;
-    g.accumulate = slabbed && i > 0;
-    if ((s = launch_tile<DH>(true, p.gh, ta, tb, tc, g, st)) != KS_OK) return s;
-    // rows v0.. of dw = d^T h
     int a3d = 0;
-    if ((s = map_mn(&ta, a.dtype, d, a.tokens, vpad, vpad, p.gw.tm, &a3d)) != KS_OK) return s;
+    if ((s = map_mn(&mg.a[1], a.dtype, d, a.tokens, vpad, vpad, t.tm, &a3d)) != KS_OK) return s;
     if (!a3d) return KS_ERR_OTHER;
-    if ((s = map_mn(&tb, a.dtype, h, a.tokens, a.dim, hs, p.gw.tn, &g.b3d)) != KS_OK) return s;
+    if ((s = map_mn(&mg.b[1], a.dtype, h, a.tokens, a.dim, hs, t.tn, &g.side[1].b3d)) != KS_OK) return s;
     char *dwp = static_cast<char *>(a.dw) + v0 * a.dw_stride * 2;
-    if ((s = map_out(&tc, a.dtype, p.pad_dw ? ws + p.o_dw : dwp, vp, a.dim, p.pad_dw ? p.ld : a.dw_stride)) != KS_OK)
+    if ((s = map_out(&mg.c[1], a.dtype, p.pad_dw ? ws + p.o_dw : dwp, vp, a.dim, p.pad_dw ? p.ld : a.dw_stride)) != KS_OK)
       return s;
-    g.M = int(vp);
-    g.group = -16;  // the column tiles of a block of dw's rows side by side: whole rows are written at about one time
-    g.kb_total = g.kb_split = int((a.tokens + kBK - 1) / kBK);
-    g.splits = 1;
-    g.out_f32 = g.accumulate = 0;
+    g.out_f32 = p.slabs;
+    g.accumulate = p.slabs && i > 0;
     const bool last = i + 1 == p.pieces && !p.slabs && !p.pad_dh;
     g.release = !last || p.pad_dw;
-    if ((s = launch_tile<DW>(true, p.gw, ta, tb, tc, g, st)) != KS_OK) return s;
+    if ((s = launch_tile<GRADS>(true, t, mg, g, &p.grads, st)) != KS_OK) return s;
     g.release = 1;
     if (p.pad_dw && (s = copy2d(true, !last, ws + p.o_dw, p.ld, dwp, a.dw_stride, vp, a.dim, st)) != KS_OK) return s;
   }
@@ -1252,7 +1325,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     const int64_t items = a.tokens * ((a.dim + 3) / 4);
     const int grid = int(std::min<int64_t>((items + 255) / 256, int64_t(ks::sm_count()) * 8));
     const int vec = reinterpret_cast<uintptr_t>(a.dh) % 8 == 0 && a.dh_stride % 4 == 0;
-    return ks::launch_kernel(true, ce_dh_finish_kernel, dim3(grid), dim3(256), 0, st, slabs, p.splits, p.slab_elems, p.slab_ld,
+    return ks::launch_kernel(true, ce_dh_finish_kernel, dim3(grid), dim3(256), 0, st, slabs, int(p.grads.splits), p.slab_elems, p.slab_ld,
                            a.tokens, a.dim, sc, static_cast<uint16_t *>(a.dh), a.dh_stride, int(a.dtype == KS_F16), vec);
   }
   if (p.pad_dh) return copy2d(true, false, ws + p.o_dh, p.ld, a.dh, a.dh_stride, a.tokens, a.dim, st);
