@@ -90,7 +90,8 @@ struct CeGemm {
   int64_t v0;             // first vocabulary column of the piece (PROB)
   const int64_t *targets;
   int64_t ignore;
-  float2 *part;           // [half tiles][rows_p] (max, sum)
+  float2 *part;           // [tokens][half tiles] (max, sum)
+  int parts;              // half tiles
   float *tlogit;          // [rows_p] the target's logit, from the accumulator
   const uint16_t *h, *w;  // for the target's dot product
   int64_t h_stride, w_stride, dim;
@@ -544,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           s += (a4[0] + a4[1]) + (a4[2] + a4[3]);
           m = mn;
           if ((k + 1) % kBlocks == 0 && row < p.tokens)
-            p.part[(int64_t(tn) * 2 + cg / kCols) * p.rows_p + row] = make_float2(m, s);
+            p.part[row * p.parts + tn * 2 + cg / kCols] = make_float2(m, s);
         }
         if constexpr (MODE == STORE) {
           if (f16) {
@@ -634,85 +635,70 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // lse and loss of every row from the tiles' (max, sum); the last block adds up
 // the loss over the rows, in a fixed order, and leaves the gradient's scalars.
-// 8 rows x 32 slices of the tiles per block: 64-byte segments of `part`.
+// A warp per row, eight rows per block.
 // ---------------------------------------------------------------------------
 constexpr int kCombRows = 8;
 
 __global__ void __launch_bounds__(256)
-    ce_combine_kernel(const float2 *__restrict__ part, int tiles, int64_t rows_p, const float *__restrict__ tlogit,
-                      const float *__restrict__ tdot,
-                      const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab, int64_t ignore, int reduction,
-                      float grad_scale, const float *dloss, float range, float *__restrict__ loss,
-                      float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc, int release) {
-  __shared__ float sm[8][kCombRows], ss[8][kCombRows];
+    ce_combine_kernel(const float2 *__restrict__ part, int tiles, const float *__restrict__ tlogit,
+                      const float *__restrict__ tdot, const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab,
+                      int64_t ignore, int reduction, float grad_scale, const float *dloss, float range,
+                      float *__restrict__ loss, float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc,
+                      int release) {
   __shared__ double shl[kCombRows], shn[kCombRows];
   __shared__ bool is_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (release) ks_pdl_release();
   ks_pdl_wait();
-  const int rr = tid & (kCombRows - 1), slice = tid / kCombRows;
-  const int64_t row = int64_t(blockIdx.x) * kCombRows + rr;
-  // the row's own values, loaded beside the partial sums
-  int64_t t = ignore;
-  float lt = 0.f, old = 0.f;
-  if (tid < kCombRows && row < tokens) {
-    t = targets[row];
-    lt = __ldcg(tdot + row);
-    old = __ldcg(tlogit + row);
-  }
-  float m = -INFINITY, s = 0.f;
-  auto add = [&](float m2, float s2) {  // (m, s) (+) (m2, s2); a side with no finite maximum adds its sum as it is
-    const float mn = fmaxf(m, m2);
-    if (mn == -INFINITY) {
-      s += s2;  // zeros, or the NaN of a row that has one
-    } else {
-      s = s * ex2((m - mn) * kLog2e) + s2 * ex2((m2 - mn) * kLog2e);
-    }
-    m = mn;
-  };
-  if (row < tokens)
+  const int64_t row = int64_t(blockIdx.x) * kCombRows + warp;
+  double l = 0.0, n = 0.0;
+  if (row < tokens) {
+    // the row's own values, loaded beside the partial sums
+    const int64_t t = targets[row];
+    const float lt = __ldcg(tdot + row), old = __ldcg(tlogit + row);
+    float m = -INFINITY, s = 0.f;
+    auto add = [&](float m2, float s2) {  // (m, s) (+) (m2, s2); a side with no finite maximum adds its sum as it is
+      const float mn = fmaxf(m, m2);
+      if (mn == -INFINITY) {
+        s += s2;  // zeros, or the NaN of a row that has one
+      } else {
+        s = s * ex2((m - mn) * kLog2e) + s2 * ex2((m2 - mn) * kLog2e);
+      }
+      m = mn;
+    };
 #pragma unroll 4
-    for (int t = slice; t < tiles; t += 256 / kCombRows) {
-      const float2 v = __ldcg(part + int64_t(t) * rows_p + row);
+    for (int i = lane; i < tiles; i += 32) {
+      const float2 v = __ldcg(part + row * tiles + i);
       add(v.x, v.y);
     }
 #pragma unroll
-  for (int o = kCombRows; o < 32; o <<= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-    add(m2, s2);
-  }
-  if (lane < kCombRows) {
-    sm[warp][lane] = m;
-    ss[warp][lane] = s;
-  }
-  __syncthreads();
-  if (tid < kCombRows) {
-    m = sm[0][tid];
-    s = ss[0][tid];
-#pragma unroll
-    for (int w = 1; w < 8; ++w) add(sm[w][tid], ss[w][tid]);
-    double l = 0.0, n = 0.0;
-    if (row < tokens) {
-      const bool valid = t != ignore && t >= 0 && t < vocab;
-      // the target's logit as the dot product, in the sum too
-      if (valid && isfinite(lt) && isfinite(old)) s += ex2((lt - m) * kLog2e) - ex2((old - m) * kLog2e);
-      const float lse = m + logf(s);  // -inf + log 0: a row of -inf logits
-      lse_out[row] = lse;
-      float v = 0.f;
-      if (t != ignore) {
-        v = valid ? lse - lt : __int_as_float(0x7fc00000);
-        n = 1.0;
-      }
-      if (reduction == KS_CE_NONE && loss) loss[row] = v;
-      l = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+      add(m2, s2);
     }
-    shl[tid] = l;
-    shn[tid] = n;
+    const bool valid = t != ignore && t >= 0 && t < vocab;
+    // the target's logit as the dot product, in the sum too
+    if (valid && isfinite(lt) && isfinite(old)) s += ex2((lt - m) * kLog2e) - ex2((old - m) * kLog2e);
+    const float lse = m + logf(s);  // -inf + log 0: a row of -inf logits
+    float v = 0.f;
+    if (t != ignore) {
+      v = valid ? lse - lt : __int_as_float(0x7fc00000);
+      n = 1.0;
+    }
+    if (lane == 0) {
+      lse_out[row] = lse;
+      if (reduction == KS_CE_NONE && loss) loss[row] = v;
+    }
+    l = v;
+  }
+  if (lane == 0) {
+    shl[warp] = l;
+    shn[warp] = n;
   }
   if (reduction == KS_CE_NONE) return;
   __syncthreads();
   if (tid == 0) {
-    double l = 0.0, n = 0.0;
+    l = n = 0.0;
     for (int j = 0; j < kCombRows; ++j) {
       l += shl[j];
       n += shn[j];
@@ -725,7 +711,7 @@ __global__ void __launch_bounds__(256)
   if (!is_last) return;
   __threadfence();
   __shared__ double wl[8], wn[8];
-  double l = 0.0, n = 0.0;
+  l = n = 0.0;
   for (unsigned j = tid; j < gridDim.x; j += 256) {
     const double2 v = __ldcg(sums + j);
     l += v.x;
@@ -752,18 +738,16 @@ __global__ void __launch_bounds__(256)
 }
 
 // STORE's exponentials e -> d in place: d = f (e exp(tile maximum - lse) -
-// [target]).  A warp takes 1024 columns of one row, four 16-byte loads a lane
-// in flight; a block's eight warps take eight rows, whose tile maxima share
-// 32-byte sectors.  Reads and writes 2 bytes a value.
+// [target]).  A CTA takes 8192 columns of one row, 16 KB, a warp 1024 of them,
+// four 16-byte loads a lane in flight.  Reads and writes 2 bytes a value.
 __global__ void __launch_bounds__(256)
-    ce_scale_kernel(uint16_t *__restrict__ d, int64_t ld, const float2 *__restrict__ part, int64_t rows_p, int tile_log2,
+    ce_scale_kernel(uint16_t *__restrict__ d, int64_t ld, const float2 *__restrict__ part, int tiles, int tile_log2,
                     const float *__restrict__ lse, const float *__restrict__ tdot, const int64_t *__restrict__ targets,
                     int64_t tokens, int64_t vocab, int64_t ignore, const CeScalars *__restrict__ sc, int f16) {
   const int lane = threadIdx.x & 31;
-  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int64_t row = blockIdx.x;
   ks_pdl_release();
   ks_pdl_wait();
-  if (row >= tokens) return;
   const int64_t t = targets[row];
   const bool valid = t != ignore && t >= 0 && t < vocab;
   const float f = valid ? __ldcg(&sc->fscale) : 0.f, fe = f16 ? f / kF16Exp : f;
@@ -771,7 +755,11 @@ __global__ void __launch_bounds__(256)
   uint16_t *dr = d + row * ld;
   const float dt = valid ? f * ex2(fmaf(__ldcg(tdot + row), kLog2e, -l2)) - f : 0.f;
   constexpr int step = 256;
-  for (int64_t c0 = int64_t(blockIdx.y) * (4 * step) + lane * 8; c0 < ld; c0 += int64_t(gridDim.y) * (4 * step)) {
+  // the last columns first: STORE wrote them last, so they are still in L2, and the
+  // first columns, where the products begin, are left there
+  const int64_t blocks = (ld + 32 * step - 1) / (32 * step);
+  for (int64_t y = blocks - 1 - blockIdx.y; y >= 0; y -= gridDim.y) {
+    const int64_t c0 = (y * 8 + (threadIdx.x >> 5)) * (4 * step) + lane * 8;
     uint4 v[4];
     float k[4];
 #pragma unroll
@@ -780,7 +768,7 @@ __global__ void __launch_bounds__(256)
       k[j] = 0.f;
       if (c < ld && valid) {
         v[j] = __ldcg(reinterpret_cast<const uint4 *>(dr + c));
-        if (c < vocab) k[j] = __ldcg(&part[(c >> tile_log2) * rows_p + row].x);
+        if (c < vocab) k[j] = __ldcg(&part[row * tiles + (c >> tile_log2)].x);
       }
     }
 #pragma unroll
@@ -1097,7 +1085,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   };
   p.o_sc = take(sizeof(CeScalars));
   p.o_sums = take(fwd ? size_t((a.tokens + kCombRows - 1) / kCombRows) * 16 : 0);
-  p.o_part = take(fwd ? size_t(p.n_tiles) * p.rows_p * 8 : 0);
+  p.o_part = take(fwd ? size_t(p.n_tiles) * a.tokens * 8 : 0);
   p.o_tlogit = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_tdot = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_lse = take(fwd ? size_t(p.rows_p) * 4 : 0);
@@ -1239,6 +1227,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     if (!lse) lse = reinterpret_cast<float *>(ws + p.o_lse);
     if ((s = map_k(&maps.b[0], a.dtype, w, a.vocab, a.dim, wst, p.g1.tn)) != KS_OK) return s;
     g.part = reinterpret_cast<float2 *>(ws + p.o_part);
+    g.parts = int(p.n_tiles);
     g.tlogit = reinterpret_cast<float *>(ws + p.o_tlogit);
     g.tdot = reinterpret_cast<float *>(ws + p.o_tdot);
     g.h = static_cast<const uint16_t *>(h);
@@ -1258,7 +1247,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     if (s != KS_OK) return s;
     const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
     s = ks::launch_kernel(
-        true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, g.part, int(p.n_tiles), p.rows_p, g.tlogit,
+        true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, g.part, g.parts, g.tlogit,
         g.tdot, a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc, int(bwd));
     if (s != KS_OK) return s;
   }
@@ -1275,10 +1264,9 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     const char *wp = static_cast<const char *>(w) + v0 * wst * 2;
     // d of the piece: [tokens, vpad], columns past the vocabulary zero
     if (p.store) {
-      const unsigned rows8 = unsigned((a.tokens + 7) / 8);
-      const unsigned cols = unsigned(std::min<int64_t>((vpad + 1023) / 1024, 65535));
-      s = ks::launch_kernel(true, ce_scale_kernel, dim3(rows8, cols), dim3(256), 0, st, reinterpret_cast<uint16_t *>(d),
-                            vpad, g.part, p.rows_p, p.g1.tn == 256 ? 7 : 6, lse, g.tdot, a.targets, a.tokens, a.vocab,
+      const unsigned cols = unsigned(std::min<int64_t>((vpad + 8191) / 8192, 65535));
+      s = ks::launch_kernel(true, ce_scale_kernel, dim3(unsigned(a.tokens), cols), dim3(256), 0, st,
+                            reinterpret_cast<uint16_t *>(d), vpad, g.part, g.parts, p.g1.tn == 256 ? 7 : 6, lse, g.tdot, a.targets, a.tokens, a.vocab,
                             a.ignore_index, sc, g.f16);
     } else {
       g.side[0] = CeSide{int(a.tokens), int(vpad), kd, 1, kd, -8, 0};
