@@ -33,7 +33,10 @@
 // bf16, 2^-11 in fp16, the size of the outputs' own rounding); the common factor
 // grad_scale / count is left out of d and applied to the fp32 accumulator, so
 // that a target's d, near -1, is near a power of two.  fp16 d is stored times
-// 1024, so that probabilities down to 6e-8 stay normal numbers.  STORE rounds
+// 1024, so that probabilities down to 6e-8 stay normal numbers.  With many
+// tokens the roundings of d average out; with few (kFew), where a row of dw is
+// one or two terms, the residual of every target's d, the largest of its row, is
+// kept in fp32 and its product added to the accumulators.  STORE rounds
 // the exponential too, a second rounding of p (not of the target's d, which is
 // formed from its logit).  The target's logit is taken a second time, as a
 // plain fp32 dot product: the tensor cores' accumulators truncate (a bias of
@@ -56,6 +59,7 @@ constexpr int kThreads = 64 + kEpiWarps * 32;  // producer, MMA, epilogue
 constexpr uint32_t kABox = kBM * kBK * 2;      // 128 rows x 64 K (or two boxes of 64 K x 64 columns): 16 KB
 constexpr uint32_t kBBox = kBK * 64 * 2;       // 64 K-rows x 64 columns: 8 KB
 constexpr uint32_t kCStage = 32 * 128;         // an epilogue warp's staging: 32 rows x 64 columns of 16 bits, or x 32 of 32
+constexpr int kFew = 64;                        // tokens up to which targets' residuals are carried
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kF16Range = 1024.f;            // factor on fp16 d
 constexpr float kF16Exp = 32768.f;             // factor on STORE's fp16 exponentials, which are at most 1
@@ -99,6 +103,8 @@ struct CeGemm {
   int64_t rows_p;
   const float *lse;
   const float *dloss;     // per token, or nullptr
+  int few;                // tokens <= kFew
+  float *lo;              // [kFew] d of the target less its 16-bit value
   CeScalars *sc;
   int out_f32, accumulate;  // dh goes to fp32 slabs, is added to them
   int release;            // another kernel of the call follows
@@ -133,6 +139,14 @@ KS_DEV uint32_t pack2(float lo, float hi, bool f16) {
     return *reinterpret_cast<uint32_t *>(&v);
   }
   return ks_pack_bf16x2(lo, hi);
+}
+
+KS_DEV float round16(float v, bool f16) {
+  return f16 ? __half2float(__float2half_rn(v)) : ks_bf16_to_f32(ks_f32_to_bf16(v));
+}
+
+KS_DEV float value16(uint16_t v, bool f16) {
+  return f16 ? __half2float(__ushort_as_half(v)) : ks_bf16_to_f32(v);
 }
 
 KS_DEV void tma_reduce_add_2d(const CUtensorMap *m, const void *src, int c0, int c1) {
@@ -454,6 +468,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool f16 = p.f16 != 0;
     float scale = 1.f, fscale = 1.f;
     if (kGrads) scale = __ldcg(&p.sc->escale);
+    int64_t few_target[2] = {-1, -1};  // tokens lane and lane + 32
+    if (kGrads && p.few)
+      for (int k = 0; k < 2; ++k)
+        if (k * 32 + lane < p.tokens && p.targets[k * 32 + lane] != p.ignore) few_target[k] = p.targets[k * 32 + lane];
     if (MODE == PROB) fscale = __ldcg(&p.sc->fscale);
     if (MODE == STATS || MODE == STORE) {
       // these warps have nothing else to do until the first tile is complete
@@ -495,6 +513,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (MODE == PROB) lse2[h] = __ldcg(p.lse + row) * kLog2e;
           }
         }
+      }
+      uint32_t mine[MH][2] = {};  // dw: the tokens whose target is this lane's row, few of them
+      if (kGrads && p.few && x.side) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          for (int r = 0; r < 32; ++r) {
+            const int64_t t = __shfl_sync(0xffffffffu, few_target[k], r);
+            if (t < 0) continue;
+#pragma unroll
+            for (int h = 0; h < MH; ++h)
+              if (t == p.v0 + int64_t(tm) * kTM + h * kBM + q * 32 + lane) mine[h][k] |= 1u << r;
+          }
       }
       if (!ks_mbar_wait(tfull + acc, acc_phase, abort, wait)) break;
       ks_tc_fence_after();
@@ -560,7 +590,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (j == tc) r[j] = __float_as_uint(__uint_as_float(r[j]) - fr);
+              if (j == tc) {
+                const float d = __uint_as_float(r[j]) - fr;
+                if (p.few) p.lo[row] = d - round16(d, f16);
+                r[j] = __float_as_uint(d);
+              }
           }
           if (left < 32 || fr == 0.f) {  // columns past the vocabulary, rows without gradient: zeros, whatever the logits
 #pragma unroll
@@ -568,6 +602,24 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (j >= left || fr == 0.f) r[j] = 0u;
           }
         } else if constexpr (kGrads) {
+          if (p.few && x.side) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t own = h == 0 ? mine[0][e] : mine[MH - 1][e];
+              while (__any_sync(0xffffffffu, own != 0)) {  // usually never
+                if (own) {
+                  const int tok = e * 32 + __ffs(own) - 1;
+                  own &= own - 1;
+                  const float lo = __ldcg(p.lo + tok);
+                  const uint16_t *hr = p.h + tok * p.h_stride;
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    if (tn * BN + cb + j < out_n)
+                      r[j] = __float_as_uint(fmaf(lo, value16(__ldcg(hr + tn * BN + cb + j), f16), __uint_as_float(r[j])));
+                }
+              }
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
         }
@@ -743,7 +795,7 @@ __global__ void __launch_bounds__(256)
 __global__ void __launch_bounds__(256)
     ce_scale_kernel(uint16_t *__restrict__ d, int64_t ld, const float2 *__restrict__ part, int tiles, int tile_log2,
                     const float *__restrict__ lse, const float *__restrict__ tdot, const int64_t *__restrict__ targets,
-                    int64_t tokens, int64_t vocab, int64_t ignore, const CeScalars *__restrict__ sc, int f16) {
+                    int64_t tokens, int64_t vocab, int64_t ignore, const CeScalars *__restrict__ sc, int f16, float *lo) {
   const int lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x;
   ks_pdl_release();
@@ -795,6 +847,7 @@ __global__ void __launch_bounds__(256)
         const int64_t at = t - c;
         if (at >= 0 && at < 8) {
           const uint32_t y = pack2(dt, dt, f16 != 0);
+          if (lo) lo[row] = dt - round16(dt, f16 != 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             if (i == at >> 1) x[i] = at & 1 ? (x[i] & 0xffffu) | (y & 0xffff0000u) : (x[i] & 0xffff0000u) | (y & 0xffffu);
@@ -860,11 +913,13 @@ __global__ void __launch_bounds__(1024)
   sc->escale = float(g / f);
 }
 
-// dh = T(escale * sum of the fp32 slabs), slabs added in order.
+// dh = T(escale * sum of the fp32 slabs), slabs added in order; with few tokens
+// the residual of the target's d is added.
 __global__ void __launch_bounds__(256)
     ce_dh_finish_kernel(const float *__restrict__ slabs, int count, int64_t slab_elems, int64_t ld, int64_t rows,
                         int64_t cols, const CeScalars *sc, uint16_t *__restrict__ out, int64_t out_stride, int f16,
-                        int vec) {
+                        int vec, const float *lo, const int64_t *targets, int64_t vocab, int64_t ignore,
+                        const uint16_t *w, int64_t w_stride) {
   ks_pdl_wait();
   const float e = __ldcg(&sc->escale);
   const int64_t cv = (cols + 3) / 4, total = rows * cv;
@@ -879,12 +934,25 @@ __global__ void __launch_bounds__(256)
       a.z += b.z;
       a.w += b.w;
     }
-    const uint32_t lo = pack2(a.x * e, a.y * e, f16 != 0), hi = pack2(a.z * e, a.w * e, f16 != 0);
+    if (lo) {  // few tokens: the target's residual
+      const int64_t t = targets[r];
+      if (t != ignore && t >= 0 && t < vocab) {
+        const float f = __ldcg(lo + r);
+        const uint16_t *wr = w + t * w_stride + c;
+        float v[4];
+        for (int j = 0; j < 4; ++j) v[j] = c + j < cols ? value16(__ldcg(wr + j), f16 != 0) : 0.f;
+        a.x = fmaf(f, v[0], a.x);
+        a.y = fmaf(f, v[1], a.y);
+        a.z = fmaf(f, v[2], a.z);
+        a.w = fmaf(f, v[3], a.w);
+      }
+    }
+    const uint32_t y0 = pack2(a.x * e, a.y * e, f16 != 0), y1 = pack2(a.z * e, a.w * e, f16 != 0);
     uint16_t *o = out + r * out_stride + c;
     if (vec && c + 4 <= cols) {
-      *reinterpret_cast<uint2 *>(o) = make_uint2(lo, hi);
+      *reinterpret_cast<uint2 *>(o) = make_uint2(y0, y1);
     } else {
-      const uint16_t v[4] = {uint16_t(lo), uint16_t(lo >> 16), uint16_t(hi), uint16_t(hi >> 16)};
+      const uint16_t v[4] = {uint16_t(y0), uint16_t(y0 >> 16), uint16_t(y1), uint16_t(y1 >> 16)};
       for (int j = 0; j < 4 && c + j < cols; ++j) o[j] = v[j];
     }
   }
@@ -1023,7 +1091,7 @@ struct Plan {
   bool slabs;            // dh goes through fp32 slabs
   bool store;            // one piece, from STORE's exponentials
   int64_t slab_ld, slab_elems;
-  size_t o_sc, o_sums, o_part, o_tlogit, o_tdot, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
+  size_t o_sc, o_sums, o_part, o_tlogit, o_tdot, o_lo, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
   size_t fixed, bytes;   // bytes: fixed + the piece's d (and padded dw)
 };
 
@@ -1088,6 +1156,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   p.o_part = take(fwd ? size_t(p.n_tiles) * a.tokens * 8 : 0);
   p.o_tlogit = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_tdot = take(fwd ? size_t(p.rows_p) * 4 : 0);
+  p.o_lo = take(bwd ? kFew * 4 : 0);
   p.o_lse = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_h = take(p.pack_h ? size_t(a.tokens) * p.ld * 2 : 0);
   p.o_w = take(p.pack_w ? size_t(a.vocab) * p.ld * 2 : 0);
@@ -1103,7 +1172,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
       p.pieces = (a.vocab + piece - 1) / piece;
       const int64_t cols = std::min(piece, a.vocab);
       p.grads = pick_grads(c, a.tokens, a.dim, (cols + kBK - 1) / kBK, cols, (a.tokens + kBK - 1) / kBK, sms);
-      p.slabs = p.grads.splits > 1 || p.pieces > 1;
+      p.slabs = p.grads.splits > 1 || p.pieces > 1 || a.tokens <= kFew;
       p.slab_ld = up(a.dim, 32);
       p.slab_elems = p.rows_p * p.slab_ld;
       p.o_dh = take(p.pad_dh && !p.slabs ? size_t(a.tokens) * p.ld * 2 : 0);
@@ -1219,6 +1288,13 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   g.rows_p = p.rows_p;
   g.sc = sc;
   g.release = 1;
+  g.h = static_cast<const uint16_t *>(h);
+  g.w = static_cast<const uint16_t *>(w);
+  g.h_stride = hs;
+  g.w_stride = wst;
+  g.dim = a.dim;
+  g.few = a.tokens <= kFew;
+  g.lo = reinterpret_cast<float *>(ws + p.o_lo);
   const int kd = int((a.dim + kBK - 1) / kBK);
   CeMaps maps = {};
   if ((s = map_k(&maps.a[0], a.dtype, h, a.tokens, a.dim, hs, p.g1.tm)) != KS_OK) return s;
@@ -1230,11 +1306,6 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.parts = int(p.n_tiles);
     g.tlogit = reinterpret_cast<float *>(ws + p.o_tlogit);
     g.tdot = reinterpret_cast<float *>(ws + p.o_tdot);
-    g.h = static_cast<const uint16_t *>(h);
-    g.w = static_cast<const uint16_t *>(w);
-    g.h_stride = hs;
-    g.w_stride = wst;
-    g.dim = a.dim;
     // STORE: [tokens, whole tiles], the columns past the vocabulary are -inf logits, zeros
     const int64_t wide = up(a.vocab, 256);
     g.side[0] = CeSide{int(a.tokens), int(p.store ? wide : a.vocab), kd, 1, kd, -8, 0};
@@ -1262,15 +1333,15 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int64_t v0 = i * p.piece, vp = std::min(p.piece, a.vocab - v0), vpad = up(vp, 256);
     const char *wp = static_cast<const char *>(w) + v0 * wst * 2;
+    g.v0 = v0;
     // d of the piece: [tokens, vpad], columns past the vocabulary zero
     if (p.store) {
       const unsigned cols = unsigned(std::min<int64_t>((vpad + 8191) / 8192, 65535));
       s = ks::launch_kernel(true, ce_scale_kernel, dim3(unsigned(a.tokens), cols), dim3(256), 0, st,
                             reinterpret_cast<uint16_t *>(d), vpad, g.part, g.parts, p.g1.tn == 256 ? 7 : 6, lse, g.tdot, a.targets, a.tokens, a.vocab,
-                            a.ignore_index, sc, g.f16);
+                            a.ignore_index, sc, g.f16, g.few ? g.lo : nullptr);
     } else {
       g.side[0] = CeSide{int(a.tokens), int(vpad), kd, 1, kd, -8, 0};
-      g.v0 = v0;
       g.lse = lse;
       g.dloss = a.reduction == KS_CE_NONE ? a.dloss : nullptr;
       if ((s = map_k(&maps.b[0], a.dtype, wp, vp, a.dim, wst, p.g1.tn)) != KS_OK) return s;
@@ -1314,7 +1385,8 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     const int grid = int(std::min<int64_t>((items + 255) / 256, int64_t(ks::sm_count()) * 8));
     const int vec = reinterpret_cast<uintptr_t>(a.dh) % 8 == 0 && a.dh_stride % 4 == 0;
     return ks::launch_kernel(true, ce_dh_finish_kernel, dim3(grid), dim3(256), 0, st, slabs, int(p.grads.splits), p.slab_elems, p.slab_ld,
-                           a.tokens, a.dim, sc, static_cast<uint16_t *>(a.dh), a.dh_stride, int(a.dtype == KS_F16), vec);
+                           a.tokens, a.dim, sc, static_cast<uint16_t *>(a.dh), a.dh_stride, int(a.dtype == KS_F16), vec, g.few ? g.lo : nullptr,
+                             a.targets, a.vocab, a.ignore_index, static_cast<const uint16_t *>(w), wst);
   }
   if (p.pad_dh) return copy2d(true, false, ws + p.o_dh, p.ld, a.dh, a.dh_stride, a.tokens, a.dim, st);
   return KS_OK;

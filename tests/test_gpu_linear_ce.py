@@ -322,6 +322,31 @@ def test_same_bits_every_time_and_on_another_stream(ks):
         assert all(torch.equal(x, y) for x, y in zip(first, got))
 
 
+@pytest.mark.parametrize("piece", [0, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n", [1, 2, 5, 33, 64])
+def test_few_tokens_keep_the_targets_residual(ks, n, dtype, piece):
+    """With few tokens dw's rows are single terms, and the rounding of the target's
+    d would be that of the whole row; its residual is carried, so dh and dw are
+    within their own rounding, at most u / sqrt(3) in the 2-norm where errors are
+    spread evenly within half a unit (0.62 u leaves 7 % for the sample), plus what the other probabilities' two
+    roundings (2 u each, of sum p^2 against the target's (1 - p)^2) and 8 e of fp32
+    add.  Several tokens share a target."""
+    N, ops, torch = ks
+    h, w, t = _make(torch, n, 264, 1500, _dt(torch, dtype), seed=40 + n, lean=3.0)
+    t = torch.where(t == IGNORE, t, t % 7 * 211)
+    t[0] = 211
+    ref = _exact(torch, h, w, t, torch.ones(n, device="cuda"))
+    _, dh, dw = ops.linear_cross_entropy_grad(h, w, t, reduction="sum", cfg=_cfg(N, 0, piece))
+    u = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -11
+    p = ((h.double() @ w.double().t()) - ref["lse"][:, None]).exp()[t != IGNORE]
+    others = p.clone()
+    others[torch.arange(len(p)), t[t != IGNORE]] = 0
+    spread = float(others.norm() / (1 - p[torch.arange(len(p)), t[t != IGNORE]]).norm())
+    for got, want in ((dh, ref["dh"]), (dw, ref["dw"])):
+        assert float((got.double() - want).norm() / want.norm()) <= (0.62 + 3 * spread) * u
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_gradients_against_differences(ks, dtype):
     """Central differences of the kernel's own loss along random +-1 steps of a
