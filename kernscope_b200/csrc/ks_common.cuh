@@ -474,6 +474,11 @@ int symbol_address(const void *symbol, void **out);
 KsWait wait_ctx();
 void set_reason(char *buf, size_t len, const char *fmt, ...);
 
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device.  The
+// runtime is asked once per kernel, device and largest size (defined in
+// runtime.cu).
+int allow_shared(const void *kernel, size_t bytes);
+
 // Launch `kernel`; `next`: as the successor of this call's previous kernel, it
 // may be set up while that one still runs and calls ks_pdl_wait() itself.
 template <typename... P, typename... A>

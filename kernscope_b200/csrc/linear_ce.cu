@@ -1202,8 +1202,8 @@ template <int MODE, int BN, int STAGES, int ACC, int MH>
 int launch(bool next, const CeMaps &maps, CeGemm &g, const Choice *c, cudaStream_t st) {
   using L = Layout<BN, STAGES, ACC, MH>;
   auto kern = ce_gemm_kernel<MODE, BN, STAGES, ACC, MH>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(L::request));
-  if (e != cudaSuccess) return ks::map_cuda(e);
+  const int s = ks::allow_shared(reinterpret_cast<const void *>(kern), L::request);
+  if (s != KS_OK) return s;
   const Tile t{kBM * MH, BN};
   const int64_t items = t.tiles(g.side[0].M, g.side[0].N) * g.side[0].splits;
   const int64_t tiles = MODE == GRADS ? t.tiles(g.side[1].M, g.side[1].N) : 0;

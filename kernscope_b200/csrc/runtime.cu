@@ -123,6 +123,27 @@ int sm_count() {
   return n;
 }
 
+int allow_shared(const void *kernel, size_t bytes) {
+  struct Entry { const void *kernel; int dev; size_t bytes; };
+  static std::vector<Entry> cache;
+  static std::mutex mu;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return map_cuda(e);
+  std::lock_guard<std::mutex> lk(mu);
+  Entry *mine = nullptr;
+  for (Entry &x : cache)
+    if (x.kernel == kernel && x.dev == dev) mine = &x;
+  if (mine != nullptr && mine->bytes >= bytes) return KS_OK;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e != cudaSuccess) return map_cuda(e);
+  if (mine != nullptr)
+    mine->bytes = bytes;
+  else
+    cache.push_back({kernel, dev, bytes});
+  return KS_OK;
+}
+
 void set_reason(char *buf, size_t len, const char *fmt, ...) {
   if (buf == nullptr || len == 0) return;
   va_list ap;

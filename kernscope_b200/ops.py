@@ -466,7 +466,9 @@ class GradClipper:
     gradients go, one tensor of the same type and size each (default: in place).
     The table of work is made once, here, and holds the tensors' addresses: make
     a new clipper when gradients move.  ``clip(max_norm)`` enqueues both passes
-    and returns the norm before clipping (fp32, one value, on the device).
+    and returns the norm before clipping (fp32, one value, on the device).  The
+    partial sums live in the clipper: calls of one clipper must not overlap on
+    the GPU (as calls that scale the same gradients must not).
     """
 
     def __init__(self, grads, out=None):
@@ -499,16 +501,17 @@ class GradClipper:
         need = C.c_size_t(0)
         N.check("ks_grad_clip_workspace_bytes", N.lib.ks_grad_clip_workspace_bytes(chunks.value, C.byref(need)))
         self._table = host.to(self.device)
-        self._need, self._chunks, self._index = need.value, chunks.value, self.device.index
+        self._scratch = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+        self._index = self.device.index
+        self._args = N.GradClipArgs(self._table.data_ptr(), chunks.value, 0.0, 0.0, None, self._scratch.data_ptr(),
+                                    need.value)
 
     def clip(self, max_norm: float, eps: float = 1e-6, stream=None) -> torch.Tensor:
         if self._index != torch.cuda.current_device():
             raise ValueError(f"the gradients are on {self.device}, not on the current device")
-        # the norm in its own small tensor: it may outlive the scratch
-        norm = _empty(self._table, 1, torch.float32, stream)
-        ws = _empty(self._table, self._need, torch.uint8, stream)
-        args = N.GradClipArgs(self._table.data_ptr(), self._chunks, max_norm, eps, norm.data_ptr(), ws.data_ptr(),
-                              self._need)
+        norm = _empty(self._scratch, 1, torch.float32, stream)
+        args = self._args
+        args.max_norm, args.eps, args.norm = max_norm, eps, norm.data_ptr()
         N.check("ks_grad_clip_launch", N.lib.ks_grad_clip_launch(C.byref(args), _raw_stream(stream, self._index)))
         return norm
 
