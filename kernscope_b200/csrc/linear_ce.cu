@@ -35,8 +35,8 @@
 // that a target's d, near -1, is near a power of two.  fp16 d is stored times
 // 1024, so that probabilities down to 6e-8 stay normal numbers.  With many
 // tokens the roundings of d average out; with few (kFew), where a row of dw is
-// one or two terms, the residual of every target's d, the largest of its row, is
-// kept in fp32 and its product added to the accumulators.  STORE rounds
+// one or two terms, d is kept in two 16-bit parts: dw takes the second as one
+// more K-block, dh the residual of its row's target, the largest of d.  STORE rounds
 // the exponential too, a second rounding of p (not of the target's d, which is
 // formed from its logit).  The target's logit is taken a second time, as a
 // plain fp32 dot product: the tensor cores' accumulators truncate (a bias of
@@ -83,6 +83,7 @@ struct CeSide {
 
 struct CeMaps {
   CUtensorMap a[2], b[2], c[2];
+  CUtensorMap a_lo;  // dw of few tokens: the second part of d
 };
 
 struct CeGemm {
@@ -105,6 +106,8 @@ struct CeGemm {
   const float *dloss;     // per token, or nullptr
   int few;                // tokens <= kFew
   float *lo;              // [kFew] d of the target less its 16-bit value
+  uint16_t *d_lo;         // [tokens][d_ld] what the rounding of d left, rounded
+  int64_t d_ld;
   CeScalars *sc;
   int out_f32, accumulate;  // dh goes to fp32 slabs, is added to them
   int release;            // another kernel of the call follows
@@ -356,18 +359,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t *a_dst = smem + L::a_off + stage * L::a_bytes;
         uint8_t *b_dst = smem + L::b_off + stage * L::b_bytes;
         ks_mbar_arrive_expect_tx(full + stage, L::a_bytes + L::b_bytes);
+        const bool second = kGrads && x.side && p.few && kb > 0;  // few tokens: one K-block of d, one of its second part
         if (kGrads && x.side)  // boxes of 64 K-rows x 64 columns, one copy for all of them
-          ks_tma_load_3d(a_dst, ma, full + stage, 0, kb * kBK, x.tm * (kTM / 64));
+          ks_tma_load_3d(a_dst, second ? &maps.a_lo : ma, full + stage, 0, second ? 0 : kb * kBK, x.tm * (kTM / 64));
         else
           ks_tma_load_2d(a_dst, ma, full + stage, kb * kBK, x.tm * kTM);
         if (!kGrads) {
           ks_tma_load_2d(b_dst, mb, full + stage, kb * kBK, x.tn * BN);
         } else if (b3d) {
-          ks_tma_load_3d(b_dst, mb, full + stage, 0, kb * kBK, x.tn * (BN / 64));
+          ks_tma_load_3d(b_dst, mb, full + stage, 0, second ? 0 : kb * kBK, x.tn * (BN / 64));
         } else {
 #pragma unroll
           for (int j = 0; j < BN / 64; ++j)
-            ks_tma_load_2d(b_dst + j * kBBox, mb, full + stage, x.tn * BN + j * 64, kb * kBK);
+            ks_tma_load_2d(b_dst + j * kBBox, mb, full + stage, x.tn * BN + j * 64, second ? 0 : kb * kBK);
         }
         armed |= 1u << stage;
         armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
@@ -468,10 +472,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool f16 = p.f16 != 0;
     float scale = 1.f, fscale = 1.f;
     if (kGrads) scale = __ldcg(&p.sc->escale);
-    int64_t few_target[2] = {-1, -1};  // tokens lane and lane + 32
-    if (kGrads && p.few)
-      for (int k = 0; k < 2; ++k)
-        if (k * 32 + lane < p.tokens && p.targets[k * 32 + lane] != p.ignore) few_target[k] = p.targets[k * 32 + lane];
     if (MODE == PROB) fscale = __ldcg(&p.sc->fscale);
     if (MODE == STATS || MODE == STORE) {
       // these warps have nothing else to do until the first tile is complete
@@ -513,18 +513,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (MODE == PROB) lse2[h] = __ldcg(p.lse + row) * kLog2e;
           }
         }
-      }
-      uint32_t mine[MH][2] = {};  // dw: the tokens whose target is this lane's row, few of them
-      if (kGrads && p.few && x.side) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          for (int r = 0; r < 32; ++r) {
-            const int64_t t = __shfl_sync(0xffffffffu, few_target[k], r);
-            if (t < 0) continue;
-#pragma unroll
-            for (int h = 0; h < MH; ++h)
-              if (t == p.v0 + int64_t(tm) * kTM + h * kBM + q * 32 + lane) mine[h][k] |= 1u << r;
-          }
       }
       if (!ks_mbar_wait(tfull + acc, acc_phase, abort, wait)) break;
       ks_tc_fence_after();
@@ -601,25 +589,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 32; ++j)
               if (j >= left || fr == 0.f) r[j] = 0u;
           }
-        } else if constexpr (kGrads) {
-          if (p.few && x.side) {
+          if (p.few && row < p.tokens && tn * BN + cb < out_n) {
+            // the second part, 64 bytes a lane straight to memory
+            uint4 *line = reinterpret_cast<uint4 *>(p.d_lo + row * p.d_ld + tn * BN + cb);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              uint32_t own = h == 0 ? mine[0][e] : mine[MH - 1][e];
-              while (__any_sync(0xffffffffu, own != 0)) {  // usually never
-                if (own) {
-                  const int tok = e * 32 + __ffs(own) - 1;
-                  own &= own - 1;
-                  const float lo = __ldcg(p.lo + tok);
-                  const uint16_t *hr = p.h + tok * p.h_stride;
+            for (int v = 0; v < 4; ++v) {
+              uint32_t y[4];
 #pragma unroll
-                  for (int j = 0; j < 32; ++j)
-                    if (tn * BN + cb + j < out_n)
-                      r[j] = __float_as_uint(fmaf(lo, value16(__ldcg(hr + tn * BN + cb + j), f16), __uint_as_float(r[j])));
-                }
+              for (int e = 0; e < 4; ++e) {
+                const float a = __uint_as_float(r[v * 8 + e * 2]), b = __uint_as_float(r[v * 8 + e * 2 + 1]);
+                y[e] = pack2(a - round16(a, f16), b - round16(b, f16), f16);
               }
+              line[v] = make_uint4(y[0], y[1], y[2], y[3]);
             }
           }
+        } else if constexpr (kGrads) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
         }
@@ -687,85 +671,85 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // lse and loss of every row from the tiles' (max, sum); the last block adds up
 // the loss over the rows, in a fixed order, and leaves the gradient's scalars.
-// A warp per row, eight rows per block.
 // ---------------------------------------------------------------------------
 constexpr int kCombRows = 8;
 
-__global__ void __launch_bounds__(256)
-    ce_combine_kernel(const float2 *__restrict__ part, int tiles, const float *__restrict__ tlogit,
-                      const float *__restrict__ tdot, const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab,
-                      int64_t ignore, int reduction, float grad_scale, const float *dloss, float range,
-                      float *__restrict__ loss, float *__restrict__ lse_out, double2 *__restrict__ sums, CeScalars *sc,
-                      int release) {
-  __shared__ double shl[kCombRows], shn[kCombRows];
-  __shared__ bool is_last;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (release) ks_pdl_release();
-  ks_pdl_wait();
-  const int64_t row = int64_t(blockIdx.x) * kCombRows + warp;
-  double l = 0.0, n = 0.0;
-  if (row < tokens) {
-    // the row's own values, loaded beside the partial sums
-    const int64_t t = targets[row];
-    const float lt = __ldcg(tdot + row), old = __ldcg(tlogit + row);
-    float m = -INFINITY, s = 0.f;
-    auto add = [&](float m2, float s2) {  // (m, s) (+) (m2, s2); a side with no finite maximum adds its sum as it is
-      const float mn = fmaxf(m, m2);
-      if (mn == -INFINITY) {
-        s += s2;  // zeros, or the NaN of a row that has one
-      } else {
-        s = s * ex2((m - mn) * kLog2e) + s2 * ex2((m2 - mn) * kLog2e);
-      }
-      m = mn;
-    };
+struct Combine {
+  const float2 *part;  // [tokens][tiles]
+  int tiles;
+  const float *tlogit, *tdot;
+  const int64_t *targets;
+  int64_t tokens, vocab, ignore;
+  int reduction;
+  float grad_scale;
+  const float *dloss;
+  float range;
+  float *loss, *lse;
+  double2 *sums;  // per block (loss, tokens that count)
+  CeScalars *sc;
+};
+
+struct RowStats {
+  int64_t target;
+  bool valid;  // a target in the vocabulary
+  float tdot, lse;
+  float loss;
+  bool counts;
+};
+
+// One row by one warp; every lane has the result.
+KS_DEV RowStats row_stats(const Combine &a, int64_t row, int lane) {
+  RowStats r;
+  // the row's own values, loaded beside the partial sums
+  r.target = a.targets[row];
+  r.tdot = __ldcg(a.tdot + row);
+  const float old = __ldcg(a.tlogit + row);
+  float m = -INFINITY, s = 0.f;
+  auto add = [&](float m2, float s2) {  // (m, s) (+) (m2, s2); a side with no finite maximum adds its sum as it is
+    const float mn = fmaxf(m, m2);
+    if (mn == -INFINITY) {
+      s += s2;  // zeros, or the NaN of a row that has one
+    } else {
+      s = s * ex2((m - mn) * kLog2e) + s2 * ex2((m2 - mn) * kLog2e);
+    }
+    m = mn;
+  };
 #pragma unroll 4
-    for (int i = lane; i < tiles; i += 32) {
-      const float2 v = __ldcg(part + row * tiles + i);
-      add(v.x, v.y);
-    }
+  for (int i = lane; i < a.tiles; i += 32) {
+    const float2 v = __ldcg(a.part + row * a.tiles + i);
+    add(v.x, v.y);
+  }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
-      add(m2, s2);
-    }
-    const bool valid = t != ignore && t >= 0 && t < vocab;
-    // the target's logit as the dot product, in the sum too
-    if (valid && isfinite(lt) && isfinite(old)) s += ex2((lt - m) * kLog2e) - ex2((old - m) * kLog2e);
-    const float lse = m + logf(s);  // -inf + log 0: a row of -inf logits
-    float v = 0.f;
-    if (t != ignore) {
-      v = valid ? lse - lt : __int_as_float(0x7fc00000);
-      n = 1.0;
-    }
-    if (lane == 0) {
-      lse_out[row] = lse;
-      if (reduction == KS_CE_NONE && loss) loss[row] = v;
-    }
-    l = v;
+  for (int o = 1; o < 32; o <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    add(m2, s2);
   }
-  if (lane == 0) {
-    shl[warp] = l;
-    shn[warp] = n;
-  }
-  if (reduction == KS_CE_NONE) return;
-  __syncthreads();
+  r.valid = r.target != a.ignore && r.target >= 0 && r.target < a.vocab;
+  // the target's logit as the dot product, in the sum too
+  if (r.valid && isfinite(r.tdot) && isfinite(old)) s += ex2((r.tdot - m) * kLog2e) - ex2((old - m) * kLog2e);
+  r.lse = m + logf(s);  // -inf + log 0: a row of -inf logits
+  r.counts = r.target != a.ignore;
+  r.loss = !r.counts ? 0.f : r.valid ? r.lse - r.tdot : __int_as_float(0x7fc00000);
+  return r;
+}
+
+// Block `block` of `blocks` (256 threads) has the sums (l, n), known to thread 0;
+// the last to arrive adds them all up.
+KS_DEV void reduce_loss(const Combine &a, double l, double n, unsigned block, unsigned blocks) {
+  __shared__ bool is_last;
+  __shared__ double wl[8], wn[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
-    l = n = 0.0;
-    for (int j = 0; j < kCombRows; ++j) {
-      l += shl[j];
-      n += shn[j];
-    }
-    sums[blockIdx.x] = make_double2(l, n);
+    a.sums[block] = make_double2(l, n);
     __threadfence();
-    is_last = gridDim.x == 1 || atomicAdd(&sc->counter, 1u) == gridDim.x - 1;
+    is_last = blocks == 1 || atomicAdd(&a.sc->counter, 1u) == blocks - 1;
   }
   __syncthreads();
   if (!is_last) return;
   __threadfence();
-  __shared__ double wl[8], wn[8];
   l = n = 0.0;
-  for (unsigned j = tid; j < gridDim.x; j += 256) {
-    const double2 v = __ldcg(sums + j);
+  for (unsigned j = tid; j < blocks; j += 256) {
+    const double2 v = __ldcg(a.sums + j);
     l += v.x;
     n += v.y;
   }
@@ -782,30 +766,84 @@ __global__ void __launch_bounds__(256)
       l += wl[j];
       n += wn[j];
     }
-    const double c = reduction == KS_CE_MEAN ? (n > 0.0 ? n : 1.0) : 1.0;
-    if (loss) loss[0] = float(l / c);
-    sc->fscale = range;
-    sc->escale = float(double(grad_scale) * (dloss ? double(dloss[0]) : 1.0) / c / double(range));
+    const double c = a.reduction == KS_CE_MEAN ? (n > 0.0 ? n : 1.0) : 1.0;
+    if (a.loss) a.loss[0] = float(l / c);
+    a.sc->fscale = a.range;
+    a.sc->escale = float(double(a.grad_scale) * (a.dloss ? double(a.dloss[0]) : 1.0) / c / double(a.range));
   }
+}
+
+// A warp per row, eight rows per block.
+__global__ void __launch_bounds__(256) ce_combine_kernel(const __grid_constant__ Combine a, int release) {
+  __shared__ double shl[kCombRows], shn[kCombRows];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (release) ks_pdl_release();
+  ks_pdl_wait();
+  const int64_t row = int64_t(blockIdx.x) * kCombRows + warp;
+  double l = 0.0, n = 0.0;
+  if (row < a.tokens) {
+    const RowStats r = row_stats(a, row, lane);
+    if (lane == 0) {
+      a.lse[row] = r.lse;
+      if (a.reduction == KS_CE_NONE && a.loss) a.loss[row] = r.loss;
+    }
+    l = r.loss;
+    n = r.counts;
+  }
+  if (lane == 0) {
+    shl[warp] = l;
+    shn[warp] = n;
+  }
+  if (a.reduction == KS_CE_NONE) return;
+  __syncthreads();
+  l = n = 0.0;
+  if (tid == 0)
+    for (int j = 0; j < kCombRows; ++j) {
+      l += shl[j];
+      n += shn[j];
+    }
+  reduce_loss(a, l, n, blockIdx.x, gridDim.x);
 }
 
 // STORE's exponentials e -> d in place: d = f (e exp(tile maximum - lse) -
 // [target]).  A CTA takes 8192 columns of one row, 16 KB, a warp 1024 of them,
 // four 16-byte loads a lane in flight.  Reads and writes 2 bytes a value.
+// COMBINE: up to kCombineRows tokens every warp takes its row's lse from the
+// tiles itself, and the combine kernel is left out (333 x 1000 x 10007: 54 -> 50
+// us for the whole call; with many rows the repeated reads cost more).
+constexpr int kCombineRows = 512;
+
+template <bool COMBINE>
 __global__ void __launch_bounds__(256)
-    ce_scale_kernel(uint16_t *__restrict__ d, int64_t ld, const float2 *__restrict__ part, int tiles, int tile_log2,
-                    const float *__restrict__ lse, const float *__restrict__ tdot, const int64_t *__restrict__ targets,
-                    int64_t tokens, int64_t vocab, int64_t ignore, const CeScalars *__restrict__ sc, int f16, float *lo) {
+    ce_scale_kernel(const __grid_constant__ Combine a, uint16_t *__restrict__ d, int64_t ld, int tile_log2, int f16,
+                    float *lo, uint16_t *d_lo) {
   const int lane = threadIdx.x & 31;
   const int64_t row = blockIdx.x;
   ks_pdl_release();
   ks_pdl_wait();
-  const int64_t t = targets[row];
-  const bool valid = t != ignore && t >= 0 && t < vocab;
-  const float f = valid ? __ldcg(&sc->fscale) : 0.f, fe = f16 ? f / kF16Exp : f;
-  const float l2 = __ldcg(lse + row) * kLog2e;
+  const int64_t vocab = a.vocab;
+  int64_t t;
+  bool valid;
+  float l2, tdot;
+  if (COMBINE) {
+    const RowStats r = row_stats(a, row, lane);
+    t = r.target;
+    valid = r.valid;
+    l2 = r.lse * kLog2e;
+    tdot = r.tdot;
+    if (blockIdx.y == 0) {
+      if (threadIdx.x == 0) a.lse[row] = r.lse;
+      reduce_loss(a, r.loss, r.counts, unsigned(row), gridDim.x);
+    }
+  } else {
+    t = a.targets[row];
+    valid = t != a.ignore && t >= 0 && t < vocab;
+    l2 = __ldcg(a.lse + row) * kLog2e;
+    tdot = __ldcg(a.tdot + row);
+  }
+  const float f = valid ? a.range : 0.f, fe = f16 ? f / kF16Exp : f;
   uint16_t *dr = d + row * ld;
-  const float dt = valid ? f * ex2(fmaf(__ldcg(tdot + row), kLog2e, -l2)) - f : 0.f;
+  const float dt = valid ? f * ex2(fmaf(tdot, kLog2e, -l2)) - f : 0.f;
   constexpr int step = 256;
   // the last columns first: STORE wrote them last, so they are still in L2, and the
   // first columns, where the products begin, are left there
@@ -820,48 +858,52 @@ __global__ void __launch_bounds__(256)
       k[j] = 0.f;
       if (c < ld && valid) {
         v[j] = __ldcg(reinterpret_cast<const uint4 *>(dr + c));
-        if (c < vocab) k[j] = __ldcg(&part[row * tiles + (c >> tile_log2)].x);
+        if (c < vocab) k[j] = __ldcg(&a.part[row * a.tiles + (c >> tile_log2)].x);
       }
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int64_t c = c0 + j * step;
       if (c >= ld) continue;
-      uint4 o = make_uint4(0, 0, 0, 0);
+      uint4 o = make_uint4(0, 0, 0, 0), rest = o;
       if (valid) {
         const float g = k[j] == -INFINITY ? 0.f : fe * ex2(fmaf(k[j], kLog2e, -l2));  // a tile of -inf logits holds zeros
-        uint32_t x[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+        const uint32_t x[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+        float y[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float lo, hi;
           if (f16) {
-            const __half2 y = *reinterpret_cast<const __half2 *>(&x[i]);
-            lo = __low2float(y);
-            hi = __high2float(y);
+            const __half2 z = *reinterpret_cast<const __half2 *>(&x[i]);
+            y[2 * i] = __low2float(z) * g;
+            y[2 * i + 1] = __high2float(z) * g;
           } else {
-            lo = ks_bf16_lo(x[i]);
-            hi = ks_bf16_hi(x[i]);
+            y[2 * i] = ks_bf16_lo(x[i]) * g;
+            y[2 * i + 1] = ks_bf16_hi(x[i]) * g;
           }
-          x[i] = pack2(lo * g, hi * g, f16 != 0);
         }
         const int64_t at = t - c;
         if (at >= 0 && at < 8) {
-          const uint32_t y = pack2(dt, dt, f16 != 0);
-          if (lo) lo[row] = dt - round16(dt, f16 != 0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i == at >> 1) x[i] = at & 1 ? (x[i] & 0xffffu) | (y & 0xffff0000u) : (x[i] & 0xffff0000u) | (y & 0xffffu);
+          for (int i = 0; i < 8; ++i)
+            if (i == at) y[i] = dt;
+          if (lo) lo[row] = dt - round16(dt, f16 != 0);
         }
         if (c + 8 > vocab) {  // columns past the vocabulary
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (c + 2 * i >= vocab) x[i] = 0;
-            else if (c + 2 * i + 1 >= vocab) x[i] &= 0xffffu;
-          }
+          for (int i = 0; i < 8; ++i)
+            if (c + i >= vocab) y[i] = 0.f;
         }
-        o = make_uint4(x[0], x[1], x[2], x[3]);
+        o = make_uint4(pack2(y[0], y[1], f16 != 0), pack2(y[2], y[3], f16 != 0), pack2(y[4], y[5], f16 != 0),
+                       pack2(y[6], y[7], f16 != 0));
+        if (d_lo) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] -= round16(y[i], f16 != 0);
+          rest = make_uint4(pack2(y[0], y[1], f16 != 0), pack2(y[2], y[3], f16 != 0), pack2(y[4], y[5], f16 != 0),
+                            pack2(y[6], y[7], f16 != 0));
+        }
       }
       *reinterpret_cast<uint4 *>(dr + c) = o;
+      if (d_lo) *reinterpret_cast<uint4 *>(d_lo + row * ld + c) = rest;
     }
   }
 }
@@ -998,16 +1040,17 @@ struct Tile {
   int64_t tiles(int64_t m, int64_t n) const { return ((m + tm - 1) / tm) * ((n + tn - 1) / tn); }
 };
 
-// What a tile costs, microseconds, measured: one K-block on one SM, and what a
-// tile's epilogue adds where the MMAs cannot run beside it.  The logits'
-// epilogue (exponentials) is the long one: 4096 x 1024 x 65536 scores took 467
-// us in 256 x 256 tiles, 402 in 128 x 256, 724 in 128 x 128; at dim 4096 the
-// large tile's smaller operand traffic wins.
+// What a tile costs, microseconds, measured under the power cap: one K-block on
+// one SM, and what a tile's epilogue adds where the MMAs cannot run beside it.
+// The logits' epilogue (exponentials) is the long one: scores of 8192 x 512 x
+// 65536 take 529 us in 256 x 256 tiles and 479 in 128 x 256; at dim 1024 the two
+// are equal, and from dim 2048 the large tile's smaller operand traffic wins (4096
+// x 2048 x 65536: 848 against 890 us, beside 846 of the library's plain product).
 struct Cost {
   Tile tile;
   double kb, tail;
 };
-constexpr Cost kLogitCosts[] = {{{256, 256}, 0.77, 3.8}, {{128, 256}, 0.43, 0.3}, {{128, 128}, 0.36, 0.5}};
+constexpr Cost kLogitCosts[] = {{{256, 256}, 0.80, 2.0}, {{128, 256}, 0.46, 0.2}, {{128, 128}, 0.36, 0.5}};
 constexpr Cost kProductCosts[] = {{{256, 256}, 0.74, 1.5}, {{128, 256}, 0.41, 0.5}, {{128, 128}, 0.29, 0.4}};
 constexpr double kSlabBytesPerUs = 5e6;  // an fp32 slab is written once and read once
 
@@ -1091,6 +1134,7 @@ struct Plan {
   bool slabs;            // dh goes through fp32 slabs
   bool store;            // one piece, from STORE's exponentials
   int64_t slab_ld, slab_elems;
+  size_t o_d_lo;         // few tokens: the second part of d
   size_t o_sc, o_sums, o_part, o_tlogit, o_tdot, o_lo, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
   size_t fixed, bytes;   // bytes: fixed + the piece's d (and padded dw)
 };
@@ -1152,7 +1196,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
     return at;
   };
   p.o_sc = take(sizeof(CeScalars));
-  p.o_sums = take(fwd ? size_t((a.tokens + kCombRows - 1) / kCombRows) * 16 : 0);
+  p.o_sums = take(fwd ? size_t(std::max<int64_t>((a.tokens + kCombRows - 1) / kCombRows, std::min<int64_t>(a.tokens, kCombineRows))) * 16 : 0);
   p.o_part = take(fwd ? size_t(p.n_tiles) * a.tokens * 8 : 0);
   p.o_tlogit = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_tdot = take(fwd ? size_t(p.rows_p) * 4 : 0);
@@ -1162,10 +1206,11 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   p.o_w = take(p.pack_w ? size_t(a.vocab) * p.ld * 2 : 0);
   p.slabs = p.store = false;
   p.piece = p.pieces = 0;
-  p.o_dh = p.o_slab = p.o_dw = p.o_d = o;
+  p.o_dh = p.o_slab = p.o_dw = p.o_d = p.o_d_lo = o;
   if (bwd) {
     const int64_t whole = up(a.vocab, 256);
-    const size_t per_col = size_t(a.tokens) * 2 + (p.pad_dw ? size_t(p.ld) * 2 : 0);
+    const bool few = a.tokens <= kFew;
+    const size_t per_col = size_t(a.tokens) * (few ? 4 : 2) + (p.pad_dw ? size_t(p.ld) * 2 : 0);
     auto lay = [&](int64_t piece, size_t from) {
       o = from;
       p.piece = piece;
@@ -1180,6 +1225,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
       p.fixed = o;
       p.o_dw = take(p.pad_dw ? size_t(std::min(piece, a.vocab)) * p.ld * 2 : 0);
       p.o_d = take(size_t(a.tokens) * piece * 2);
+      p.o_d_lo = take(few ? size_t(a.tokens) * piece * 2 : 0);
       p.bytes = o;
     };
     const size_t from = o;
@@ -1299,6 +1345,8 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   CeMaps maps = {};
   if ((s = map_k(&maps.a[0], a.dtype, h, a.tokens, a.dim, hs, p.g1.tm)) != KS_OK) return s;
   float *lse = a.lse;
+  Combine comb = {};
+  const bool combine_in_scale = p.store && a.tokens <= kCombineRows;
   if (fwd) {
     if (!lse) lse = reinterpret_cast<float *>(ws + p.o_lse);
     if ((s = map_k(&maps.b[0], a.dtype, w, a.vocab, a.dim, wst, p.g1.tn)) != KS_OK) return s;
@@ -1316,11 +1364,13 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
       s = launch_tile<STATS>(next, p.g1, maps, g, nullptr, st);
     }
     if (s != KS_OK) return s;
-    const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
-    s = ks::launch_kernel(
-        true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, g.part, g.parts, g.tlogit,
-        g.tdot, a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction, a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc, int(bwd));
-    if (s != KS_OK) return s;
+    comb = Combine{g.part, g.parts, g.tlogit, g.tdot, a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction,
+                   a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc};
+    if (!combine_in_scale) {
+      const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
+      s = ks::launch_kernel(true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, comb, int(bwd));
+      if (s != KS_OK) return s;
+    }
   }
   if (!bwd) return KS_OK;
   if (!fwd) {
@@ -1334,12 +1384,14 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     const int64_t v0 = i * p.piece, vp = std::min(p.piece, a.vocab - v0), vpad = up(vp, 256);
     const char *wp = static_cast<const char *>(w) + v0 * wst * 2;
     g.v0 = v0;
+    g.d_lo = reinterpret_cast<uint16_t *>(ws + p.o_d_lo);
+    g.d_ld = vpad;
     // d of the piece: [tokens, vpad], columns past the vocabulary zero
     if (p.store) {
       const unsigned cols = unsigned(std::min<int64_t>((vpad + 8191) / 8192, 65535));
-      s = ks::launch_kernel(true, ce_scale_kernel, dim3(unsigned(a.tokens), cols), dim3(256), 0, st,
-                            reinterpret_cast<uint16_t *>(d), vpad, g.part, g.parts, p.g1.tn == 256 ? 7 : 6, lse, g.tdot, a.targets, a.tokens, a.vocab,
-                            a.ignore_index, sc, g.f16, g.few ? g.lo : nullptr);
+      s = ks::launch_kernel(true, combine_in_scale ? ce_scale_kernel<true> : ce_scale_kernel<false>,
+                            dim3(unsigned(a.tokens), cols), dim3(256), 0, st, comb, reinterpret_cast<uint16_t *>(d), vpad,
+                            p.g1.tn == 256 ? 7 : 6, g.f16, g.few ? g.lo : nullptr, g.few ? g.d_lo : nullptr);
     } else {
       g.side[0] = CeSide{int(a.tokens), int(vpad), kd, 1, kd, -8, 0};
       g.lse = lse;
@@ -1353,9 +1405,11 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     const Tile t = p.grads.tile;
     CeMaps mg = {};
     const int kv = int((vp + kBK - 1) / kBK), kt = int((a.tokens + kBK - 1) / kBK), per = int(p.grads.kb_split);
-    g.side[0] = CeSide{int(a.tokens), int(a.dim), kv, (kv + per - 1) / per, per, 8, 0};
+    g.side[0] = CeSide{int(a.tokens), int(a.dim), kv, (kv + per - 1) / per, per, -16, 0};
     // dw: the column tiles of a block of rows side by side, so that whole rows are written at about one time
-    g.side[1] = CeSide{int(vp), int(a.dim), kt, 1, kt, -16, 0};
+    const int kd2 = g.few ? 2 : kt;  // few tokens: d and its second part, a K-block each
+    g.side[1] = CeSide{int(vp), int(a.dim), kd2, 1, kd2, -16, 0};
+    static_assert(kFew <= kBK, "few tokens are one K-block");
     if ((s = map_k(&mg.a[0], a.dtype, d, a.tokens, vp, vpad, t.tm)) != KS_OK) return s;
     if ((s = map_mn(&mg.b[0], a.dtype, wp, vp, a.dim, wst, t.tn, &g.side[0].b3d)) != KS_OK) return s;
     if (p.slabs)
@@ -1368,6 +1422,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     int a3d = 0;
     if ((s = map_mn(&mg.a[1], a.dtype, d, a.tokens, vpad, vpad, t.tm, &a3d)) != KS_OK) return s;
     if (!a3d) return KS_ERR_OTHER;
+    if (g.few && (s = map_mn(&mg.a_lo, a.dtype, g.d_lo, a.tokens, vpad, vpad, t.tm, &a3d)) != KS_OK) return s;
     if ((s = map_mn(&mg.b[1], a.dtype, h, a.tokens, a.dim, hs, t.tn, &g.side[1].b3d)) != KS_OK) return s;
     char *dwp = static_cast<char *>(a.dw) + v0 * a.dw_stride * 2;
     if ((s = map_out(&mg.c[1], a.dtype, p.pad_dw ? ws + p.o_dw : dwp, vp, a.dim, p.pad_dw ? p.ld : a.dw_stride)) != KS_OK)
