@@ -416,10 +416,10 @@ struct Sum {
   }
 };
 
-constexpr int64_t kGroup = 64;  // chunks whose partials one CTA adds up
+constexpr int64_t kGroup = 32;  // chunks whose partials one CTA adds up
 
 // A token that lies in chunks a to b, of which this CTA has left a partial sum.
-// The last of the CTAs that hold a part of it, within each group of 64 chunks,
+// The last of the CTAs that hold a part of it, within each group of 32 chunks,
 // adds the group's partials in order; the last group adds the groups'.  So the
 // order of the sum is that of the chunks, whoever comes last, and a token that
 // fills the whole batch is joined in two short chains.  (A kernel of its own
@@ -446,7 +446,7 @@ KS_DEV void join(const GradArgs<DT, ODT> &g, const Part &t, int64_t ch, int64_t 
   const int64_t first = max(a, ch / kGroup * kGroup), last = min(b, ch / kGroup * kGroup + kGroup - 1);
   S sum;
   sum.clear();
-#pragma unroll 4
+#pragma unroll 8
   for (int64_t j = first; j <= last; ++j) sum.add_part(slot(j), c, g.dim);
   const int64_t ga = a / kGroup, gb = b / kGroup;
   if (ga != gb) {
@@ -459,7 +459,7 @@ KS_DEV void join(const GradArgs<DT, ODT> &g, const Part &t, int64_t ch, int64_t 
     if (!last_group) return;
     __threadfence();
     sum.clear();
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t j = ga; j <= gb; ++j) sum.add_part(slot(max(a, j * kGroup)), c, g.dim);
   }
   sum.finish(g.dtable + int64_t(t.key) * g.dtable_stride, c, g.dim, g.scale, g.accumulate != 0);
