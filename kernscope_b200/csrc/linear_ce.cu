@@ -241,29 +241,6 @@ KS_DEV void wait_loaded(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
-// Maximum over COLS columns of this lane's accumulator row, `left` of them
-// inside the vocabulary.
-template <int COLS>
-KS_DEV float cols_max(uint32_t t_addr, int64_t left) {
-  static_assert(COLS % 64 == 0, "pairs of blocks");
-  float m = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < COLS; c += 64) {
-    uint32_t r[2][32];
-    ks_tmem_ld32(t_addr + c, r[0]);
-    ks_tmem_ld32(t_addr + c + 32, r[1]);
-    wait_loaded(r[0]);
-    wait_loaded(r[1]);
-    if (left - c < 64) {
-#pragma unroll
-      for (int j = 0; j < 64; ++j)
-        if (j >= left - c) r[j / 32][j % 32] = __float_as_uint(-INFINITY);
-    }
-    m = fmaxf(m, fmaxf(max32(r[0]), max32(r[1])));
-  }
-  return m;
-}
-
 // <h[row], w[t]> in fp32 by one warp.
 KS_DEV float target_dot(const uint16_t *h, const uint16_t *w, int64_t dim, bool f16, int lane) {
   auto val = [&](uint32_t v, int hi) {
@@ -518,16 +495,93 @@ __global__ void __launch_bounds__(kThreads, 1)
       ks_tc_fence_after();
       const uint32_t t_addr = tmem_base + (uint32_t(q * 32) << 16) + acc * BN * MH + cg;
       const int64_t col0 = p.v0 + int64_t(tn) * BN;  // first vocabulary column of the tile (STATS, STORE, PROB)
-      float m = -INFINITY, s = 0.f;
+      if constexpr (MODE == STATS || MODE == STORE) {
+        // A half's columns go into registers at once and the accumulator is free:
+        // the next tile's MMAs run while the exponentials are taken (256 x 256 tiles
+        // of 4096 x 2048 x 32768: the tensor pipe was 72 % busy when each 32-column
+        // block was loaded as it was worked on, and the maximum read them twice).
+#pragma unroll 1
+        for (int h = 0; h < MH; ++h) {
+          uint32_t r[kBlocks][32];
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k) ks_tmem_ld32(t_addr + h * BN + k * 32, r[k]);
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k) wait_loaded(r[k]);
+          ks_tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ks_mbar_arrive(tempty + acc * MH + h);
+          const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
+          const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cg;  // the target inside this warp's columns
+          if (__any_sync(0xffffffffu, tc >= 0 && tc < kCols)) {
+            float v = 0.f;
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (k * 32 + j == tc) v = __uint_as_float(r[k][j]);
+            if (tc >= 0 && tc < kCols) p.tlogit[row] = v;
+          }
+          const int64_t left = p.vocab - (col0 + cg);  // columns inside the vocabulary
+          if (left < kCols) {
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k)
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (k * 32 + j >= left) r[k][j] = __float_as_uint(-INFINITY);
+          }
+          float m = max32(r[0]);
+#pragma unroll
+          for (int k = 1; k < kBlocks; ++k) m = fmaxf(m, max32(r[k]));
+          // an all -inf row: exponentials against 0 are 0, not NaN
+          const float base = m == -INFINITY || m != m ? 0.f : m * kLog2e;
+          float a4[4] = {0.f, 0.f, 0.f, 0.f};
+          uint8_t *line = stg + lane * 128;
+          const int64_t r0 = int64_t(tm) * kTM + h * kBM + q * 32;
+#pragma unroll
+          for (int k = 0; k < kBlocks; ++k) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float x = ex2(fmaf(__uint_as_float(r[k][j]), kLog2e, -base));
+              a4[j & 3] += x;
+              if (MODE == STORE) r[k][j] = __float_as_uint(f16 ? x * kF16Exp : x);
+            }
+            if constexpr (MODE == STORE) {
+              // two blocks side by side fill the staging's 128-byte rows (row =
+              // lane, 128-byte swizzle: 16-byte chunk v at position v ^ (lane & 7))
+              if (k % 2 == 0) {
+                if (lane == 0) ks_bulk_wait_read<0>();  // the last store has read the staging
+                __syncwarp();
+              }
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                uint4 y;
+                y.x = pack2(__uint_as_float(r[k][v * 8 + 0]), __uint_as_float(r[k][v * 8 + 1]), f16);
+                y.y = pack2(__uint_as_float(r[k][v * 8 + 2]), __uint_as_float(r[k][v * 8 + 3]), f16);
+                y.z = pack2(__uint_as_float(r[k][v * 8 + 4]), __uint_as_float(r[k][v * 8 + 5]), f16);
+                y.w = pack2(__uint_as_float(r[k][v * 8 + 6]), __uint_as_float(r[k][v * 8 + 7]), f16);
+                *reinterpret_cast<uint4 *>(line + (((v + k % 2 * 4) ^ (lane & 7)) * 16)) = y;
+              }
+              if (k % 2 == 1) {
+                const int c0 = tn * BN + cg + (k - 1) * 32;
+                ks_fence_proxy_async();
+                __syncwarp();
+                if (lane == 0 && c0 < out_n && r0 < out_m) {  // blocks past the edge hold nothing
+                  ks_tma_store_2d(&maps.c[0], stg, c0, int(r0));
+                  ks_bulk_commit_group();
+                }
+              }
+            }
+          }
+          if (row < p.tokens)
+            p.part[row * p.parts + tn * 2 + cg / kCols] = make_float2(m, (a4[0] + a4[1]) + (a4[2] + a4[3]));
+        }
+        continue;
+      }
       // block k: half k / kBlocks, columns cg + k % kBlocks * 32.  `next` is loaded while `r` is worked on.
       auto step = [&](int k, uint32_t (&r)[32], uint32_t (&next)[32]) {
         const int h = k / kBlocks, cb = cg + k % kBlocks * 32;
         wait_loaded(r);
         if (k + 1 < MH * kBlocks) ks_tmem_ld32(t_addr + (k + 1) / kBlocks * BN + (k + 1) % kBlocks * 32, next);
-        if ((MODE == STATS || MODE == STORE) && k % kBlocks == 0) {
-          s = 0.f;
-          m = MODE == STORE ? cols_max<kCols>(t_addr + h * BN, p.vocab - col0 - cg) : -INFINITY;
-        }
         if ((k + 1) % kBlocks == 0) {  // this warp's part of the half is in registers
           ks_tc_fence_before();
           __syncwarp();
@@ -536,41 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t row = int64_t(tm) * kTM + h * kBM + q * 32 + lane;
         const int tc = (h == 0 ? tcol[0] : tcol[MH - 1]) - cb;  // the target inside the block
         const int64_t left = p.vocab - (col0 + cb);             // columns of the block inside the vocabulary
-        if constexpr (MODE == STATS || MODE == STORE) {
-          if (__any_sync(0xffffffffu, tc >= 0 && tc < 32)) {
-            float v = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j == tc) v = __uint_as_float(r[j]);
-            if (tc >= 0 && tc < 32) p.tlogit[row] = v;
-          }
-          if (left < 32) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (j >= left) r[j] = __float_as_uint(-INFINITY);
-          }
-          const float mn = MODE == STORE ? m : fmaxf(m, max32(r));
-          // an all -inf row so far: exponentials against 0 are 0, not NaN
-          const float base = mn == -INFINITY ? 0.f : mn * kLog2e;
-          float a4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float x = ex2(fmaf(__uint_as_float(r[j]), kLog2e, -base));
-            a4[j & 3] += x;
-            if (MODE == STORE) r[j] = __float_as_uint(x);
-          }
-          if (MODE == STATS) s *= ex2(fmaf(m, kLog2e, -base));
-          s += (a4[0] + a4[1]) + (a4[2] + a4[3]);
-          m = mn;
-          if ((k + 1) % kBlocks == 0 && row < p.tokens)
-            p.part[row * p.parts + tn * 2 + cg / kCols] = make_float2(m, s);
-        }
-        if constexpr (MODE == STORE) {
-          if (f16) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * kF16Exp);
-          }
-        } else if constexpr (MODE == PROB) {
+        if constexpr (MODE == PROB) {
           const float fr = h == 0 ? f[0] : f[MH - 1];
           const float l2 = h == 0 ? lse2[0] : lse2[MH - 1];
 #pragma unroll
@@ -607,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * escale);
         }
-        if constexpr (MODE != STATS) {
+        {
           // 16 bits: two blocks side by side fill the staging's 128-byte rows, the
           // second one stores both.  (32-column stores, 64 bytes a row, wrote dw of
           // 16 tokens x 1024 x 32000 at 3 TB/s.)
