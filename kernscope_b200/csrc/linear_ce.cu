@@ -39,9 +39,16 @@
 // more K-block, dh the residual of its row's target, the largest of d.  STORE rounds
 // the exponential too, a second rounding of p (not of the target's d, which is
 // formed from its logit).  The target's logit is taken a second time, as a
-// plain fp32 dot product: the tensor cores' accumulators truncate (a bias of
-// about 4e-6 of a logit at dim 2048), which the sum over the vocabulary
-// averages out but a loss of one large logit would show.
+// plain fp32 dot product: the tensor cores' accumulators truncate, which the sum
+// over the vocabulary averages out but a loss of one large logit shows (4096 x
+// 2048 x 65536: losses off by 2.3e-6 without it, 3.3e-7 with it, against 64 bits).
+//
+// What bounds it: many tokens, the tensor pipe and then the power cap (4096 x
+// 2048 x 32768 bf16, loss and gradients 1341 us: STORE 363, 1.51 PFLOP/s; the
+// pass over d 96, memory; GRADS 680, 1.62 PFLOP/s; scores of 4096 x 2048 x 65536
+// in 847, beside 846 of the library's plain product under the same cap).  Few
+// tokens, one read of w and the start of two launches (16 x 1024 x 32000: 22.6
+// us, 10 of them the 66 MB).
 //
 // Every mbarrier wait is bounded (KsWait), as in matmul.cu.
 #include <algorithm>
@@ -183,7 +190,7 @@ KS_DEV void work_coords(int t, int num_m, int num_n, int group, int &tm, int &tn
 // of the second, dealt round robin within each of the two classes of CTAs, so
 // that the tiles in work at one time lie side by side and share operands in L2
 // (runs of neighbouring tiles per CTA read d from DRAM once per column tile:
-// 745 instead of 667 us for the two products of 4096 x 2048 x 32768).
+// 745 instead of 674 us for the two products of 4096 x 2048 x 32768).
 template <bool TWO, int TM, int TN>
 struct Work {
   int count, first;  // items in all, of the first product
@@ -793,7 +800,8 @@ KS_DEV void reduce_loss(const Combine &a, double l, double n, unsigned block, un
   }
 }
 
-// A warp per row, eight rows per block.
+// A warp per row, eight rows per block.  Reads 8 bytes for every half tile of a
+// row: 10 us for 4096 rows of 32768 columns, behind its launch and chain of loads.
 __global__ void __launch_bounds__(256) ce_combine_kernel(const __grid_constant__ Combine a, int release) {
   __shared__ double shl[kCombRows], shn[kCombRows];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -827,10 +835,11 @@ __global__ void __launch_bounds__(256) ce_combine_kernel(const __grid_constant__
 
 // STORE's exponentials e -> d in place: d = f (e exp(tile maximum - lse) -
 // [target]).  A CTA takes 8192 columns of one row, 16 KB, a warp 1024 of them,
-// four 16-byte loads a lane in flight.  Reads and writes 2 bytes a value.
+// four 16-byte loads a lane in flight.  Reads and writes 2 bytes a value: 537 MB
+// for 4096 x 32768 in 91 to 97 us, 5.5 to 5.9 TB/s, the rate of a copy.
 // COMBINE: up to kCombineRows tokens every warp takes its row's lse from the
-// tiles itself, and the combine kernel is left out (333 x 1000 x 10007: 54 -> 50
-// us for the whole call; with many rows the repeated reads cost more).
+// tiles itself, and the combine kernel is left out (333 x 1000 x 10007: 54.4 ->
+// 51.6 us for the whole call; with many rows the repeated reads cost more).
 constexpr int kCombineRows = 512;
 
 template <bool COMBINE>
@@ -1102,9 +1111,10 @@ Tile pick_logits(const ks_linear_ce_config &cfg, int64_t m, int64_t n, int64_t k
 
 // Tile and K-splits of dh [m, n] over kbs K-blocks beside dw [vocab, n] over
 // kb2: all work evenly over the SMs, but no less than the longest item, plus
-// the slabs' traffic where K is split (at least 8 K-blocks a split).  (333 x
-// 1000 over 10007 columns, dh alone: 8 large tiles; split 17 ways 21 us,
-// unsplit 113.)
+// the slabs' traffic where K is split (at least 8 K-blocks a split; 4 or 16 make
+// no difference).  Loss and gradients, bf16, as chosen and without a split: 333 x
+// 1000 x 10007 56 and 81 us, 128 x 4096 x 32000 167 and 231, 64 x 2048 x 32768
+// 109 and 201; where there are tiles enough the two are one.
 Choice pick_grads(const ks_linear_ce_config &cfg, int64_t m, int64_t n, int64_t kbs, int64_t vocab, int64_t kb2, int sms) {
   Choice best = {};
   double least = 0;
