@@ -25,9 +25,11 @@ import sys
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser()
     ap.add_argument("--family", required=True,
-                    choices=("softmax", "layernorm", "bias_gelu", "reduction", "matmul", "flash_attention"))
+                    choices=("softmax", "layernorm", "bias_gelu", "reduction", "matmul", "flash_attention",
+                             "linear_ce", "linear_ce_grad", "embedding", "embedding_grad", "grad_clip"))
     ap.add_argument("--shape", required=True, help="softmax/layernorm/bias_gelu R,C; reduction N (full sum) or "
-                    "R,C (axis 0); matmul M,N,K; flash_attention B,H,N,d")
+                    "R,C (axis 0); matmul M,N,K; flash_attention B,H,N,d; linear_ce*/embedding* tokens,dim,vocab; "
+                    "grad_clip tensors,elements (of each, bf16)")
     ap.add_argument("--launches", type=int, default=4)
     ap.add_argument("--causal", action="store_true")
     ap.add_argument("--gelu", default="tanh", choices=("erf", "tanh"))
@@ -83,6 +85,27 @@ def main(argv=None) -> int:
         am, bm = (rn(m, k) * s).bfloat16(), (rn(k, n) * s).bfloat16()
         c = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
         run = lambda i: ops.matmul(am, bm, out=c, cfg=mk(N.MatmulConfig))  # noqa: E731
+    elif f in ("linear_ce", "linear_ce_grad", "embedding", "embedding_grad"):
+        n, dim, vocab = shape
+        # token ids by a power law, as in text
+        ids = [(torch.rand(n, generator=g, device="cuda") ** 4 * vocab).long() for _ in range(R)]
+        hs = [rn(n, dim).bfloat16() for _ in range(R)]
+        w = (rn(vocab, dim) / math.sqrt(dim)).bfloat16()
+        if f == "linear_ce":
+            run = lambda i: ops.linear_cross_entropy(hs[i % R], w, ids[i % R], cfg=mk(N.LinearCeConfig))  # noqa: E731
+        elif f == "linear_ce_grad":
+            run = lambda i: ops.linear_cross_entropy_grad(hs[i % R], w, ids[i % R], cfg=mk(N.LinearCeConfig))  # noqa: E731
+        elif f == "embedding":
+            run = lambda i: ops.embedding(ids[i % R], w, scale=2.0)  # noqa: E731
+        else:
+            run = lambda i: ops.embedding_backward(ids[i % R], hs[i % R], vocab,  # noqa: E731
+                                                   cfg=mk(N.EmbeddingGradConfig))
+    elif f == "grad_clip":
+        count, numel = shape
+        clippers = [ops.GradClipper([rn(numel).bfloat16() for _ in range(count)],
+                                    out=[torch.empty(numel, dtype=torch.bfloat16, device="cuda") for _ in range(count)])
+                    for _ in range(R)]
+        run = lambda i: clippers[i % R].clip(1.0)  # noqa: E731
     else:
         q, k, v = (rn(*shape).bfloat16() for _ in range(3))
         o = torch.empty_like(q)
