@@ -120,8 +120,9 @@ KS_DEV uint32_t token_key(int64_t t, int64_t vocab, int64_t padding) {
 //
 // Up to kRankMax positions: each position's place is the number of smaller
 // (token, position) pairs, counted directly, 16 threads a position, every CTA
-// with all keys in shared memory.  (At 8192 positions this and the radix sort took
-// the same 20 us, but the comparisons keep 128 SMs from writing zeros.)
+// with all keys in shared memory.  (Whole calls with the limit at 8192 and as it is:
+// 6208 x 72 into 3351 rows 21.0 and 20.5 us, 8192 x 256 into 32768 34.0 and 22.5:
+// the comparisons keep the SMs from writing zeros.)
 //
 // More: radix, below.
 // One cluster of 8 CTAs sorts: least-significant-digit radix passes of up to
@@ -132,7 +133,7 @@ KS_DEV uint32_t token_key(int64_t t, int64_t vocab, int64_t padding) {
 // zeros meanwhile, up to 512 KB a CTA: the sort is latency-bound and uses no bandwidth
 // to speak of.  (With one zeroing CTA per SM the clusters that found no room at
 // first made a second round of it: 134 MB in 36 us, 537 MB in 134, where it is 29
-// and 94 now.  8192 tokens alone sort in about 20 us, 131072 in 61.)
+// and 94 now.  8192 tokens alone sort in 14 us, 131072 in 61.)
 // ---------------------------------------------------------------------------
 constexpr int kCluster = 8;
 constexpr int kSortThreads = 1024;
@@ -244,8 +245,8 @@ __global__ void __launch_bounds__(kSortThreads, 1)
     for (int i = tid; i < kSortWarps * bins; i += kSortThreads) count[i] = 0;
     __syncthreads();
     uint32_t *mine = count + warp * bins;
+    uint2 kv[kBatch];
     for (int64_t i = lo + lane; i < hi; i += 32 * kBatch) {
-      uint2 kv[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u)
         if (i + u * 32 < hi) kv[u] = fetch(i + u * 32);
@@ -298,10 +299,11 @@ __global__ void __launch_bounds__(kSortThreads, 1)
     if (tid < bins) base[tid] = before + incl - total + (warp ? wsum[warp - 1] : 0u);
     __syncthreads();
     for (int64_t i0 = lo + lane; i0 - lane < hi; i0 += 32 * kBatch) {
-      uint2 kv[kBatch];
+      if (per_warp > 32 * kBatch) {  // otherwise they are still in kv
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
-        if (i0 + u * 32 < hi) kv[u] = fetch(i0 + u * 32);
+        for (int u = 0; u < kBatch; ++u)
+          if (i0 + u * 32 < hi) kv[u] = fetch(i0 + u * 32);
+      }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         if (i0 - lane + u * 32 >= hi) break;
@@ -326,8 +328,10 @@ __global__ void __launch_bounds__(kSortThreads, 1)
 // shared memory, kStages stages of kRows rows, filled by bulk copies (one per
 // row, of up to 4 KB), so that about 100 KB a CTA are in flight while the
 // threads add; reading them into registers instead (warps over short windows,
-// 4 to 8 rows in flight each) reached 3.4 TB/s at 131072 x 1024 fp32.  Rows that
-// are not 16-byte aligned are read with plain loads, four rows at a time.
+// 4 to 8 rows in flight each) reached 3.4 TB/s at 131072 x 1024 fp32.  Of rows that
+// are not 16-byte aligned the ring takes the 16-byte granules they lie in, and the
+// threads read single values at the row's offset.  (20000 x 510 bf16 into 50000 rows
+// 36.8 us a call; with plain loads, four rows at a time, 56.7.)
 // Measured: 131072 x 1024 fp32 into as many rows 123 us, 5.2 TB/s; 8192 x 2048 bf16
 // 19 us, where the chain of start, sorted keys, first rows and joins (3 us) bounds
 // it and not its 60 MB.
@@ -358,12 +362,14 @@ struct GradArgs {
   int64_t chunks;
 };
 
-// A thread's sums: `per` adjacent columns (VEC), or 8 of them blockDim apart.
+// A thread's sums: 16 bytes' worth of columns, adjacent (VEC) or blockDim apart.
+// The methods take addresses at the segment's first column; `left`: columns from
+// there to the row's end.
 template <int DT, int ODT, bool VEC>
 struct Sum {
   using E = Elem<DT>;
   using O = Elem<ODT>;
-  static constexpr int W = VEC ? E::kPer : 8;
+  static constexpr int W = E::kPer;
   float a[W];
   KS_DEV static int cols() { return blockDim.x * W; }
   KS_DEV static int col(int j) { return VEC ? threadIdx.x * W + j : threadIdx.x + j * blockDim.x; }
@@ -371,39 +377,38 @@ struct Sum {
 #pragma unroll
     for (int j = 0; j < W; ++j) a[j] = 0.f;
   }
-  // c: the segment's first column
-  KS_DEV void put_part(float *p, int64_t c, int64_t dim) const {
+  KS_DEV void put_part(float *p, int left) const {
 #pragma unroll
     for (int j = 0; j < W; j += VEC ? 4 : 1) {
-      if (c + col(j) >= dim) continue;
+      if (col(j) >= left) continue;
       if constexpr (VEC)
-        *reinterpret_cast<float4 *>(p + c + col(j)) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
+        *reinterpret_cast<float4 *>(p + col(j)) = make_float4(a[j], a[j + 1], a[j + 2], a[j + 3]);
       else
-        p[c + col(j)] = a[j];
+        p[col(j)] = a[j];
     }
   }
-  KS_DEV void add_part(const float *p, int64_t c, int64_t dim) {
+  KS_DEV void add_part(const float *p, int left) {
 #pragma unroll
     for (int j = 0; j < W; j += VEC ? 4 : 1) {
-      if (c + col(j) >= dim) continue;
+      if (col(j) >= left) continue;
       if constexpr (VEC) {
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + c + col(j)));
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + col(j)));
         a[j] += v.x;
         a[j + 1] += v.y;
         a[j + 2] += v.z;
         a[j + 3] += v.w;
       } else {
-        a[j] += __ldcg(p + c + col(j));
+        a[j] += __ldcg(p + col(j));
       }
     }
   }
-  KS_DEV void finish(typename O::T *row, int64_t c, int64_t dim, float scale, bool accumulate) const {
+  KS_DEV void finish(typename O::T *row, int left, float scale, bool accumulate) const {
     constexpr int step = VEC ? W < O::kPer ? W : O::kPer : 1;  // values per 16-byte store
     static_assert(!VEC || step * sizeof(typename O::T) == 16, "whole vectors");
 #pragma unroll
     for (int j = 0; j < W; j += step) {
-      if (c + col(j) >= dim) continue;
-      typename O::T *p = row + c + col(j);
+      if (col(j) >= left) continue;
+      typename O::T *p = row + col(j);
       alignas(16) typename O::T o[step];
       if (accumulate) {
         if constexpr (VEC)
@@ -447,15 +452,16 @@ KS_DEV void join(const GradArgs<DT, ODT> &g, const Part &t, int64_t ch, int64_t 
   using S = Sum<DT, ODT, VEC>;
   __shared__ bool last_group;
   const int64_t c = seg * S::cols(), a = t.a, b = t.b;
-  auto slot = [&](int64_t chunk) { return g.part + (chunk * 2 + (chunk == a ? 1 : 0)) * g.ld; };
+  const int left = int(min(int64_t(S::cols()), g.dim - c));
+  auto slot = [&](int64_t chunk) { return g.part + (chunk * 2 + (chunk == a ? 1 : 0)) * g.ld + c; };
   const int64_t first = max(a, ch / kGroup * kGroup), last = min(b, ch / kGroup * kGroup + kGroup - 1);
   S sum;
   sum.clear();
 #pragma unroll 8
-  for (int64_t j = first; j <= last; ++j) sum.add_part(slot(j), c, g.dim);
+  for (int64_t j = first; j <= last; ++j) sum.add_part(slot(j), left);
   const int64_t ga = a / kGroup, gb = b / kGroup;
   if (ga != gb) {
-    sum.put_part(slot(first), c, g.dim);
+    sum.put_part(slot(first), left);
     __threadfence();
     __syncthreads();
     if (threadIdx.x == 0)
@@ -465,9 +471,9 @@ KS_DEV void join(const GradArgs<DT, ODT> &g, const Part &t, int64_t ch, int64_t 
     __threadfence();
     sum.clear();
 #pragma unroll 8
-    for (int64_t j = ga; j <= gb; ++j) sum.add_part(slot(max(a, j * kGroup)), c, g.dim);
+    for (int64_t j = ga; j <= gb; ++j) sum.add_part(slot(max(a, j * kGroup)), left);
   }
-  sum.finish(g.dtable + int64_t(t.key) * g.dtable_stride, c, g.dim, g.scale, g.accumulate != 0);
+  sum.finish(g.dtable + int64_t(t.key) * g.dtable_stride + c, left, g.scale, g.accumulate != 0);
 }
 
 template <int DT, int ODT, bool VEC>
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(kSegThreads)
   using S = Sum<DT, ODT, VEC>;
   using E = Elem<DT>;
   using T = typename E::T;
-  extern __shared__ __align__(128) uint8_t ring[];  // VEC: [kStages][kRows][16 * blockDim]
+  extern __shared__ __align__(128) uint8_t ring[];  // [kStages][kRows][pitch]
   __shared__ uint2 kv[kMaxChunk];
   __shared__ uint64_t full[kStages];
   __shared__ int gave_up;
@@ -484,7 +490,7 @@ __global__ void __launch_bounds__(kSegThreads)
   const int64_t ch = blockIdx.x / g.segs, seg = blockIdx.x - ch * g.segs, c = seg * S::cols();
   const int64_t lo = ch * g.chunk;
   const int held = int(min(int64_t(g.chunk), g.n - lo));
-  if (VEC && tid == 0) {
+  if (tid == 0) {
     for (int s = 0; s < kStages; ++s) ks_mbar_init(full + s, 1);
     gave_up = 0;
     ks_fence_mbar_init();
@@ -507,22 +513,28 @@ __global__ void __launch_bounds__(kSegThreads)
     next = none;
   }
   if (cnt == 0) return;
-  constexpr int R = VEC ? kRows : 4;  // plain loads: 8 x 4 registers in flight
-  const int stages = (cnt + R - 1) / R;
-  const uint32_t row_bytes = uint32_t(min(int64_t(S::cols()), g.dim - c) * int64_t(sizeof(T)));
-  const uint32_t pitch = blockDim.x * 16;
-  // rows of stage st into its place of the ring, one copy per lane
-  auto fill = [&](int st) {
+  const int stages = (cnt + kRows - 1) / kRows;
+  const int left = int(min(int64_t(S::cols()), g.dim - c));
+  const uint32_t row_bytes = uint32_t(left) * sizeof(T);
+  const uint32_t pitch = blockDim.x * 16 + (VEC ? 0 : 16);
+  // where a row lies in its 16-byte granules
+  const uint32_t first_byte = uint32_t(reinterpret_cast<uintptr_t>(g.dout + c)), step = uint32_t(g.dout_stride * sizeof(T));
+  auto offset = [&](uint32_t pos) { return VEC ? 0u : (first_byte + pos * step) & 15u; };
+  // rows of stage st into slot s of the ring, one copy per lane; !VEC: the whole
+  // granules that hold the row (a granule with a byte of it is mapped memory)
+  auto fill = [&](int st, int s) {
     if (st >= stages || tid >= 32) return;
-    const int rows = min(kRows, cnt - st * kRows), s = st % kStages;
-    if (tid == 0) ks_mbar_arrive_expect_tx(full + s, rows * row_bytes);
+    const int rows = min(kRows, cnt - st * kRows);
+    const uint32_t pos = kv[st * kRows + min(tid, rows - 1)].y, off = offset(pos);
+    uint32_t bytes = VEC ? row_bytes : (off + row_bytes + 15) & ~15u, all = rows * row_bytes;
+    if constexpr (!VEC) all = __reduce_add_sync(0xffffffffu, tid < rows ? bytes : 0u);
+    if (tid == 0) ks_mbar_arrive_expect_tx(full + s, all);
     __syncwarp();
     if (tid < rows)
-      ks_bulk_load(ring + (s * kRows + tid) * pitch, g.dout + int64_t(kv[st * kRows + tid].y) * g.dout_stride + c, row_bytes,
-                   full + s);
+      ks_bulk_load(ring + (s * kRows + tid) * pitch,
+                   reinterpret_cast<const char *>(g.dout + int64_t(pos) * g.dout_stride + c) - off, bytes, full + s);
   };
-  if constexpr (VEC)
-    for (int s = 0; s < kStages; ++s) fill(s);
+  for (int s = 0; s < kStages; ++s) fill(s, s);
   // chunks that the first and the last token reach to, searched for while the
   // first rows are on their way: 32 chunk edges at a time, by every warp for itself
   int64_t first_chunk = ch, last_chunk = ch;
@@ -551,53 +563,65 @@ __global__ void __launch_bounds__(kSegThreads)
   bool head_goes_on = false;
   S sum;
   sum.clear();
+  int slot = 0;
+  uint32_t phase = 0;
+  constexpr int R = kRows / 2;  // rows taken into registers at once
   for (int st = 0; st < stages; ++st) {
-    T x[R][S::W];
-    if constexpr (VEC) {
-      if (!ks_mbar_wait(full + st % kStages, (st / kStages) & 1, &gave_up, wait)) {
-        for (int k = st; k < min(st + kStages, stages); ++k)  // copies still on their way into this CTA's memory
-          ks_mbar_wait(full + k % kStages, (k / kStages) & 1, nullptr, wait);
-        return;
+    const int i0 = st * kRows, rows = min(kRows, cnt - i0);
+    // bit r: the token of row r ends there, or the chunk does
+    const int k = min(i0 + (tid & (kRows - 1)), cnt - 1);
+    const uint32_t ends = __ballot_sync(0xffffffffu, k == cnt - 1 || kv[k + 1].x != kv[k].x);
+    if (!ks_mbar_wait(full + slot, phase, &gave_up, wait)) {
+      for (int n = st; n < min(st + kStages, stages); ++n) {  // copies still on their way into this CTA's memory
+        ks_mbar_wait(full + slot, phase, nullptr, wait);
+        if (++slot == kStages) slot = 0, phase ^= 1;
       }
-    } else {
+      return;
+    }
+#pragma unroll
+    for (int r0 = 0; r0 < kRows; r0 += R) {
+      if (r0 >= rows) break;
+      T x[R][S::W];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {  // rows past `rows` are read and not used
+        const uint8_t *at = ring + (slot * kRows + r0 + r) * pitch;
+        if constexpr (VEC) {
+          const uint4 v = *reinterpret_cast<const uint4 *>(at + tid * 16);
+          *reinterpret_cast<uint4 *>(x[r]) = v;
+        } else {
+          at += offset(kv[min(i0 + r0 + r, cnt - 1)].y);
+#pragma unroll
+          for (int j = 0; j < S::W; ++j) x[r][j] = reinterpret_cast<const T *>(at)[S::col(j)];
+        }
+      }
+      if (r0 + R >= rows) {
+        __syncthreads();  // the slot has been read
+        fill(st + kStages, slot);
+      }
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const bool in = st * R + r < cnt;
-        const T *p = g.dout + (in ? int64_t(kv[st * R + r].y) * g.dout_stride : 0) + c;
+        if (r0 + r >= rows) break;
 #pragma unroll
-        for (int j = 0; j < S::W; ++j) x[r][j] = in && c + S::col(j) < g.dim ? __ldg(p + S::col(j)) : T(0);
+        for (int j = 0; j < S::W; ++j) sum.a[j] += E::get(x[r][j]);
+        if (!(ends >> (r0 + r) & 1)) continue;
+        const int i = i0 + r0 + r;
+        const uint32_t key = kv[i].x;
+        const bool goes_on = i == cnt - 1 && next == key;
+        if (from_before) {
+          sum.put_part(g.part + ch * 2 * g.ld + c, left);
+          head = key;
+          head_goes_on = goes_on;
+        } else if (goes_on) {
+          sum.put_part(g.part + (ch * 2 + 1) * g.ld + c, left);
+          tail = key;
+        } else {
+          sum.finish(g.dtable + int64_t(key) * g.dtable_stride + c, left, g.scale, g.accumulate != 0);
+        }
+        sum.clear();
+        from_before = false;
       }
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int i = st * R + r;
-      if (i >= cnt) break;
-      if constexpr (VEC) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(ring + ((st % kStages) * kRows + r) * pitch + tid * 16);
-        *reinterpret_cast<uint4 *>(x[r]) = v;
-      }
-#pragma unroll
-      for (int j = 0; j < S::W; ++j) sum.a[j] += E::get(x[r][j]);
-      const uint32_t key = kv[i].x, after = i + 1 < cnt ? kv[i + 1].x : next;
-      const bool goes_on = after == key;
-      if (goes_on && i + 1 < cnt) continue;
-      if (from_before) {
-        sum.put_part(g.part + ch * 2 * g.ld, c, g.dim);
-        head = key;
-        head_goes_on = goes_on;
-      } else if (goes_on) {
-        sum.put_part(g.part + (ch * 2 + 1) * g.ld, c, g.dim);
-        tail = key;
-      } else {
-        sum.finish(g.dtable + int64_t(key) * g.dtable_stride, c, g.dim, g.scale, g.accumulate != 0);
-      }
-      sum.clear();
-      from_before = false;
-    }
-    if constexpr (VEC) {
-      __syncthreads();  // the stage has been read
-      fill(st + kStages);
-    }
+    if (++slot == kStages) slot = 0, phase ^= 1;
   }
   if (head == none && tail == none) return;
   // both arrivals at once: a fence and an atomic take about a microsecond each
@@ -679,17 +703,21 @@ GradPlan grad_plan(const ks_embedding_grad_config &c, const ks_embedding_grad_ar
                    aligned16(a.dtable, a.dtable_stride, a.dim, elem_size(a.out_dtype)) && a.dim % (16 / esz) == 0;
   for (const bool v : {!vec, vec}) {
     p.vec = v;
-    const int64_t want = v ? (a.dim * esz + 15) / 16 : (a.dim + 7) / 8;  // threads for a whole row
+    const int64_t want = (a.dim * esz + 15) / 16;  // threads for a whole row
     p.segs = (want + kSegThreads - 1) / kSegThreads;
     p.threads = int(((want + p.segs - 1) / p.segs + 31) / 32 * 32);
     p.segs = (want + p.threads - 1) / p.threads;
-    p.shm = v ? size_t(kStages) * kRows * p.threads * 16 : 0;
+    p.shm = size_t(kStages) * kRows * (p.threads * 16 + (v ? 0 : 16));
     // one round of CTAs, as many as the SMs hold; two where chunks stay long
     // (131072 x 1024 fp32: 242 us in one round of 448 positions, 222 in two)
     const int64_t per_sm = std::min<int64_t>({int64_t(227 * 1024 / (p.shm + 9 * 1024 + 512)), 1024 / p.threads, 16});
     int64_t even = (n * p.segs + per_sm * ks::sm_count() - 1) / (per_sm * ks::sm_count());
     if (even >= 256) even = (even + 1) / 2;
-    p.chunk = c.chunk ? c.chunk : int(std::min<int64_t>(kMaxChunk, std::max<int64_t>(even, kRows)));
+    // at least 8 positions; 16 from 4096 on, where a frequent token would lie in many
+    // chunks (5178 x 104 into 529 rows: 21.2 us in chunks of 8, 17.7 in 16; 4142 x 408
+    // unaligned 28.7 and 23.1; 777 x 1001 13.8 and 15.6)
+    const int64_t least = std::min<int64_t>(16, std::max<int64_t>(kRows, n / 256));
+    p.chunk = c.chunk ? c.chunk : int(std::min<int64_t>(kMaxChunk, std::max<int64_t>(even, least)));
     p.chunks = (n + p.chunk - 1) / p.chunk;
     p.counters = p.chunks * 3 * p.segs;
     most_chunks = std::max(most_chunks, p.chunks);
