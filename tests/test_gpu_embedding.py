@@ -164,6 +164,27 @@ def test_accumulate_padding_and_strides(ks, names, pad, offset):
     assert torch.equal(full[:, dim:], base[:, dim:])
 
 
+@pytest.mark.parametrize("names", [("bf16", "bf16"), ("fp16", "fp32"), ("fp32", "fp32")], ids=lambda v: "-".join(v))
+@pytest.mark.parametrize("dim", [1, 7, 250, 2047, 2056, 4099])
+@pytest.mark.parametrize("pad,offset", [(1, 0), (2, 3), (5, 7), (8, 2)])
+def test_gradient_of_unaligned_rows(ks, dim, pad, offset, names):
+    """Rows at every offset within 16 bytes, one and several segments wide, with
+    NaN in all that lies between them."""
+    N, ops, torch = ks
+    n, vocab = 300, 90
+    g = _gen(torch, dim + pad)
+    dtype = _dt(torch, names[0])
+    flat = torch.full((n * (dim + pad) + offset + 16,), float("nan"), dtype=dtype, device="cuda")
+    dout = flat[offset:offset + n * (dim + pad)].view(n, dim + pad)[:, :dim]
+    dout.copy_(torch.randn(n, dim, generator=g, device="cuda"))
+    tokens = torch.randint(0, vocab, (n,), generator=g, device="cuda")
+    got = ops.embedding_backward(tokens, dout, vocab, 2.5, dtype=_dt(torch, names[1]))
+    _check_grad(torch, got, tokens, dout, vocab, 2.5, names[1])
+    full = torch.full((vocab, dim + 3), 9.0, dtype=_dt(torch, names[1]), device="cuda")
+    ops.embedding_backward(tokens, dout, vocab, 2.5, dtable=full[:, :dim])
+    assert torch.equal(full[:, :dim], got) and (full[:, dim:] == 9).all()
+
+
 def test_excluded_rows_may_hold_anything(ks):
     N, ops, torch = ks
     dout = torch.randn(100, 64, device="cuda").bfloat16()
