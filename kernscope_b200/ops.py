@@ -302,10 +302,10 @@ _ce_scratch: dict = {}  # problem size and alignment -> preferred workspace byte
 def _linear_ce_run(a, cfg, workspace, like, stream):
     if workspace is None:
         if cfg is None:
-            # all that the size depends on
-            aligned = [not ((p or 0) & 15 or stride & 7) for p, stride in
-                       ((a.h, a.h_stride), (a.w, a.w_stride), (a.dh, a.dh_stride), (a.dw, a.dw_stride))]
-            key = (a.tokens, a.dim, a.vocab, a.ce_pass, LINEAR_CE_WORKSPACE_LIMIT, *aligned)
+            # all that the size depends on: sizes, and what keeps a row from a 16-byte boundary
+            key = (a.tokens, a.dim, a.vocab, a.ce_pass, LINEAR_CE_WORKSPACE_LIMIT, (a.h | a.h_stride << 1) & 15,
+                   (a.w | a.w_stride << 1) & 15, ((a.dh or 0) | a.dh_stride << 1) & 15,
+                   ((a.dw or 0) | a.dw_stride << 1) & 15)
             size = _ce_scratch.get(key)
             if size is None:
                 if len(_ce_scratch) >= 4096:
