@@ -258,6 +258,16 @@ def _rows(name, t, dtypes, dev: int) -> tuple[int, int, int]:
                      f"{t.device})")
 
 
+def _as_rows(name, t, n: int, dim: int) -> torch.Tensor:
+    """t, or its view as [n, dim] where it has another rank than 2."""
+    if t.dim() == 2:
+        return t
+    try:
+        return t.view(n, dim)
+    except RuntimeError:
+        raise ValueError(f"{name} must be [{n}, {dim}] or view as it (got {tuple(t.shape)}, strides {t.stride()})") from None
+
+
 def _values(name, t, dtype, n: int, dev: int) -> int:
     """Address of a contiguous tensor of n values on device `dev`."""
     if t.dtype is dtype and t.get_device() == dev and t.numel() == n and t.is_contiguous():
@@ -390,7 +400,8 @@ def linear_cross_entropy_grad(h, w, targets, ignore_index: int = -100, reduction
 
 def embedding(tokens, table, scale: float = 1.0, out=None, stream=None) -> torch.Tensor:
     """scale * table[tokens] (tokens int64 of any shape, table [vocab, dim] in
-    bf16, fp16 or fp32); tokens outside [0, vocab) give rows of zeros."""
+    bf16, fp16 or fp32); tokens outside [0, vocab) give rows of zeros.  `out`:
+    [number of tokens, dim] with any row stride, or what views as that."""
     dev = torch.cuda.current_device()
     vocab, dim, table_stride = _rows("table", table, _DT_TRAIN, dev)
     n = tokens.numel()
@@ -399,9 +410,9 @@ def embedding(tokens, table, scale: float = 1.0, out=None, stream=None) -> torch
         out = _empty(table, (*tokens.shape, dim), table.dtype, stream)
         out_stride = dim
     else:
-        if out.numel() != n * dim:
-            raise ValueError(f"out must hold {n} rows of {dim}")
-        out_stride = _rows("out", out if out.dim() == 2 else out.view(n, dim), (table.dtype,), dev)[2]
+        rows, cols, out_stride = _rows("out", _as_rows("out", out, n, dim), (table.dtype,), dev)
+        if (rows, cols) != (n, dim):
+            raise ValueError(f"out must be [{n}, {dim}], or of another rank and {n} rows of {dim} as a view")
     if n == 0:
         return out
     args = N.EmbeddingArgs(ids, n, table.data_ptr(), out.data_ptr(), vocab, dim, table_stride, out_stride,
