@@ -96,6 +96,12 @@ int ks_selftest_bounded_wait(uint64_t limit_ns, void *stream);
 /* Bound (ns) that every spin-wait in the kernels uses; default 4e9. */
 int ks_set_wait_limit_ns(uint64_t limit_ns);
 
+/* 1 where two sets of rows (`bytes` each, `stride` bytes apart) share a byte, else
+ * 0: the test that the entries below make of their outputs.  Rows that lie
+ * between one another's share none.  Host arithmetic only.                    */
+int ks_rows_overlap(const void *a, int64_t a_rows, int64_t a_bytes, int64_t a_stride,
+                    const void *b, int64_t b_rows, int64_t b_bytes, int64_t b_stride);
+
 /* ---- shared enums ------------------------------------------------------ */
 typedef enum ks_dtype { KS_BF16 = 0, KS_F32 = 1, KS_F64 = 2, KS_F16 = 3 } ks_dtype;
 
@@ -278,7 +284,9 @@ int ks_flash_attention_launch(const ks_flash_attention_config *cfg,
  * multiple of 256; 0 = as many as the workspace holds.
  * ks_linear_ce_workspace_bytes() gives the least size that works and the
  * size that the call makes use of (at most about limit bytes, or `least`
- * where that is more); the workspace is 256-byte aligned.                    */
+ * where that is more); the workspace is 256-byte aligned.
+ * An output or the workspace may share no byte with another tensor of the
+ * call: KS_ERR_INVALID_ARGS.                                                 */
 typedef enum ks_ce_pass { KS_CE_FORWARD = 0, KS_CE_BACKWARD = 1, KS_CE_GRAD = 2 } ks_ce_pass;
 typedef enum ks_ce_reduction { KS_CE_NONE = 0, KS_CE_MEAN = 1, KS_CE_SUM = 2 } ks_ce_reduction;
 typedef struct ks_linear_ce_config { int tile_m; int tile_n; int64_t piece; } ks_linear_ce_config;

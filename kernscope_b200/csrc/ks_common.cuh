@@ -479,6 +479,18 @@ void set_reason(char *buf, size_t len, const char *fmt, ...);
 // runtime.cu).
 int allow_shared(const void *kernel, size_t bytes);
 
+// Rows of a tensor in memory: `bytes` each, `stride` bytes apart (any stride where
+// there is one row).  p == nullptr or no row: no memory.
+struct Rows {
+  const void *p;
+  int64_t rows, bytes, stride;
+};
+// Whether two tensors share a byte.  Rows that lie between one another's, as two
+// column ranges of one matrix do, share none (defined in runtime.cu).
+bool overlap(const Rows &a, const Rows &b);
+// Whether one of the first `outputs` of `n` tensors overlaps another of the n.
+bool outputs_overlap(const Rows *t, int outputs, int n);
+
 // Launch `kernel`; `next`: as the successor of this call's previous kernel, it
 // may be set up while that one still runs and calls ks_pdl_wait() itself.
 template <typename... P, typename... A>

@@ -1513,6 +1513,19 @@ int ks_linear_ce_launch(const ks_linear_ce_config *cfg, const ks_linear_ce_args 
   Plan p;
   make_plan(*cfg, *a, a->workspace_bytes, p);
   if (!a->workspace || p.bytes > a->workspace_bytes || odd(a->workspace, 256)) return KS_ERR_WORKSPACE;
+  // dw is written while other tiles of the launch still read h and w, and dh too
+  const bool fwd = a->pass != KS_CE_BACKWARD, bwd = a->pass != KS_CE_FORWARD;
+  const int64_t n = a->tokens, row = a->dim * 2, one = a->reduction == KS_CE_NONE ? n * 4 : 4;
+  const ks::Rows mem[] = {{a->workspace, 1, int64_t(p.bytes), 0},
+                          {bwd ? a->dh : nullptr, n, row, a->dh_stride * 2},
+                          {bwd ? a->dw : nullptr, a->vocab, row, a->dw_stride * 2},
+                          {fwd ? a->loss : nullptr, 1, one, 0},
+                          {a->lse, 1, n * 4, 0},
+                          {a->h, n, row, a->h_stride * 2},
+                          {a->w, a->vocab, row, a->w_stride * 2},
+                          {a->targets, 1, n * 8, 0},
+                          {bwd ? a->dloss : nullptr, 1, one, 0}};
+  if (ks::outputs_overlap(mem, 5, 9)) return KS_ERR_INVALID_ARGS;
   if ((s = ks::check_arch_sm100()) != KS_OK) return s;
   return run(*a, p, static_cast<cudaStream_t>(stream));
 }

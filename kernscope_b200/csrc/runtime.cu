@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <vector>
@@ -142,6 +143,39 @@ int allow_shared(const void *kernel, size_t bytes) {
   else
     cache.push_back({kernel, dev, bytes});
   return KS_OK;
+}
+
+bool overlap(const Rows &a, const Rows &b) {
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.bytes <= 0 || b.bytes <= 0) return false;
+  using Int = __int128;  // a product of any two 64-bit values
+  const Int pa = Int(reinterpret_cast<uintptr_t>(a.p)), pb = Int(reinterpret_cast<uintptr_t>(b.p));
+  const Int ea = pa + Int(a.rows - 1) * a.stride + a.bytes, eb = pb + Int(b.rows - 1) * b.stride + b.bytes;
+  if (ea <= pb || eb <= pa) return false;
+  if ((a.rows > 1 && a.stride < a.bytes) || (b.rows > 1 && b.stride < b.bytes)) return true;  // rows that overlap themselves
+  if (a.rows > 1 && a.stride == a.bytes) return overlap(Rows{a.p, 1, a.rows * a.bytes, 0}, b);
+  if (b.rows > 1 && b.stride == b.bytes) return overlap(a, Rows{b.p, 1, b.rows * b.bytes, 0});
+  if (a.rows > 1 && b.rows > 1 && a.stride == b.stride) {
+    // where b's rows begin within a's period; the ranges meet, so the rows that could collide are there
+    const Int off = ((pb - pa) % a.stride + a.stride) % a.stride;
+    return off < a.bytes || off + b.bytes > a.stride;
+  }
+  // each row of the tensor with fewer, against the last row of the other that begins before its end
+  const Rows &x = a.rows <= b.rows ? a : b, &y = a.rows <= b.rows ? b : a;
+  const Int px = Int(reinterpret_cast<uintptr_t>(x.p)), py = Int(reinterpret_cast<uintptr_t>(y.p));
+  for (int64_t i = 0; i < x.rows; ++i) {
+    const Int from = px + Int(i) * x.stride, to = from + x.bytes;
+    if (to <= py) continue;
+    const Int last = y.rows == 1 ? 0 : std::min(Int(y.rows - 1), (to - 1 - py) / y.stride);
+    if (py + last * y.stride + y.bytes > from) return true;
+  }
+  return false;
+}
+
+bool outputs_overlap(const Rows *t, int outputs, int n) {
+  for (int i = 0; i < outputs; ++i)
+    for (int j = i + 1; j < n; ++j)
+      if (overlap(t[i], t[j])) return true;
+  return false;
 }
 
 void set_reason(char *buf, size_t len, const char *fmt, ...) {
@@ -348,6 +382,11 @@ int ks_device_error_take(int *word) {
   e = cudaMemcpyFromSymbol(word, g_ks_device_error, sizeof(int));
   if (e == cudaSuccess) e = cudaMemcpyToSymbol(g_ks_device_error, &zero, sizeof(int));
   return ks::map_cuda(e);
+}
+
+int ks_rows_overlap(const void *a, int64_t a_rows, int64_t a_bytes, int64_t a_stride, const void *b, int64_t b_rows,
+                    int64_t b_bytes, int64_t b_stride) {
+  return ks::overlap(ks::Rows{a, a_rows, a_bytes, a_stride}, ks::Rows{b, b_rows, b_bytes, b_stride});
 }
 
 int ks_set_wait_limit_ns(uint64_t limit_ns) {

@@ -172,6 +172,8 @@ PROTOTYPES = {
     "ks_gpu_event_elapsed_ms": (C.c_int, [C.c_void_p, C.c_void_p, _P(C.c_float)]),
     "ks_device_error_take": (C.c_int, [_P(C.c_int)]),
     "ks_selftest_bounded_wait": (C.c_int, [C.c_uint64, C.c_void_p]),
+    "ks_rows_overlap": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
+                                  C.c_int64]),
     "ks_set_wait_limit_ns": (C.c_int, [C.c_uint64]),
     "ks_softmax_validate": (C.c_int, [_P(SoftmaxConfig), C.c_int64, C.c_int64, C.c_char_p, C.c_size_t]),
     "ks_softmax_launch": (C.c_int, [_P(SoftmaxConfig), _P(SoftmaxArgs), C.c_void_p]),

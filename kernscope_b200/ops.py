@@ -276,6 +276,17 @@ def _values(name, t, dtype, n: int, dev: int) -> int:
                      f"{t.dtype} {tuple(t.shape)}, {t.device})")
 
 
+def _name_overlap(outputs: int, **memory) -> None:
+    """After a launch that was refused for its arguments: a ValueError where one of
+    the first `outputs` tensors shares memory with another.  memory: (address, rows,
+    bytes per row, bytes between rows) of each."""
+    names = list(memory)
+    for i, a in enumerate(names[:outputs]):
+        for b in names[i + 1:]:
+            if N.lib.ks_rows_overlap(*memory[a], *memory[b]):
+                raise ValueError(f"{a} overlaps {b}")
+
+
 def _linear_ce_args(h, w, targets, ce_pass, reduction, ignore_index, grad_scale=1.0) -> N.LinearCeArgs:
     dev = torch.cuda.current_device()
     n, dim, h_stride = _rows("h", h, _DT_HALF, dev)
@@ -327,8 +338,14 @@ def _linear_ce_run(a, cfg, workspace, like, stream):
         a.workspace, a.workspace_bytes = workspace.data_ptr(), size
     else:
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    N.check("ks_linear_ce_launch", N.lib.ks_linear_ce_launch(C.byref(cfg or _CE_DEFAULT), C.byref(a),
-                                                             _raw_stream(stream, like.get_device())))
+    status = N.lib.ks_linear_ce_launch(C.byref(cfg or _CE_DEFAULT), C.byref(a), _raw_stream(stream, like.get_device()))
+    if status == N.KS_ERR_INVALID_ARGS:
+        n, row = a.tokens, a.dim * 2
+        _name_overlap(3, dh=(a.dh, n, row, a.dh_stride * 2), dw=(a.dw, a.vocab, row, a.dw_stride * 2),
+                      workspace=(a.workspace, 1, a.workspace_bytes, 0), h=(a.h, n, row, a.h_stride * 2),
+                      w=(a.w, a.vocab, row, a.w_stride * 2), targets=(a.targets, 1, n * 8, 0),
+                      lse=(a.lse, 1, n * 4, 0), dloss=(a.dloss, 1, n * 4 if a.reduction == N.KS_CE_NONE else 4, 0))
+    N.check("ks_linear_ce_launch", status)
 
 
 def linear_cross_entropy(h, w, targets, ignore_index: int = -100, reduction: str = "none", cfg=None, workspace=None,
@@ -369,7 +386,8 @@ def linear_cross_entropy_backward(h, w, targets, lse, dloss=None, ignore_index: 
     """Gradients (dh, dw) of linear_cross_entropy from its lse.  dloss: the
     incoming fp32 gradient, one value per token for reduction "none", one value
     otherwise; None stands for ones.  Tokens with targets == ignore_index take no
-    part, and the mean divides by the number of the others."""
+    part, and the mean divides by the number of the others.  dh and dw, where
+    given, overlap neither one another nor h or w."""
     a = _linear_ce_args(h, w, targets, N.KS_CE_BACKWARD, reduction, ignore_index, grad_scale)
     dev = h.get_device()
     a.lse = _values("lse", lse, torch.float32, a.tokens, dev)
@@ -385,7 +403,8 @@ def linear_cross_entropy_backward(h, w, targets, lse, dloss=None, ignore_index: 
 def linear_cross_entropy_grad(h, w, targets, ignore_index: int = -100, reduction: str = "mean", grad_scale: float = 1.0,
                               dh=None, dw=None, cfg=None, workspace=None, stream=None):
     """Loss (fp32, one value) and the gradients of grad_scale * loss with respect
-    to h and w in one call: what a training step needs of its last layer."""
+    to h and w in one call: what a training step needs of its last layer.  dh and
+    dw, where given, overlap neither one another nor h or w."""
     a = _linear_ce_args(h, w, targets, N.KS_CE_GRAD, reduction, ignore_index, grad_scale)
     if reduction == "none":
         raise ValueError("loss and gradient in one call need reduction 'mean' or 'sum'")

@@ -87,3 +87,115 @@ def test_embedding_out_whose_rows_cannot_be_viewed(front):
     with pytest.raises(ValueError):
         ops.embedding(tokens, table, out=fake(torch.zeros(8, 16, 32).bfloat16()[:, :8]))
     assert not rec.calls
+
+
+def test_rows_overlap_against_every_byte(front):
+    """The overlap test against sets of bytes: equal and different strides, rows
+    between one another's, one row, none."""
+    import random
+
+    N, ops, rec = front
+    r = random.Random(3)
+    seen = {0: 0, 1: 0}
+    for i in range(4000):
+        def rows():
+            width = r.randint(1, 9)
+            return r.randint(1, 120), r.choice([0, 1, 1, 2, 3, 7]), width, r.choice([width, 10, 10, 10, r.randint(width, 24)])
+
+        a, b = rows(), rows()
+        held = lambda t: {t[0] + k * t[3] + c for k in range(t[1]) for c in range(t[2])}  # noqa: E731
+        want = int(bool(held(a) & held(b)))
+        assert N.lib.ks_rows_overlap(*a, *b) == want, (a, b)
+        seen[want] += 1
+    assert min(seen.values()) > 500
+    assert N.lib.ks_rows_overlap(None, 4, 8, 8, 1, 4, 8, 8) == 0
+    far = (1 << 62, 1 << 40, 1 << 20, 1 << 60)  # no overflow
+    assert N.lib.ks_rows_overlap(*far, 1 << 61, 4, 8, 8) == 0
+
+
+def _scratch(n):
+    flat = torch.zeros(n + 256, dtype=torch.uint8)
+    at = -flat.data_ptr() % 256
+    return fake(flat[at:at + n])
+
+
+def _ce_case(n=70, dim=64, vocab=300):
+    wide = fake(torch.zeros(max(n, vocab) * 3, 4 * dim).bfloat16())
+    return (wide, wide[:n, :dim], wide[:vocab, dim:2 * dim], fake(torch.zeros(n, dtype=torch.int64)), fake(torch.zeros(n)),
+            _scratch(64 << 20))
+
+
+@pytest.fixture
+def refusing(front, monkeypatch):
+    """The real launches, which refuse before any CUDA call; one that would go on
+    stops at the check for a device instead (this test is for machines without)."""
+    if torch.cuda.is_available():
+        pytest.skip("an accepted launch would run on host addresses")
+    N, ops, rec = front
+    monkeypatch.setattr(N, "lib", rec._lib)
+    return N, ops
+
+
+CE_ALIASES = {  # dh and dw as views of the buffer that also holds h (columns 0..63) and w (64..127)
+    "dh is h": lambda b, n, v, d: (b[:n, :d], None),
+    "dh begins inside h": lambda b, n, v, d: (b[n - 1:2 * n - 1, :d], None),
+    "dh shares one column with w": lambda b, n, v, d: (b[:n, 2 * d - 1:3 * d - 1], None),
+    "dw is w": lambda b, n, v, d: (None, b[:v, d:2 * d]),
+    "dw shares one row with h": lambda b, n, v, d: (None, b[n - 1:n - 1 + v, :d]),
+    "dw shares one row with dh": lambda b, n, v, d: (b[v:v + n, 2 * d:3 * d], b[v + n - 1:2 * v + n - 1, 2 * d:3 * d]),
+}
+
+
+@pytest.mark.parametrize("alias", CE_ALIASES, ids=str)
+def test_cross_entropy_gradients_that_overlap(refusing, alias):
+    """dw's tiles are written while others still read h and w, and dh's beside them."""
+    N, ops = refusing
+    wide, h, w, t, lse, ws = _ce_case()
+    dh, dw = CE_ALIASES[alias](wide, 70, 300, 64)
+    for call in (lambda: ops.linear_cross_entropy_grad(h, w, t, dh=dh, dw=dw, workspace=ws),
+                 lambda: ops.linear_cross_entropy_backward(h, w, t, lse, dh=dh, dw=dw, workspace=ws)):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+
+
+def test_cross_entropy_workspace_that_overlaps(refusing):
+    N, ops = refusing
+    wide, h, w, t, lse, ws = _ce_case()
+    inside = ws[4096:4096 + 300 * 64 * 2].view(torch.bfloat16).view(300, 64)
+    for call in (lambda: ops.linear_cross_entropy(h, inside, t, workspace=ws),
+                 lambda: ops.linear_cross_entropy_grad(h, w, t, dw=inside, workspace=ws)):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
+
+
+def test_cross_entropy_gradients_between_the_inputs_rows(refusing):
+    """Column ranges of one buffer share nothing: the launch goes on to look for a device."""
+    N, ops = refusing
+    wide, h, w, t, lse, ws = _ce_case()
+    with pytest.raises(N.KsError) as e:
+        ops.linear_cross_entropy_grad(h, w, t, dh=wide[:70, 128:192], dw=wide[:300, 192:], workspace=ws)
+    assert e.value.status not in (N.KS_ERR_INVALID_ARGS, N.KS_ERR_WORKSPACE)
+
+
+def test_cross_entropy_c_entry_refuses_overlaps(refusing):
+    N, ops = refusing
+    ws = _scratch(1 << 20)
+    cfg = N.LinearCeConfig(0, 0, 0)
+
+    def launch(**kw):
+        a = N.LinearCeArgs(0x100000, 0x200000, 0x300000, 10, 64, 100, 64, 64, N.KS_BF16, N.KS_CE_GRAD, N.KS_CE_MEAN, 1.0,
+                           -100, None, 0x400000, 0x500000, 0x600000, 0x700000, 64, 64, ws.data_ptr(), 1 << 20)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return N.lib.ks_linear_ce_launch(C.byref(cfg), C.byref(a), None)
+
+    assert launch() not in (N.KS_ERR_INVALID_ARGS, N.KS_ERR_WORKSPACE)  # no device
+    for kw in (dict(dh=0x100000), dict(dh=0x200000), dict(dw=0x200000), dict(dw=0x100000), dict(dw=0x600000),
+               dict(dh=0x300000), dict(loss=0x300000), dict(loss=0x500000), dict(lse=0x300040), dict(lse=0x700000),
+               dict(dloss=0x400000), dict(h=ws.data_ptr()), dict(dw=ws.data_ptr())):
+        assert launch(**kw) == N.KS_ERR_INVALID_ARGS, kw
+    # the backward pass reads lse and writes no loss
+    assert launch(ce_pass=N.KS_CE_BACKWARD, loss=0x300000) != N.KS_ERR_INVALID_ARGS
+    assert launch(ce_pass=N.KS_CE_BACKWARD, dh=0x500000) == N.KS_ERR_INVALID_ARGS
+    # the forward pass writes neither dh nor dw
+    assert launch(ce_pass=N.KS_CE_FORWARD, dh=0x100000, dw=0x200000) != N.KS_ERR_INVALID_ARGS
