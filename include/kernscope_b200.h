@@ -325,7 +325,8 @@ int ks_embedding_launch(const ks_embedding_args *args, void *stream);
  * cfg.chunk: sorted positions after which a token's sum is split, 1..1024, 0 =
  * chosen from the sizes.
  * The workspace (256-byte aligned) holds the sorted tokens and the partial
- * sums of tokens that lie in several chunks.                                 */
+ * sums of tokens that lie in several chunks.  dtable and the workspace may
+ * share no byte with another tensor of the call: KS_ERR_INVALID_ARGS.         */
 typedef struct ks_embedding_grad_config { int chunk; } ks_embedding_grad_config;
 typedef struct ks_embedding_grad_args {
   const int64_t *tokens; int64_t tokens_count; const void *dout; void *dtable;

@@ -867,6 +867,12 @@ int ks_embedding_grad_launch(const ks_embedding_grad_config *cfg, const ks_embed
   if (off(a->tokens, 8) || off(a->dout, esz) || off(a->dtable, osz)) return KS_ERR_INVALID_ARGS;
   const GradPlan p = grad_plan(*cfg, *a);
   if (!a->workspace || off(a->workspace, 256) || a->workspace_bytes < p.bytes) return KS_ERR_WORKSPACE;
+  // the table's zeros are written before dout is read
+  const ks::Rows mem[] = {{a->dtable, a->vocab, a->dim * osz, a->dtable_stride * osz},
+                          {a->workspace, 1, int64_t(p.bytes), 0},
+                          {a->dout, a->tokens_count, a->dim * esz, a->dout_stride * esz},
+                          {a->tokens, 1, a->tokens_count * 8, 0}};
+  if (ks::outputs_overlap(mem, 2, 4)) return KS_ERR_INVALID_ARGS;
   if ((s = ks::check_arch_sm100()) != KS_OK) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char *ws = static_cast<char *>(a->workspace);

@@ -449,7 +449,8 @@ def embedding_backward(tokens, dout, vocab: int, scale: float = 1.0, padding_idx
     """Gradient of `embedding` with respect to its table: [vocab, dim] in dout's
     type or fp32 (`dtype`, or that of `dtable`).  accumulate adds to `dtable`'s
     values and touches the rows of `tokens` alone; otherwise every row is
-    written.  Tokens equal to padding_idx or outside [0, vocab) have no part."""
+    written.  Tokens equal to padding_idx or outside [0, vocab) have no part.
+    dtable, where given, does not overlap dout."""
     dev = torch.cuda.current_device()
     rows = dout if dout.dim() == 2 else dout.view(tokens.numel(), dout.shape[-1])
     n, dim, dout_stride = _rows("dout", rows, _DT_TRAIN, dev)
@@ -484,8 +485,13 @@ def embedding_backward(tokens, dout, vocab: int, scale: float = 1.0, padding_idx
         args.workspace, args.workspace_bytes = workspace.data_ptr(), size
     else:
         args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    N.check("ks_embedding_grad_launch",
-            N.lib.ks_embedding_grad_launch(C.byref(cfg), C.byref(args), _raw_stream(stream, dev)))
+    status = N.lib.ks_embedding_grad_launch(C.byref(cfg), C.byref(args), _raw_stream(stream, dev))
+    if status == N.KS_ERR_INVALID_ARGS:
+        size, out_size = dout.element_size(), dtable.element_size()
+        _name_overlap(2, dtable=(args.dtable, vocab, dim * out_size, dtable_stride * out_size),
+                      workspace=(args.workspace, 1, args.workspace_bytes, 0),
+                      dout=(args.dout, n, dim * size, dout_stride * size), tokens=(ids, 1, n * 8, 0))
+    N.check("ks_embedding_grad_launch", status)
     return dtable
 
 

@@ -199,3 +199,28 @@ def test_cross_entropy_c_entry_refuses_overlaps(refusing):
     assert launch(ce_pass=N.KS_CE_BACKWARD, dh=0x500000) == N.KS_ERR_INVALID_ARGS
     # the forward pass writes neither dh nor dw
     assert launch(ce_pass=N.KS_CE_FORWARD, dh=0x100000, dw=0x200000) != N.KS_ERR_INVALID_ARGS
+
+
+@pytest.mark.parametrize("dtype", [None, torch.float32], ids=str)
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_embedding_gradient_that_overlaps(refusing, accumulate, dtype):
+    """The table's rows are zeroed (or written) while dout is still to be read."""
+    N, ops = refusing
+    n, dim, vocab = 40, 32, 100
+    buf = fake(torch.zeros(400, 4 * dim).bfloat16())
+    tokens = fake(torch.zeros(n, dtype=torch.int64))
+    ws = _scratch(1 << 20)
+    as_table = lambda t: t if dtype is None else t.view(torch.float32)  # noqa: E731
+    width = dim if dtype is None else 2 * dim  # columns of bf16 that a row of the table takes
+    call = lambda dout, dtable, ws=ws: ops.embedding_backward(tokens, dout, vocab, dtable=dtable, accumulate=accumulate,  # noqa: E731
+                                                              workspace=ws)
+    for dout, dtable in ((buf[:n, :dim], as_table(buf[:vocab, :width])),
+                         (buf[vocab - 1:vocab - 1 + n, :dim], as_table(buf[:vocab, :width])),
+                         (buf[:n, width - 1:width - 1 + dim], as_table(buf[:vocab, :width]))):
+        with pytest.raises(ValueError, match="dtable overlaps dout"):
+            call(dout, dtable)
+    with pytest.raises(ValueError, match="workspace"):
+        call(buf[:n, :dim], fake(ws[:vocab * width * 2]).view(torch.bfloat16 if dtype is None else dtype).view(vocab, dim))
+    with pytest.raises(N.KsError) as e:  # the table's rows lie between dout's: on to the check for a device
+        call(buf[:n, width:width + dim], as_table(buf[:vocab, :width]))
+    assert e.value.status not in (N.KS_ERR_INVALID_ARGS, N.KS_ERR_WORKSPACE)
