@@ -307,8 +307,9 @@ int ks_linear_ce_launch(const ks_linear_ce_config *cfg, const ks_linear_ce_args 
 /* ---- embedding ------------------------------------------------------------
  * out[i,:] = scale * table[tokens[i],:] in fp32, rounded once; a token outside
  * [0, vocab) gives zeros (the rows of another shard of the table).  bf16,
- * fp16 or fp32; row strides in elements, dense rows; tokens int64.  No
- * counterpart in the reference.                                             */
+ * fp16 or fp32; row strides in elements, dense rows; tokens int64.  out may
+ * share no byte with table or tokens: KS_ERR_INVALID_ARGS.  No counterpart in
+ * the reference.                                                            */
 typedef struct ks_embedding_args {
   const int64_t *tokens; int64_t tokens_count; const void *table; void *out;
   int64_t vocab; int64_t dim; int64_t table_stride; int64_t out_stride;

@@ -835,6 +835,10 @@ int ks_embedding_launch(const ks_embedding_args *a, void *stream) {
   if (s != KS_OK) return s;
   const int esz = elem_size(a->dtype);
   if (off(a->tokens, 8) || off(a->table, esz) || off(a->out, esz)) return KS_ERR_INVALID_ARGS;
+  const ks::Rows mem[] = {{a->out, a->tokens_count, a->dim * esz, a->out_stride * esz},
+                          {a->table, a->vocab, a->dim * esz, a->table_stride * esz},
+                          {a->tokens, 1, a->tokens_count * 8, 0}};
+  if (ks::outputs_overlap(mem, 1, 3)) return KS_ERR_INVALID_ARGS;
   if ((s = ks::check_arch_sm100()) != KS_OK) return s;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {

@@ -420,7 +420,8 @@ def linear_cross_entropy_grad(h, w, targets, ignore_index: int = -100, reduction
 def embedding(tokens, table, scale: float = 1.0, out=None, stream=None) -> torch.Tensor:
     """scale * table[tokens] (tokens int64 of any shape, table [vocab, dim] in
     bf16, fp16 or fp32); tokens outside [0, vocab) give rows of zeros.  `out`:
-    [number of tokens, dim] with any row stride, or what views as that."""
+    [number of tokens, dim] with any row stride, or what views as that; it does not
+    overlap table."""
     dev = torch.cuda.current_device()
     vocab, dim, table_stride = _rows("table", table, _DT_TRAIN, dev)
     n = tokens.numel()
@@ -436,7 +437,12 @@ def embedding(tokens, table, scale: float = 1.0, out=None, stream=None) -> torch
         return out
     args = N.EmbeddingArgs(ids, n, table.data_ptr(), out.data_ptr(), vocab, dim, table_stride, out_stride,
                            _DT_TRAIN[table.dtype], scale)
-    N.check("ks_embedding_launch", N.lib.ks_embedding_launch(C.byref(args), _raw_stream(stream, dev)))
+    status = N.lib.ks_embedding_launch(C.byref(args), _raw_stream(stream, dev))
+    if status == N.KS_ERR_INVALID_ARGS:
+        size = table.element_size()
+        _name_overlap(1, out=(args.out, n, dim * size, out_stride * size),
+                      table=(args.table, vocab, dim * size, table_stride * size), tokens=(ids, 1, n * 8, 0))
+    N.check("ks_embedding_launch", status)
     return out
 
 

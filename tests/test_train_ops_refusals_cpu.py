@@ -224,3 +224,20 @@ def test_embedding_gradient_that_overlaps(refusing, accumulate, dtype):
     with pytest.raises(N.KsError) as e:  # the table's rows lie between dout's: on to the check for a device
         call(buf[:n, width:width + dim], as_table(buf[:vocab, :width]))
     assert e.value.status not in (N.KS_ERR_INVALID_ARGS, N.KS_ERR_WORKSPACE)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_embedding_out_that_overlaps(refusing, dtype):
+    """Rows of the table that another warp has yet to read."""
+    N, ops = refusing
+    n, dim, vocab = 40, 32, 100
+    buf = fake(torch.zeros(400, 4 * dim, dtype=dtype))
+    tokens = fake(torch.zeros(n, dtype=torch.int64))
+    table = buf[:vocab, dim:2 * dim]
+    for out in (table[:n], buf[vocab - 1:vocab - 1 + n, dim:2 * dim], buf[:n, 1:dim + 1], buf[:n, 2 * dim - 1:3 * dim - 1]):
+        with pytest.raises(ValueError, match="out overlaps table"):
+            ops.embedding(tokens, table, out=out)
+    for out in (buf[:n, :dim], buf[:n, 2 * dim:3 * dim], buf[vocab:vocab + n, dim:2 * dim]):  # on to the check for a device
+        with pytest.raises(N.KsError) as e:
+            ops.embedding(tokens, table, out=out)
+        assert e.value.status != N.KS_ERR_INVALID_ARGS
