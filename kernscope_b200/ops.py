@@ -276,6 +276,14 @@ def _values(name, t, dtype, n: int, dev: int) -> int:
                      f"{t.dtype} {tuple(t.shape)}, {t.device})")
 
 
+def _scratch(workspace, dev: int) -> tuple[int, int]:
+    """(address, bytes) of a caller's workspace: any type, contiguous, on device `dev`."""
+    if workspace.get_device() == dev and workspace.is_contiguous():
+        return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    raise ValueError(f"workspace must be a contiguous tensor on the current CUDA device (got {tuple(workspace.shape)}, "
+                     f"strides {workspace.stride()}, {workspace.device})")
+
+
 def _name_overlap(outputs: int, **memory) -> None:
     """After a launch that was refused for its arguments: a ValueError where one of
     the first `outputs` tensors shares memory with another.  memory: (address, rows,
@@ -337,7 +345,7 @@ def _linear_ce_run(a, cfg, workspace, like, stream):
         workspace = _empty(like, size, torch.uint8, stream)
         a.workspace, a.workspace_bytes = workspace.data_ptr(), size
     else:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        a.workspace, a.workspace_bytes = _scratch(workspace, like.get_device())
     status = N.lib.ks_linear_ce_launch(C.byref(cfg or _CE_DEFAULT), C.byref(a), _raw_stream(stream, like.get_device()))
     if status == N.KS_ERR_INVALID_ARGS:
         n, row = a.tokens, a.dim * 2
@@ -490,7 +498,7 @@ def embedding_backward(tokens, dout, vocab: int, scale: float = 1.0, padding_idx
         workspace = _empty(dout, size, torch.uint8, stream)
         args.workspace, args.workspace_bytes = workspace.data_ptr(), size
     else:
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        args.workspace, args.workspace_bytes = _scratch(workspace, dev)
     status = N.lib.ks_embedding_grad_launch(C.byref(cfg), C.byref(args), _raw_stream(stream, dev))
     if status == N.KS_ERR_INVALID_ARGS:
         size, out_size = dout.element_size(), dtable.element_size()

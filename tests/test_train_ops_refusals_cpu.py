@@ -241,3 +241,32 @@ def test_embedding_out_that_overlaps(refusing, dtype):
         with pytest.raises(N.KsError) as e:
             ops.embedding(tokens, table, out=out)
         assert e.value.status != N.KS_ERR_INVALID_ARGS
+
+
+BAD_WORKSPACES = {"in host memory": lambda: torch.zeros(1 << 20, dtype=torch.uint8),
+                  "every other byte": lambda: fake(torch.zeros(1 << 21, dtype=torch.uint8))[::2],
+                  "columns of a matrix": lambda: fake(torch.zeros(1024, 2048, dtype=torch.uint8))[:, :1024]}
+
+
+@pytest.mark.parametrize("kind", BAD_WORKSPACES, ids=str)
+def test_workspace_that_kernels_cannot_use(front, kind):
+    """A host address, or bytes between which lie another tensor's."""
+    N, ops, rec = front
+    ws = BAD_WORKSPACES[kind]()
+    h, w, t = fake(torch.zeros(8, 64).bfloat16()), fake(torch.zeros(100, 64).bfloat16()), fake(torch.zeros(8, dtype=torch.int64))
+    for call in (lambda: ops.linear_cross_entropy(h, w, t, workspace=ws),
+                 lambda: ops.linear_cross_entropy_grad(h, w, t, workspace=ws),
+                 lambda: ops.linear_cross_entropy_backward(h, w, t, fake(torch.zeros(8)), workspace=ws),
+                 lambda: ops.embedding_backward(t, h, 100, workspace=ws)):
+        with pytest.raises(ValueError, match="workspace"):
+            call()
+    assert not rec.calls
+
+
+def test_workspace_of_any_type(front):
+    N, ops, rec = front
+    h, t = fake(torch.zeros(8, 64).bfloat16()), fake(torch.zeros(8, dtype=torch.int64))
+    ws = fake(torch.zeros(1 << 10, 1 << 8))
+    ops.embedding_backward(t, h, 100, workspace=ws)
+    (_, a), = rec.calls
+    assert (a.workspace, a.workspace_bytes) == (ws.data_ptr(), 1 << 20)
