@@ -518,7 +518,9 @@ class GradClipper:
     a new clipper when gradients move.  ``clip(max_norm)`` enqueues both passes
     and returns the norm before clipping (fp32, one value, on the device).  The
     partial sums live in the clipper: calls of one clipper must not overlap on
-    the GPU (as calls that scale the same gradients must not).
+    the GPU (as calls that scale the same gradients must not).  A clipper may be
+    dropped while its calls still run, on whatever stream; one whose calls were
+    captured in a CUDA graph has to live as long as the graph.
     """
 
     def __init__(self, grads, out=None):
@@ -553,6 +555,7 @@ class GradClipper:
         self._table = host.to(self.device)
         self._scratch = torch.empty(need.value, dtype=torch.uint8, device=self.device)
         self._index = self.device.index
+        self._streams = {_raw_stream(None, self._index)}  # whose pool the table and the scratch come from
         self._args = N.GradClipArgs(self._table.data_ptr(), chunks.value, 0.0, 0.0, None, self._scratch.data_ptr(),
                                     need.value)
 
@@ -560,9 +563,17 @@ class GradClipper:
         if self._index != torch.cuda.current_device():
             raise ValueError(f"the gradients are on {self.device}, not on the current device")
         norm = _empty(self._scratch, 1, torch.float32, stream)
+        raw = _raw_stream(stream, self._index)
+        if raw not in self._streams:
+            # the clipper may be dropped with this call still queued there, and what it alone
+            # keeps alive must not be given to another tensor before
+            user = torch.cuda.current_stream(self.device) if stream is None else stream
+            for t in (self._table, self._scratch, *self.grads, *self.out):
+                t.record_stream(user)
+            self._streams.add(raw)
         args = self._args
         args.max_norm, args.eps, args.norm = max_norm, eps, norm.data_ptr()
-        N.check("ks_grad_clip_launch", N.lib.ks_grad_clip_launch(C.byref(args), _raw_stream(stream, self._index)))
+        N.check("ks_grad_clip_launch", N.lib.ks_grad_clip_launch(C.byref(args), raw))
         return norm
 
 

@@ -270,3 +270,36 @@ def test_workspace_of_any_type(front):
     ops.embedding_backward(t, h, 100, workspace=ws)
     (_, a), = rec.calls
     assert (a.workspace, a.workspace_bytes) == (ws.data_ptr(), 1 << 20)
+
+
+class Stream:
+    def __init__(self, raw):
+        self.cuda_stream = raw
+
+
+@pytest.fixture
+def clipping(front, monkeypatch):
+    """Host memory for what a clipper allocates on the GPU."""
+    N, ops, rec = front
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **k: fake(empty(*a, **k)))
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, *a, **k: fake(self))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(0))
+    return ops, rec
+
+
+def test_clipper_keeps_its_memory_for_the_stream_it_ran_on(clipping):
+    """The table and the scratch come from the pool of the stream that was current when
+    the clipper was made; after a call on another stream, dropping the clipper (and
+    with it the last reference to a gradient) must not free them for reuse there."""
+    ops, rec = clipping
+    grads, outs = [fake(torch.ones(n)) for n in (100, 7)], [fake(torch.ones(n)) for n in (100, 7)]
+    clipper = ops.GradClipper(grads, out=outs)
+    clipper.clip(1.0)
+    assert not FakeCuda.recorded  # its own stream
+    clipper.clip(1.0, stream=Stream(7))
+    mine = {a.table for _, a in rec.calls} | {a.workspace for _, a in rec.calls}
+    assert len(mine) == 2
+    assert {(p, 7) for p in mine | {t.data_ptr() for t in grads + outs}} == set(FakeCuda.recorded)
+    clipper.clip(1.0, stream=Stream(9))
+    assert {p for p, s in FakeCuda.recorded if s == 9} == {p for p, s in FakeCuda.recorded if s == 7}
