@@ -303,3 +303,39 @@ def test_clipper_keeps_its_memory_for_the_stream_it_ran_on(clipping):
     assert {(p, 7) for p in mine | {t.data_ptr() for t in grads + outs}} == set(FakeCuda.recorded)
     clipper.clip(1.0, stream=Stream(9))
     assert {p for p, s in FakeCuda.recorded if s == 9} == {p for p, s in FakeCuda.recorded if s == 7}
+
+
+def test_clipper_calls_have_arguments_of_their_own(clipping, monkeypatch):
+    """Two host threads in clip() at once: each launch has its own limit and leaves
+    its norm where its own caller looks."""
+    import threading
+
+    ops, rec = clipping
+    clipper = ops.GradClipper([fake(torch.ones(100))])
+    both = threading.Barrier(2, timeout=20)
+    raw, returned, failed = ops._raw_stream, {}, []
+
+    def meet(stream, dev):  # each thread fetches its stream while the other is in clip() too
+        both.wait()
+        return raw(stream, dev)
+
+    def launch(args, stream):
+        both.wait()  # both have filled their arguments
+        a = args._obj
+        rec.calls.append((a.max_norm, a.norm))
+        return 0
+
+    def call(limit):
+        try:
+            returned[limit] = clipper.clip(limit).data_ptr()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    monkeypatch.setattr(ops, "_raw_stream", meet)
+    monkeypatch.setattr(rec, "ks_grad_clip_launch", launch, raising=False)
+    threads = [threading.Thread(target=call, args=(limit,)) for limit in (1.0, 2.0)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and sorted(rec.calls) == sorted((k, p) for k, p in returned.items())
