@@ -339,3 +339,26 @@ def test_clipper_calls_have_arguments_of_their_own(clipping, monkeypatch):
     for t in threads:
         t.join()
     assert not failed and sorted(rec.calls) == sorted((k, p) for k, p in returned.items())
+
+
+@pytest.mark.parametrize("ce_pass", ["KS_CE_FORWARD", "KS_CE_BACKWARD", "KS_CE_GRAD"])
+@pytest.mark.parametrize("tokens,dim,vocab", [(8192, 4096, 512), (2048, 4096, 1024), (4096, 2048, 4000), (1000, 64, 512),
+                                              (64, 4096, 512), (65, 1001, 257), (333, 1000, 10007), (1, 1, 1)])
+def test_least_workspace_of_the_cross_entropy(refusing, tokens, dim, vocab, ce_pass):
+    """The least size is no more than what a call makes use of under any limit, is
+    accepted, and one byte less is not."""
+    N, ops = refusing
+    cfg = N.LinearCeConfig(0, 0, 0)
+    a = N.LinearCeArgs(1 << 40, 2 << 40, 3 << 40, tokens, dim, vocab, dim, dim, N.KS_BF16, getattr(N, ce_pass), N.KS_CE_SUM, 1.0,
+                       -100, None, 4 << 40, 5 << 40, 6 << 40, 7 << 40, dim, dim, 8 << 40, 0)
+    least, want = C.c_size_t(0), C.c_size_t(0)
+    sizes = set()
+    for limit in (0, 1, 1 << 20, 8 << 20, 64 << 20, 1 << 30, 1 << 40):
+        assert N.lib.ks_linear_ce_workspace_bytes(C.byref(cfg), C.byref(a), limit, C.byref(least), C.byref(want)) == 0
+        assert 0 < least.value <= want.value <= max(limit, least.value)
+        sizes |= {least.value, want.value}
+    for size in sizes:
+        a.workspace_bytes = size
+        assert N.lib.ks_linear_ce_launch(C.byref(cfg), C.byref(a), None) not in (N.KS_ERR_WORKSPACE, N.KS_ERR_INVALID_ARGS)
+    a.workspace_bytes = least.value - 1
+    assert N.lib.ks_linear_ce_launch(C.byref(cfg), C.byref(a), None) == N.KS_ERR_WORKSPACE
