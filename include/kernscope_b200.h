@@ -274,7 +274,9 @@ int ks_flash_attention_launch(const ks_flash_attention_config *cfg,
  * (over the tokens that count; 0 with zero gradients when none does) and
  * KS_CE_SUM: loss and dloss have one.  dloss == NULL stands for ones.
  * g[r] = grad_scale * dloss / (mean: number of tokens that count), and 0 for
- * the tokens that do not count or whose target is out of range.
+ * the tokens that do not count or whose target is out of range.  Their rows of
+ * h, and those whose own dloss is 0, may hold anything, NaN and infinities
+ * included: dh is 0 there, and dw what it is with rows of zeros.
  * The logits are never kept.  A gradient call forms d (16 bits a value) in the
  * workspace, in pieces of the vocabulary, from logits taken a second time;
  * KS_CE_GRAD with a workspace that holds d whole keeps 16-bit exponentials

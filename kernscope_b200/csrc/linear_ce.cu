@@ -78,6 +78,7 @@ struct CeScalars {
   float fscale;  // on every row's f: the range factor of d
   float escale;  // on the accumulators of GRADS
   unsigned int counter;
+  unsigned int foul;  // there is a row in `foul` (below)
 };
 
 // One product: output M x N over kb_total K-blocks of 64.
@@ -114,6 +115,7 @@ struct CeGemm {
   int few;                // tokens <= kFew
   float *lo;              // [kFew] d of the target less its 16-bit value
   uint16_t *d_lo;         // [tokens][d_ld] what the rounding of d left, rounded
+  const uint8_t *foul;    // [rows_p] 1: a row of h without gradient that is not finite
   int64_t d_ld;
   CeScalars *sc;
   int out_f32, accumulate;  // dh goes to fp32 slabs, is added to them
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   ks_pdl_wait();
   if ((MODE == STATS || MODE == STORE) && blockIdx.x == 0 && threadIdx.x == 0)
-    p.sc->counter = 0;  // for the combine kernel that follows
+    p.sc->counter = p.sc->foul = 0;  // for the combine kernel that follows
 
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------ producer
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1 && lane == 0) {
     // ------------------------------------------------------------ MMA issuer
     const uint32_t fmt = p.f16 ? (7u << 7) | (7u << 10) : 0;  // f16 operands: format 0
+    const bool foul = kGrads && __ldcg(&p.sc->foul) != 0;
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -393,6 +396,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     };
+    // dw = d^T h: d of a token without gradient is 0, and 0 * NaN would reach every
+    // row of dw.  Where there are such rows of h, they are zeroed in the stage (a
+    // K-row of a box is 128 bytes, whatever the swizzle does within them) before the
+    // first MMA reads it.  Rows past the tokens are zeros already.
+    auto clean = [&](int st, int kb) {
+      const uint8_t *rows = p.foul + int64_t(p.few ? 0 : kb) * kBK;
+      uint8_t *b = smem + L::b_off + st * L::b_bytes;
+#pragma unroll 1
+      for (int r0 = 0; r0 < kBK; r0 += 16) {
+        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(rows + r0));
+#pragma unroll 1
+        for (int r = 0; r < 16; ++r) {
+          const uint32_t word = r < 8 ? (r < 4 ? v.x : v.y) : (r < 12 ? v.z : v.w);
+          if ((word >> (r % 4 * 8) & 0xff) == 0) continue;
+#pragma unroll 8
+          for (int c = 0; c < BN / 64 * 8; ++c)
+            *reinterpret_cast<uint4 *>(b + c / 8 * kBBox + (r0 + r) * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      ks_fence_proxy_async();
+    };
     for (int i = 0; i < work.count && ok; ++i) {
       const Item x = item_at(p, work, i);
       const bool a_mn = kGrads && x.side;
@@ -412,6 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         ks_tc_fence_after();
+        if (a_mn && foul) clean(stage, kb);
         issue(a_mn, stage, kb == x.kb0, d_tmem, 0, 1);
         if (!rest_free) {
           if (pend + 1 < STAGES && kb + 1 < x.kb1 &&
@@ -607,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 32; ++j)
               if (j == tc) {
                 const float d = __uint_as_float(r[j]) - fr;
-                if (p.few) p.lo[row] = d - round16(d, f16);
+                if (p.few) p.lo[row] = fr == 0.f ? 0.f : d - round16(d, f16);
                 r[j] = __float_as_uint(d);
               }
           }
@@ -714,6 +739,7 @@ struct Combine {
   float *loss, *lse;
   double2 *sums;  // per block (loss, tokens that count)
   CeScalars *sc;
+  uint8_t *foul;  // [tokens] for the gradient, or nullptr
 };
 
 struct RowStats {
@@ -758,6 +784,17 @@ KS_DEV RowStats row_stats(const Combine &a, int64_t row, int lane) {
   r.counts = r.target != a.ignore;
   r.loss = !r.counts ? 0.f : r.valid ? r.lse - r.tdot : __int_as_float(0x7fc00000);
   return r;
+}
+
+// What one thread leaves of a row.  A value of h that is not finite makes every
+// logit of its row infinite or NaN, and so the lse: no look at h is needed.
+KS_DEV void put_row(const Combine &a, int64_t row, const RowStats &r) {
+  a.lse[row] = r.lse;
+  if (a.foul) {
+    const bool foul = !r.valid && !isfinite(r.lse);
+    a.foul[row] = foul;
+    if (foul) a.sc->foul = 1;
+  }
 }
 
 // Block `block` of `blocks` (256 threads) has the sums (l, n), known to thread 0;
@@ -812,7 +849,7 @@ __global__ void __launch_bounds__(256) ce_combine_kernel(const __grid_constant__
   if (row < a.tokens) {
     const RowStats r = row_stats(a, row, lane);
     if (lane == 0) {
-      a.lse[row] = r.lse;
+      put_row(a, row, r);
       if (a.reduction == KS_CE_NONE && a.loss) a.loss[row] = r.loss;
     }
     l = r.loss;
@@ -861,7 +898,7 @@ __global__ void __launch_bounds__(256)
     l2 = r.lse * kLog2e;
     tdot = r.tdot;
     if (blockIdx.y == 0) {
-      if (threadIdx.x == 0) a.lse[row] = r.lse;
+      if (threadIdx.x == 0) put_row(a, row, r);
       reduce_loss(a, r.loss, r.counts, unsigned(row), gridDim.x);
     }
   } else {
@@ -940,21 +977,29 @@ __global__ void __launch_bounds__(256)
 // Gradient scalars of a backward call: mean and sum count the tokens; with a
 // dloss per token its largest magnitude is taken out of d by a power of two,
 // so that fp16 d keeps its range (one block: a few microseconds at 8192 tokens).
+// Rows without gradient whose lse is not finite are noted, as put_row does.
 __global__ void __launch_bounds__(1024)
     ce_scalars_kernel(const int64_t *__restrict__ targets, int64_t tokens, int64_t vocab, int64_t ignore, int reduction,
-                      float grad_scale, const float *__restrict__ dloss, float range, CeScalars *sc) {
+                      float grad_scale, const float *__restrict__ dloss, const float *__restrict__ lse, float range,
+                      CeScalars *sc, uint8_t *foul) {
   __shared__ float shm[32];
   __shared__ double shn[32];
   ks_pdl_release();
   ks_pdl_wait();
   float mx = 0.f;
   double n = 0.0;
+  bool any = false;
   for (int64_t r = threadIdx.x; r < tokens; r += 1024) {
     const int64_t t = targets[r];
-    if (t == ignore) continue;
-    n += 1.0;
-    if (reduction == KS_CE_NONE && dloss && t >= 0 && t < vocab) mx = fmaxf(mx, fabsf(dloss[r]));
+    const bool valid = t != ignore && t >= 0 && t < vocab;
+    const float g = valid && reduction == KS_CE_NONE && dloss ? dloss[r] : float(valid);
+    const bool bad = g == 0.f && !isfinite(lse[r]);
+    foul[r] = bad;
+    any |= bad;
+    if (t != ignore) n += 1.0;
+    if (reduction == KS_CE_NONE && dloss) mx = fmaxf(mx, fabsf(g));
   }
+  any = __syncthreads_or(any);
   mx = ks_warp_max(mx);
   n = ks_warp_sum_f64(n);
   if ((threadIdx.x & 31) == 0) {
@@ -982,6 +1027,7 @@ __global__ void __launch_bounds__(1024)
   }
   sc->fscale = float(f);
   sc->escale = float(g / f);
+  sc->foul = any;
 }
 
 // dh = T(escale * sum of the fp32 slabs), slabs added in order; with few tokens
@@ -1165,6 +1211,7 @@ struct Plan {
   bool store;            // one piece, from STORE's exponentials
   int64_t slab_ld, slab_elems;
   size_t o_d_lo;         // few tokens: the second part of d
+  size_t o_foul;         // [rows_p] rows of h without gradient that are not finite
   size_t o_sc, o_sums, o_part, o_tlogit, o_tdot, o_lo, o_lse, o_h, o_w, o_dh, o_slab, o_dw, o_d;
   size_t fixed, bytes;   // bytes: fixed + the piece's d (and padded dw)
 };
@@ -1231,6 +1278,7 @@ void make_plan(const ks_linear_ce_config &c, const ks_linear_ce_args &a, size_t 
   p.o_tlogit = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_tdot = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_lo = take(bwd ? kFew * 4 : 0);
+  p.o_foul = take(bwd ? size_t(p.rows_p) : 0);
   p.o_lse = take(fwd ? size_t(p.rows_p) * 4 : 0);
   p.o_h = take(p.pack_h ? size_t(a.tokens) * p.ld * 2 : 0);
   p.o_w = take(p.pack_w ? size_t(a.vocab) * p.ld * 2 : 0);
@@ -1371,6 +1419,8 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   g.dim = a.dim;
   g.few = a.tokens <= kFew;
   g.lo = reinterpret_cast<float *>(ws + p.o_lo);
+  auto foul = bwd ? reinterpret_cast<uint8_t *>(ws + p.o_foul) : nullptr;
+  g.foul = foul;
   const int kd = int((a.dim + kBK - 1) / kBK);
   CeMaps maps = {};
   if ((s = map_k(&maps.a[0], a.dtype, h, a.tokens, a.dim, hs, p.g1.tm)) != KS_OK) return s;
@@ -1395,7 +1445,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     }
     if (s != KS_OK) return s;
     comb = Combine{g.part, g.parts, g.tlogit, g.tdot, a.targets, a.tokens, a.vocab, a.ignore_index, a.reduction,
-                   a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc};
+                   a.grad_scale, a.dloss, range, a.loss, lse, reinterpret_cast<double2 *>(ws + p.o_sums), sc, foul};
     if (!combine_in_scale) {
       const unsigned blocks = unsigned((a.tokens + kCombRows - 1) / kCombRows);
       s = ks::launch_kernel(true, ce_combine_kernel, dim3(blocks), dim3(256), 0, st, comb, int(bwd));
@@ -1405,7 +1455,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   if (!bwd) return KS_OK;
   if (!fwd) {
     s = ks::launch_kernel(next, ce_scalars_kernel, dim3(1), dim3(1024), 0, st, a.targets, a.tokens, a.vocab, a.ignore_index,
-                        a.reduction, a.grad_scale, a.dloss, range, sc);
+                        a.reduction, a.grad_scale, a.dloss, lse, range, sc, foul);
     if (s != KS_OK) return s;
   }
   char *d = ws + p.o_d;
