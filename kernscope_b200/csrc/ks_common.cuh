@@ -474,8 +474,8 @@ int symbol_address(const void *symbol, void **out);
 KsWait wait_ctx();
 void set_reason(char *buf, size_t len, const char *fmt, ...);
 
-// Lets `kernel` use `bytes` of dynamic shared memory on the current device.  The
-// runtime is asked once per kernel, device and largest size (defined in
+// Lets `kernel` use `bytes` of dynamic shared memory in the current context.  The
+// runtime is asked once per kernel, context and largest size (defined in
 // runtime.cu).
 int allow_shared(const void *kernel, size_t bytes);
 

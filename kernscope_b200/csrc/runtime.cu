@@ -124,24 +124,41 @@ int sm_count() {
   return n;
 }
 
+// The driver's number of the context current on this thread, which no other
+// context of the process ever has, one made after a reset of the device
+// included; 0 when there is none yet.
+static unsigned long long context_id() {
+  static PFN_cuCtxGetId_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuCtxGetId", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuCtxGetId_v12000>(p);
+  });
+  unsigned long long id = 0;
+  return fn != nullptr && fn(nullptr, &id) == CUDA_SUCCESS ? id : 0;
+}
+
 int allow_shared(const void *kernel, size_t bytes) {
-  struct Entry { const void *kernel; int dev; size_t bytes; };
+  // the attribute belongs to the kernel as loaded in one context
+  struct Entry { const void *kernel; unsigned long long ctx; size_t bytes; };
   static std::vector<Entry> cache;
   static std::mutex mu;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return map_cuda(e);
+  const unsigned long long ctx = context_id();
   std::lock_guard<std::mutex> lk(mu);
   Entry *mine = nullptr;
   for (Entry &x : cache)
-    if (x.kernel == kernel && x.dev == dev) mine = &x;
-  if (mine != nullptr && mine->bytes >= bytes) return KS_OK;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (x.kernel == kernel && x.ctx == ctx) mine = &x;
+  if (ctx != 0 && mine != nullptr && mine->bytes >= bytes) return KS_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
   if (e != cudaSuccess) return map_cuda(e);
+  if (ctx == 0) return KS_OK;
   if (mine != nullptr)
     mine->bytes = bytes;
   else
-    cache.push_back({kernel, dev, bytes});
+    cache.push_back({kernel, ctx, bytes});
   return KS_OK;
 }
 
