@@ -85,7 +85,7 @@ struct CeScalars {
 struct CeSide {
   int M, N;
   int kb_total, splits, kb_split;  // K-splits and K-blocks per split (dh)
-  int group;                       // raster: > 0 groups of M-tiles, < 0 bands of N-tiles
+  int band;                        // raster: N-tiles per band
   int b3d;                         // MN-major B map is (64 columns, K, blocks)
 };
 
@@ -168,24 +168,15 @@ KS_DEV void tma_reduce_add_2d(const CUtensorMap *m, const void *src, int c0, int
                : "memory");
 }
 
-// Work item t of a product -> output tile and K-split; splits outermost, tiles
-// rastered as in matmul.cu (group > 0: groups of M-tiles, M fastest; group < 0:
-// bands of N-tiles, N fastest).
-KS_DEV void work_coords(int t, int num_m, int num_n, int group, int &tm, int &tn, int &split) {
-  const int tiles = num_m * num_n;
+// Work item t of a product -> output tile and K-split; splits outermost, tiles in
+// bands of N-tiles, N fastest within a band's rows.
+KS_DEV void work_coords(int t, int num_m, int num_n, int band, int &tm, int &tn, int &split) {
+  const int tiles = num_m * num_n, size = band * num_m;
   split = t / tiles;
   t -= split * tiles;
-  if (group < 0) {
-    const int band = -group, size = band * num_m;
-    const int b = t / size, first = b * band, bn = min(num_n - first, band), r = t - b * size;
-    tn = first + r % bn;
-    tm = r / bn;
-  } else {
-    const int size = group * num_n;
-    const int g = t / size, first = g * group, gm = min(num_m - first, group), r = t - g * size;
-    tm = first + r % gm;
-    tn = r / gm;
-  }
+  const int b = t / size, first = b * band, bn = min(num_n - first, band), r = t - b * size;
+  tn = first + r % bn;
+  tm = r / bn;
 }
 
 // A CTA's work: items of the first product dealt round robin, then (GRADS) tiles
@@ -224,7 +215,7 @@ KS_DEV Item item_at(const CeGemm &p, const Work<TWO, TM, TN> &w, int i) {
   x.side = TWO && i >= w.first;
   const CeSide &d = p.side[TWO ? x.side : 0];
   const int t = x.side ? w.second + (i - w.first) * w.step : int(blockIdx.x) + i * int(gridDim.x);
-  work_coords(t, (d.M + TM - 1) / TM, (d.N + TN - 1) / TN, d.group, x.tm, x.tn, x.split);
+  work_coords(t, (d.M + TM - 1) / TM, (d.N + TN - 1) / TN, d.band, x.tm, x.tn, x.split);
   x.kb0 = x.split * d.kb_split;
   x.kb1 = min(x.kb0 + d.kb_split, d.kb_total);
   return x;
@@ -1436,7 +1427,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.tdot = reinterpret_cast<float *>(ws + p.o_tdot);
     // STORE: [tokens, whole tiles], the columns past the vocabulary are -inf logits, zeros
     const int64_t wide = up(a.vocab, 256);
-    g.side[0] = CeSide{int(a.tokens), int(p.store ? wide : a.vocab), kd, 1, kd, -8, 0};
+    g.side[0] = CeSide{int(a.tokens), int(p.store ? wide : a.vocab), kd, 1, kd, 8, 0};
     if (p.store) {
       if ((s = map_out(&maps.c[0], a.dtype, ws + p.o_d, a.tokens, wide, wide)) != KS_OK) return s;
       s = launch_tile<STORE>(next, p.g1, maps, g, nullptr, st);
@@ -1473,7 +1464,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
                             dim3(unsigned(a.tokens), cols), dim3(256), 0, st, comb, reinterpret_cast<uint16_t *>(d), vpad,
                             p.g1.tn == 256 ? 7 : 6, g.f16, g.few ? g.lo : nullptr, g.few ? g.d_lo : nullptr);
     } else {
-      g.side[0] = CeSide{int(a.tokens), int(vpad), kd, 1, kd, -8, 0};
+      g.side[0] = CeSide{int(a.tokens), int(vpad), kd, 1, kd, 8, 0};
       g.lse = lse;
       g.dloss = a.reduction == KS_CE_NONE ? a.dloss : nullptr;
       if ((s = map_k(&maps.b[0], a.dtype, wp, vp, a.dim, wst, p.g1.tn)) != KS_OK) return s;
@@ -1485,10 +1476,10 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     const Tile t = p.grads.tile;
     CeMaps mg = {};
     const int kv = int((vp + kBK - 1) / kBK), kt = int((a.tokens + kBK - 1) / kBK), per = int(p.grads.kb_split);
-    g.side[0] = CeSide{int(a.tokens), int(a.dim), kv, (kv + per - 1) / per, per, -16, 0};
+    g.side[0] = CeSide{int(a.tokens), int(a.dim), kv, (kv + per - 1) / per, per, 16, 0};
     // dw: the column tiles of a block of rows side by side, so that whole rows are written at about one time
     const int kd2 = g.few ? 2 : kt;  // few tokens: d and its second part, a K-block each
-    g.side[1] = CeSide{int(vp), int(a.dim), kd2, 1, kd2, -16, 0};
+    g.side[1] = CeSide{int(vp), int(a.dim), kd2, 1, kd2, 16, 0};
     static_assert(kFew <= kBK, "few tokens are one K-block");
     if ((s = map_k(&mg.a[0], a.dtype, d, a.tokens, vp, vpad, t.tm)) != KS_OK) return s;
     if ((s = map_mn(&mg.b[0], a.dtype, wp, vp, a.dim, wst, t.tn, &g.side[0].b3d)) != KS_OK) return s;
