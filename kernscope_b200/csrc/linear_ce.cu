@@ -865,10 +865,18 @@ __global__ void __launch_bounds__(256) ce_combine_kernel(const __grid_constant__
 // [target]).  A CTA takes 8192 columns of one row, 16 KB, a warp 1024 of them,
 // four 16-byte loads a lane in flight.  Reads and writes 2 bytes a value: 537 MB
 // for 4096 x 32768 in 91 to 97 us, 5.5 to 5.9 TB/s, the rate of a copy.
-// COMBINE: up to kCombineRows tokens every warp takes its row's lse from the
-// tiles itself, and the combine kernel is left out (333 x 1000 x 10007: 54.4 ->
-// 51.6 us for the whole call; with many rows the repeated reads cost more).
+// COMBINE: every warp takes its row's lse from the tiles itself, and the combine
+// kernel is left out.  That reads a row's (max, sum) pairs once per warp, so it is
+// a matter of the bytes read again: up to kCombineBytes, and kCombineRows tokens.
+// Whole calls without / with it, us, by those MB: 16 x 1024 x 32000 (1) 67.5 / 65.4,
+// 333 x 1000 x 10007 (3) 54.6 / 52.8, 512 x 512 x 10007 (5) 42.8 / 42.8, 128 x 512 x
+// 32000 (8) 40.1 / 39.5, 333 x 512 x 32768 (22) 62.7 / 60.8, 512 x 512 x 32768 (34)
+// 74.6 / 76.5, 256 x 512 x 65536 (67) 85.6 / 88.2, 128 x 512 x 131072 (134) 114.5 /
+// 119.8, 512 x 512 x 131072 (537) 252 / 298; 64 x 256 x 131072 (67) 80.5 / 78.8 is
+// the one of these on the wrong side.
 constexpr int kCombineRows = 512;
+constexpr int64_t kCombineBytes = 24 << 20;
+constexpr int kScaleCols = 8192;  // columns of a CTA: eight warps
 
 template <bool COMBINE>
 __global__ void __launch_bounds__(256)
@@ -1417,7 +1425,8 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
   if ((s = map_k(&maps.a[0], a.dtype, h, a.tokens, a.dim, hs, p.g1.tm)) != KS_OK) return s;
   float *lse = a.lse;
   Combine comb = {};
-  const bool combine_in_scale = p.store && a.tokens <= kCombineRows;
+  const int64_t again = (up(a.vocab, 256) + kScaleCols - 1) / kScaleCols * 8 * a.tokens * p.n_tiles * sizeof(float2);
+  const bool combine_in_scale = p.store && a.tokens <= kCombineRows && again <= kCombineBytes;
   if (fwd) {
     if (!lse) lse = reinterpret_cast<float *>(ws + p.o_lse);
     if ((s = map_k(&maps.b[0], a.dtype, w, a.vocab, a.dim, wst, p.g1.tn)) != KS_OK) return s;
@@ -1459,7 +1468,7 @@ int run(const ks_linear_ce_args &a, const Plan &p, cudaStream_t st) {
     g.d_ld = vpad;
     // d of the piece: [tokens, vpad], columns past the vocabulary zero
     if (p.store) {
-      const unsigned cols = unsigned(std::min<int64_t>((vpad + 8191) / 8192, 65535));
+      const unsigned cols = unsigned(std::min<int64_t>((vpad + kScaleCols - 1) / kScaleCols, 65535));
       s = ks::launch_kernel(true, combine_in_scale ? ce_scale_kernel<true> : ce_scale_kernel<false>,
                             dim3(unsigned(a.tokens), cols), dim3(256), 0, st, comb, reinterpret_cast<uint16_t *>(d), vpad,
                             p.g1.tn == 256 ? 7 : 6, g.f16, g.few ? g.lo : nullptr, g.few ? g.d_lo : nullptr);
