@@ -277,10 +277,11 @@ int ks_flash_attention_launch(const ks_flash_attention_config *cfg,
  * the tokens that do not count or whose target is out of range.  Their rows of
  * h, and those whose own dloss is 0, may hold anything, NaN and infinities
  * included: dh is 0 there, and dw what it is with rows of zeros.
- * The logits are never kept.  A gradient call forms d (16 bits a value) in the
- * workspace, in pieces of the vocabulary, from logits taken a second time;
- * KS_CE_GRAD with a workspace that holds d whole keeps 16-bit exponentials
- * there in the first pass and saves the second.
+ * KS_CE_FORWARD keeps nothing of the logits' size.  A gradient call forms d (16
+ * bits a value) in the workspace, in pieces of the vocabulary, from logits taken a
+ * second time; KS_CE_GRAD with a workspace that holds d whole (2 bytes for every
+ * token and vocabulary entry) keeps 16-bit exponentials there in the first pass
+ * and saves the second.
  * cfg.tile_m x cfg.tile_n: 0 x 0 = chosen from the sizes for each product,
  * 128 x 128, 128 x 256 or 256 x 256.  cfg.piece: vocabulary columns per piece of the backward pass, a
  * multiple of 256; 0 = as many as the workspace holds.
@@ -323,7 +324,8 @@ int ks_embedding_launch(const ks_embedding_args *args, void *stream);
 /* Gradient of the table: dtable[v,:] = scale * sum over tokens[i] == v of
  * dout[i,:] (added to dtable's values if accumulate != 0; else every row is
  * written, zeros where no token is).  fp32 sums in the order of the positions,
- * one rounding; the same bits every time.  Tokens outside [0, vocab) and
+ * one rounding; the same bits every time.  Of rows that do not begin and end on 16
+ * bytes the granules of 16 that hold them are read, up to 14 bytes beside a row.  Tokens outside [0, vocab) and
  * those equal to padding_idx have no part.  out_dtype: dout's type or fp32.
  * cfg.chunk: sorted positions after which a token's sum is split, 1..1024, 0 =
  * chosen from the sizes.
@@ -347,8 +349,9 @@ int ks_embedding_grad_launch(const ks_embedding_grad_config *cfg, const ks_embed
  * norm = sqrt(sum of g^2 over all tensors) and out = g * min(1, max_norm /
  * (norm + eps)), rounded once, for any number of dense tensors in bf16, fp16
  * and fp32.  out may be the gradient itself (NULL stands for it) but may not
- * overlap another tensor.  Squares are summed in fp32 over at most 32 values,
- * then in fp64; the same bits every time.  A norm that is not finite gives
+ * overlap another tensor.  Squares are taken in fp32 (infinite for values above
+ * 1.8e19, zero below 2.6e-23) and summed in fp32 over at most 34 values, then in
+ * fp64; the same bits every time.  A norm that is not finite gives
  * what the formula gives.  No counterpart in the reference.
  * ks_grad_clip_plan() (host only) writes the table of work for a set of
  * tensors into host memory; `table` NULL asks for its size.  The caller

@@ -159,7 +159,9 @@ KS_DEV double block_sum(double v, double *sh) {
   return sh[0];
 }
 
-// Squares: fp32 within a chunk's share of a thread (at most 32 values), fp64 across.
+// Squares: fp32 within a chunk's share of a thread (at most 34 values: 32 of whole
+// vectors, one before and one after them), fp64 across.  Squares in fp32 bound the values:
+// above 1.8e19 they are infinite, below 2.6e-23 zero.
 __global__ void __launch_bounds__(kThreads) clip_norm_kernel(const Chunk *__restrict__ table, int64_t chunks,
                                                              double *__restrict__ partial) {
   __shared__ double sh[32];

@@ -58,12 +58,11 @@ class VocabModel:
 
 
 def synthetic_text(vocab: int, tokens: int, seed: int, branches: int = 4):
-    """tokens + 1 ids in which each token is followed by one of a few others."""
+    """(tokens, targets): independent pairs of a token and one of its few successors."""
     gen = torch.Generator()
     gen.manual_seed(1)
     after = torch.randint(0, vocab, (vocab, branches), generator=gen)
     gen.manual_seed(seed)
-    # independent pairs: a token and one of its successors
     first = torch.randint(0, vocab, (tokens,), generator=gen)
     second = after[first, torch.randint(0, branches, (tokens,), generator=gen)]
     return first.cuda(), second.cuda()
