@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // teardown: every load this thread issued must have landed before exit
     for (int s = 0; s < STAGES; ++s)
       if (armed & (1u << s)) ks_mbar_wait(full + s, (armed_parity >> s) & 1u, nullptr, wait);
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     const uint32_t fmt = p.f16 ? (7u << 7) | (7u << 10) : 0;  // f16 operands: format 0
     const bool foul = kGrads && __ldcg(&p.sc->foul) != 0;
@@ -400,27 +400,51 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     };
     // dw = d^T h: d of a token without gradient is 0, and 0 * NaN would reach every
-    // row of dw.  Where there are such rows of h, they are zeroed in the stage (a
-    // K-row of a box is 128 bytes, whatever the swizzle does within them) before the
-    // first MMA reads it.  Rows past the tokens are zeros already.
-    auto clean = [&](int st, int kb) {
-      const uint8_t *rows = p.foul + int64_t(p.few ? 0 : kb) * kBK;
-      uint8_t *b = smem + L::b_off + st * L::b_bytes;
-#pragma unroll 1
-      for (int r0 = 0; r0 < kBK; r0 += 16) {
-        const uint4 v = __ldcg(reinterpret_cast<const uint4 *>(rows + r0));
-#pragma unroll 1
-        for (int r = 0; r < 16; ++r) {
-          const uint32_t word = r < 8 ? (r < 4 ? v.x : v.y) : (r < 12 ? v.z : v.w);
-          if ((word >> (r % 4 * 8) & 0xff) == 0) continue;
-#pragma unroll 8
-          for (int c = 0; c < BN / 64 * 8; ++c)
-            *reinterpret_cast<uint4 *>(b + c / 8 * kBBox + (r0 + r) * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+    // row of dw.  Where there are such rows of h, the whole warp zeroes them in the
+    // stage before the first MMA reads it (a K-row of a box is 128 bytes, whatever the
+    // swizzle does within them; rows past the tokens are zeros already).  Without
+    // them one thread is at work, as below.  (4096 x 2048 x 32768 with 5 / 30 % of the
+    // rows NaN 1.41 / 1.68 ms a call, 1.34 / 1.28 with finite values in their place.)
+    for (int i = 0; foul && i < work.count && ok; ++i) {
+      const Item x = item_at(p, work, i);
+      const int acc = i % ACC;
+      for (int h = 0; h < MH && ok; ++h)
+        ok = __all_sync(0xffffffffu, ks_mbar_wait(tempty + acc * MH + h, ((i / ACC) & 1) ^ 1u, abort, wait));
+      ks_tc_fence_after();
+      // lane l: the marks of rows 2 l and 2 l + 1 of a K-block, fetched one ahead
+      auto marks = [&](int kb) {
+        return __ldcg(reinterpret_cast<const uint16_t *>(p.foul + int64_t(p.few ? 0 : min(kb, x.kb1 - 1)) * kBK) + lane);
+      };
+      uint32_t next = x.side ? marks(x.kb0) : 0;
+      for (int kb = x.kb0; kb < x.kb1 && ok; ++kb) {
+        const uint32_t mark = next;
+        if (x.side) next = marks(kb + 1);
+        ok = __all_sync(0xffffffffu, ks_mbar_wait(full + stage, phase, abort, wait));
+        if (!ok) break;
+        if (x.side) {
+          uint8_t *b = smem + L::b_off + stage * L::b_bytes;
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            for (uint32_t m = __ballot_sync(0xffffffffu, mark >> (8 * r) & 0xff); m; m &= m - 1)
+              if (lane < BN / 8)
+                *reinterpret_cast<uint4 *>(b + lane / 8 * kBBox + ((__ffs(m) - 1) * 2 + r) * 128 + lane % 8 * 16) =
+                    make_uint4(0, 0, 0, 0);
+          ks_fence_proxy_async();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          ks_tc_fence_after();
+          issue(x.side != 0, stage, kb == x.kb0, tmem_base + acc * BN * MH, 0, MH);
+          ks_umma_commit(empty + stage);
+        }
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      ks_fence_proxy_async();
-    };
-    for (int i = 0; i < work.count && ok; ++i) {
+      if (ok && lane == 0) ks_umma_commit(tfull + acc);
+    }
+    for (int i = 0; !foul && lane == 0 && i < work.count && ok; ++i) {
       const Item x = item_at(p, work, i);
       const bool a_mn = kGrads && x.side;
       const int acc = i % ACC;
@@ -439,7 +463,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           break;
         }
         ks_tc_fence_after();
-        if (a_mn && foul) clean(stage, kb);
         issue(a_mn, stage, kb == x.kb0, d_tmem, 0, 1);
         if (!rest_free) {
           if (pend + 1 < STAGES && kb + 1 < x.kb1 &&
@@ -472,8 +495,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) ks_umma_commit(tfull + acc);
     }
     // teardown: all MMAs issued by this thread complete before TMEM is freed
-    ks_umma_commit(drain);
-    ks_mbar_wait(drain, 0, nullptr, wait);
+    if (lane == 0) {
+      ks_umma_commit(drain);
+      ks_mbar_wait(drain, 0, nullptr, wait);
+    }
   } else if (warp >= 2) {
     // ------------------------------------------------------------ epilogue
     constexpr int kCols = BN / 2;        // columns of a tile that one warp drains, of each 128-row half
