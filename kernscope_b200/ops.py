@@ -556,7 +556,8 @@ class GradClipper:
         self._scratch = torch.empty(need.value, dtype=torch.uint8, device=self.device)
         self._index = self.device.index
         self._streams = {_raw_stream(None, self._index)}  # whose pool the table and the scratch come from
-        self._chunks = chunks.value
+        self._args = N.GradClipArgs(self._table.data_ptr(), chunks.value, 0.0, 0.0, None, self._scratch.data_ptr(),
+                                    need.value)
 
     def clip(self, max_norm: float, eps: float = 1e-6, stream=None) -> torch.Tensor:
         if self._index != torch.cuda.current_device():
@@ -570,9 +571,8 @@ class GradClipper:
             for t in (self._table, self._scratch, *self.grads, *self.out):
                 t.record_stream(user)
             self._streams.add(raw)
-        # of this call alone: another host thread may be in here too
-        args = N.GradClipArgs(self._table.data_ptr(), self._chunks, max_norm, eps, norm.data_ptr(),
-                              self._scratch.data_ptr(), self._scratch.numel())
+        args = N.GradClipArgs.from_buffer_copy(self._args)  # another host thread may be in here too
+        args.max_norm, args.eps, args.norm = max_norm, eps, norm.data_ptr()
         N.check("ks_grad_clip_launch", N.lib.ks_grad_clip_launch(C.byref(args), raw))
         return norm
 
